@@ -324,6 +324,53 @@ int plx_decode_partial_exchange(const plx_decode_problem *p, const plx_exchange 
                                 const int32_t *seqused_k, const int32_t *cache_start, void *workspace,
                                 size_t workspace_bytes, plx_stream_t stream);
 
+/* ------------------------------------------------------------------------- *
+ * Pages of a paged cache.  (No counterpart in the reference, which names paged caches but
+ * does not implement them.)
+ *
+ * A pool is the k / v of a paged plx_decode_problem: n_pages pages of page_size keys (a power of
+ * two) by ELEMENT strides for (page, key, head), head_dim contiguous, 16-bit elements; k and v
+ * have strides of their own.  A page table (batch x pages_per_seq) and lengths (batch) as there:
+ * the ACTIVE entries of row b are the first ceil(lens[b] / page_size).  A page is live while some
+ * row's active entry names it.  Entries, rows and pages out of range are passed over.  Everything is
+ * device memory, nothing is read by the host.  Results are new tables: they must not overlap the
+ * old ones.  The workspace (plx_pages_workspace_bytes, 16-byte aligned) needs no initial contents;
+ * launches that can overlap must not share one.
+ * ------------------------------------------------------------------------- */
+typedef struct plx_page_pool {
+    void *k, *v;
+    int32_t n_pages, page_size, heads_kv, head_dim;      /* head_dim: a multiple of 8 */
+    int64_t k_stride_p, k_stride_t, k_stride_h;          /* multiples of 8 */
+    int64_t v_stride_p, v_stride_t, v_stride_h;
+} plx_page_pool;
+
+/* Page src[i] of k and of v to page dst[i], i < n.  No page may be a target twice, or a source and a
+ * target (what such a page holds afterwards is not defined). */
+int plx_pages_copy(const plx_page_pool *p, const int32_t *src, const int32_t *dst, int32_t n, plx_stream_t stream);
+
+/* n_forks: the n of plx_pages_fork; 0 for the other two */
+int plx_pages_workspace_bytes(int32_t n_pages, int32_t batch, int32_t n_forks, size_t *bytes);
+
+/* Row children[i] becomes row parents[i] (as it was before the call), i < n; of a row mentioned twice among the
+ * children the last one counts.  Whole pages are shared; the keys of a last page that is not full are copied to a page of
+ * its own, the lowest that was not live before the call, in the order of the lists.  `missing` (one int): rows for which there
+ * was none; they end with their whole pages. */
+int plx_pages_fork(const plx_page_pool *p, const int32_t *page_table, const int32_t *lens, int32_t batch, int32_t pages_per_seq,
+                   const int32_t *parents, const int32_t *children, int32_t n, int32_t *new_page_table, int32_t *new_lens,
+                   int32_t *missing, void *workspace, size_t workspace_bytes, plx_stream_t stream);
+
+/* Moves the live pages to the front: of n live pages, the i-th from page n on goes to the i-th free page below n.
+ * `n_live` (one int) is n; the pages from n on are free. */
+int plx_pages_compact(const plx_page_pool *p, const int32_t *page_table, const int32_t *lens, int32_t batch,
+                      int32_t pages_per_seq, int32_t *new_page_table, int32_t *n_live, void *workspace,
+                      size_t workspace_bytes, plx_stream_t stream);
+
+/* Lengths with those of `rows` 0, and the pages that are not live then, ascending: free_list (n_pages ints; -1 behind
+ * the last), n_free (one int). */
+int plx_pages_free(const int32_t *page_table, const int32_t *lens, int32_t batch, int32_t pages_per_seq, const int32_t *rows,
+                   int32_t n_rows, int32_t n_pages, int32_t page_size, int32_t *new_lens, int32_t *free_list, int32_t *n_free,
+                   void *workspace, size_t workspace_bytes, plx_stream_t stream);
+
 /* ------------------------------------------------------------------------- */
 int plx_abi_version(void);
 const char *plx_strerror(int status);

@@ -8,6 +8,8 @@ ABI.  ``parallax.triton`` and ``parallax.cute`` mirror the reference's
 sub-packages for code that imports the decode front ends from there
 (``parallax/triton/__init__.py:8``, ``parallax/cute/__init__.py``).
 
+What this build adds to the reference (the pages of a paged cache among it) goes by names of its own.
+
 ``parallax_reference`` (the fp32 PyTorch implementation, ``parallax/reference.py``
 upstream) is deliberately absent: this package has no CPU path, and a name that
 silently computed on the CPU would defeat that.  Accessing it raises an
@@ -19,7 +21,11 @@ from parallax_b200 import (
     cute_decode_available,
     parallax_attn_with_kvcache,
     parallax_bwd,
+    parallax_compact_pages,
+    parallax_copy_pages,
     parallax_decode,
+    parallax_fork_pages,
+    parallax_free_pages,
     parallax_func,
     parallax_fwd,
     parallax_varlen_func,
@@ -34,6 +40,10 @@ __all__ = [
     "parallax_attn_with_kvcache",
     "parallax_decode",
     "GraphedDecode",
+    "parallax_copy_pages",
+    "parallax_fork_pages",
+    "parallax_compact_pages",
+    "parallax_free_pages",
     "cute_decode_available",
 ]
 

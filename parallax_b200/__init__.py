@@ -11,6 +11,7 @@ reference.  All device work runs in ``lib/libplx_sm100.so`` (build it with
 ``python -m parallax_b200.build``); there is no Triton, PyTorch or CPU fallback.
 """
 from .decode import GraphedDecode, parallax_attn_with_kvcache, parallax_decode
+from .pages import parallax_compact_pages, parallax_copy_pages, parallax_fork_pages, parallax_free_pages
 from .train import parallax_bwd, parallax_func, parallax_fwd
 from .varlen import parallax_varlen_func
 
@@ -31,5 +32,9 @@ __all__ = [
     "parallax_attn_with_kvcache",
     "parallax_decode",
     "GraphedDecode",
+    "parallax_copy_pages",
+    "parallax_fork_pages",
+    "parallax_compact_pages",
+    "parallax_free_pages",
     "cute_decode_available",
 ]

@@ -25,6 +25,7 @@ SYMBOLS = (
     "plx_train_workspace_bytes", "plx_train_fwd", "plx_train_extend", "plx_train_bwd", "plx_train_bwd_stages",
     "plx_decode_choose_splits", "plx_decode_choose_splits_gqa", "plx_decode_workspace_bytes", "plx_decode_stage", "plx_decode_step", "plx_decode", "plx_decode_static", "plx_decode_partial",
     "plx_decode_merge", "plx_decode_exchange_bytes", "plx_decode_exchange_merge", "plx_decode_partial_exchange",
+    "plx_pages_copy", "plx_pages_workspace_bytes", "plx_pages_fork", "plx_pages_compact", "plx_pages_free",
 )
 EXCHANGE_MAX_RANKS = 16
 
@@ -56,6 +57,15 @@ class Exchange(C.Structure):
         ("world", C.c_int32), ("rank", C.c_int32), ("n_records", C.c_int32), ("head_dim", C.c_int32),
         ("dtype", C.c_int32), ("wait_ms", C.c_uint32), ("status", C.c_void_p),
         ("inbox", C.c_void_p * EXCHANGE_MAX_RANKS),
+    ]
+
+
+class PagePool(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p),
+        ("n_pages", C.c_int32), ("page_size", C.c_int32), ("heads_kv", C.c_int32), ("head_dim", C.c_int32),
+        ("k_stride_p", C.c_int64), ("k_stride_t", C.c_int64), ("k_stride_h", C.c_int64),
+        ("v_stride_p", C.c_int64), ("v_stride_t", C.c_int64), ("v_stride_h", C.c_int64),
     ]
 
 
@@ -117,6 +127,17 @@ def _declare(lib):
     lib.plx_decode_exchange_merge.argtypes = [C.POINTER(Exchange), vp, vp, vp]
     lib.plx_decode_partial_exchange.restype = C.c_int
     lib.plx_decode_partial_exchange.argtypes = [C.POINTER(DecodeProblem), C.POINTER(Exchange)] + [vp] * 7 + [vp, sz, vp]
+    pool = C.POINTER(PagePool)
+    lib.plx_pages_copy.restype = C.c_int
+    lib.plx_pages_copy.argtypes = [pool, vp, vp, i32, vp]
+    lib.plx_pages_workspace_bytes.restype = C.c_int
+    lib.plx_pages_workspace_bytes.argtypes = [i32, i32, i32, C.POINTER(sz)]
+    lib.plx_pages_fork.restype = C.c_int
+    lib.plx_pages_fork.argtypes = [pool, vp, vp, i32, i32, vp, vp, i32, vp, vp, vp, vp, sz, vp]
+    lib.plx_pages_compact.restype = C.c_int
+    lib.plx_pages_compact.argtypes = [pool, vp, vp, i32, i32, vp, vp, vp, sz, vp]
+    lib.plx_pages_free.restype = C.c_int
+    lib.plx_pages_free.argtypes = [vp, vp, i32, i32, vp, i32, i32, i32, vp, vp, vp, vp, sz, vp]
 
 
 def lib():

@@ -12,7 +12,7 @@ static std::atomic<uint64_t> g_launches{0};
 void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
 
 // The kernels are built for sm_100a only; anything else must fail loudly, not fall back.
-static int check_device() {
+int check_device() {
     static std::atomic<int> cached[64];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return PLX_ERR_DEVICE;
@@ -515,6 +515,36 @@ int plx_decode_exchange_merge(const plx_exchange *x, const float *part, void *ou
     const ErrorWords err = sm100_error_words();
     if (!err.word) return PLX_ERR_LAUNCH;
     return launch_decode_exchange_merge(e, part, x->head_dim, x->dtype, out, err, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int plx_pages_copy(const plx_page_pool *p, const int32_t *src, const int32_t *dst, int32_t n, plx_stream_t stream) {
+    return launch_pages_copy(p, src, dst, n, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int plx_pages_workspace_bytes(int32_t n_pages, int32_t batch, int32_t n_forks, size_t *bytes) {
+    if (n_pages <= 0 || batch <= 0 || n_forks < 0 || !bytes) return PLX_ERR_BAD_ARG;
+    *bytes = pages_workspace_bytes(n_pages, batch, n_forks);
+    return PLX_OK;
+}
+
+int plx_pages_fork(const plx_page_pool *p, const int32_t *page_table, const int32_t *lens, int32_t batch, int32_t pages_per_seq,
+                   const int32_t *parents, const int32_t *children, int32_t n, int32_t *new_page_table, int32_t *new_lens,
+                   int32_t *missing, void *workspace, size_t workspace_bytes, plx_stream_t stream) {
+    return launch_pages_fork(p, page_table, lens, batch, pages_per_seq, parents, children, n, new_page_table, new_lens, missing,
+           workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int plx_pages_compact(const plx_page_pool *p, const int32_t *page_table, const int32_t *lens, int32_t batch, int32_t pages_per_seq,
+                      int32_t *new_page_table, int32_t *n_live, void *workspace, size_t workspace_bytes, plx_stream_t stream) {
+    return launch_pages_compact(p, page_table, lens, batch, pages_per_seq, new_page_table, n_live, workspace, workspace_bytes,
+           reinterpret_cast<cudaStream_t>(stream));
+}
+
+int plx_pages_free(const int32_t *page_table, const int32_t *lens, int32_t batch, int32_t pages_per_seq, const int32_t *rows, int32_t n_rows,
+                   int32_t n_pages, int32_t page_size, int32_t *new_lens, int32_t *free_list, int32_t *n_free, void *workspace,
+                   size_t workspace_bytes, plx_stream_t stream) {
+    return launch_pages_free(page_table, lens, batch, pages_per_seq, rows, n_rows, n_pages, page_size, new_lens, free_list, n_free,
+           workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -3,6 +3,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "../../include/plx_abi.h"
+
 namespace plx {
 
 struct TrainArgs;
@@ -36,6 +38,9 @@ inline int item_group(int n_bh, int n_tiles, int sms) {
 // plx_kernel_launch_count() can report how many ran.
 void count_launch();
 
+// PLX_OK where the current device is an sm_100 one
+int check_device();
+
 int launch_train_fwd_mma(const TrainArgs &a, int dtype, int head_dim, cudaStream_t stream);
 int launch_train_bwd_mma(const TrainArgs &a, int dtype, int head_dim, int stages, cudaStream_t stream);
 
@@ -68,5 +73,16 @@ int launch_decode_stage(void *q, const void *q_src, void *r, const void *r_src, 
                         cudaStream_t stream);
 int launch_decode_merge(const float *parts, int n_parts, int n_records, int head_dim, int dtype, void *out,
                         cudaStream_t stream);
+
+// pages of a cache (see plx_pages.cu)
+int launch_pages_copy(const plx_page_pool *p, const int32_t *src, const int32_t *dst, int n, cudaStream_t stream);
+size_t pages_workspace_bytes(int n_pages, int batch, int n_forks);
+int launch_pages_fork(const plx_page_pool *p, const int32_t *table, const int32_t *lens, int batch, int pages_per_seq, const int32_t *parents,
+                      const int32_t *children, int n, int32_t *new_table, int32_t *new_lens, int32_t *missing, void *ws, size_t ws_bytes,
+                      cudaStream_t stream);
+int launch_pages_compact(const plx_page_pool *p, const int32_t *table, const int32_t *lens, int batch, int pages_per_seq, int32_t *new_table, int32_t *n_live,
+                         void *ws, size_t ws_bytes, cudaStream_t stream);
+int launch_pages_free(const int32_t *table, const int32_t *lens, int batch, int pages_per_seq, const int32_t *rows, int n_rows, int n_pages, int page_size,
+                      int32_t *new_lens, int32_t *free_list, int32_t *n_free, void *ws, size_t ws_bytes, cudaStream_t stream);
 
 }  // namespace plx
