@@ -134,6 +134,23 @@ int plx_train_bwd_stages(const plx_train_problem *p, int32_t stages, const void 
                          void *dq, void *dr, void *dk, void *dv, void *workspace,
                          size_t workspace_bytes, plx_stream_t stream);
 
+/* The same with SINKS: the first sink_tokens keys of every sequence (of every batch row; with packed input of
+ * every packed sequence) stay visible to all rows from them on behind the sliding window:
+ *     key j is visible iff j <= pos and (j >= pos - window_left + 1 or j < sink_tokens).
+ * 0, or no window, is the call without.  With sinks window_left may be 0 for tensor-core kernels too (nothing but sinks is
+ * seen).  plx_train_bwd_sink needs plx_train_workspace_bytes_sink() bytes, and the forward's outputs with the same
+ * sink_tokens.  (No counterpart in the reference.) */
+int plx_train_workspace_bytes_sink(const plx_train_problem *p, int32_t sink_tokens, size_t *bytes);
+int plx_train_fwd_sink(const plx_train_problem *p, int32_t sink_tokens, const void *q, const void *r, const void *k,
+                       const void *v, void *o, void *barv, float *d1, float *bart, float *m, plx_stream_t stream);
+int plx_train_extend_sink(const plx_train_problem *p, int32_t sink_tokens, const void *q, const void *r, const void *k,
+                          const void *v, void *o, const int32_t *seqused_k, const int32_t *page_table, int32_t page_size,
+                          int32_t pages_per_seq, int32_t n_pages, plx_stream_t stream);
+int plx_train_bwd_sink(const plx_train_problem *p, int32_t sink_tokens, const void *q, const void *r, const void *k,
+                       const void *v, const void *o, const void *barv, const float *d1, const float *bart, const float *m,
+                       const void *grad_o, void *dq, void *dr, void *dk, void *dv, void *workspace, size_t workspace_bytes,
+                       plx_stream_t stream);
+
 /* ------------------------------------------------------------------------- *
  * Decode: one query token per sequence against a KV cache.
  *
@@ -238,6 +255,37 @@ int plx_decode_step(const plx_decode_problem *p, void *q, const void *q_src, voi
 int plx_decode(const plx_decode_problem *p, const void *q, const void *r, const void *k,
                const void *v, void *out, const int32_t *seqused_k, const int32_t *cache_start,
                void *workspace, size_t workspace_bytes, plx_stream_t stream);
+
+/* plx_decode and plx_decode_step with SINKS: the first sink_tokens keys of a row, from its first valid one (cache_start) on, stay
+ * visible behind the sliding window.  0, or no window, is the call without.  Not for a key-sharded cache (kv_offset).  Split count
+ * and workspace: those of window_left + sink_tokens keys.  (No counterpart in the reference.) */
+int plx_decode_sink(const plx_decode_problem *p, int32_t sink_tokens, const void *q, const void *r, const void *k,
+                    const void *v, void *out, const int32_t *seqused_k, const int32_t *cache_start, void *workspace,
+                    size_t workspace_bytes, plx_stream_t stream);
+int plx_decode_step_sink(const plx_decode_problem *p, int32_t sink_tokens, void *q, const void *q_src, void *r,
+                         const void *r_src, const void *k, const void *v, void *out, int32_t *seqused_k,
+                         const int32_t *seqused_src, void *workspace, size_t workspace_bytes, plx_stream_t stream);
+
+/* plx_decode for a batch whose rows all begin with the same `len` keys, which are read once for all of them.  The prefix
+ * is either keys of its own, (len, heads_kv, head_dim) by the element strides (token, head) of k / v -- `p` then describes what
+ * follows it, and lengths (seqused_k, 0 to cache_len, NULL: cache_len) count that -- or, with k and v NULL, the first len keys of the paged
+ * cache of `p` itself: every row's page table begins with the same pages, len is a multiple of the page size, and lengths count
+ * the prefix too (shorter ones count as len).  Only the first row's entries of it are read.  No sliding window, no kv_offset.
+ * The q heads of a kv head of all rows are the M dimension of tensor-core products over the prefix, whose keys are cut into
+ * n_splits parts (plx_decode_prefix_splits); each row's own keys are a plx_decode_partial, and a third launch merges.
+ * Workspace: plx_decode_prefix_workspace_bytes(), ZERO-FILLED ONCE like that of plx_decode.  (No counterpart in the reference.) */
+#define PLX_PREFIX_MAX_SPLITS 31
+typedef struct plx_prefix {
+    const void *k, *v;
+    int64_t stride_t, stride_h;
+    int32_t len;
+    int32_t n_splits;
+} plx_prefix;
+int plx_decode_prefix_splits(int32_t batch, int32_t heads_q, int32_t heads_kv, int32_t len, int32_t sm_count);
+int plx_decode_prefix_workspace_bytes(const plx_decode_problem *p, const plx_prefix *x, size_t *bytes);
+int plx_decode_prefix(const plx_decode_problem *p, const plx_prefix *x, const void *q, const void *r, const void *k,
+                      const void *v, void *out, const int32_t *seqused_k, void *workspace, size_t workspace_bytes,
+                      plx_stream_t stream);
 
 /* plx_decode for callers that cannot allocate device memory.  (No counterpart in
  * the reference: upstream always allocates its split-KV workspace with torch.)

@@ -24,6 +24,7 @@ from parallax_b200 import (
     parallax_compact_pages,
     parallax_copy_pages,
     parallax_decode,
+    parallax_decode_shared_prefix,
     parallax_fork_pages,
     parallax_free_pages,
     parallax_func,
@@ -40,6 +41,7 @@ __all__ = [
     "parallax_attn_with_kvcache",
     "parallax_decode",
     "GraphedDecode",
+    "parallax_decode_shared_prefix",
     "parallax_copy_pages",
     "parallax_fork_pages",
     "parallax_compact_pages",

@@ -10,7 +10,7 @@ Same names and argument meaning as ``parallax/__init__.py:84-95`` of the
 reference.  All device work runs in ``lib/libplx_sm100.so`` (build it with
 ``python -m parallax_b200.build``); there is no Triton, PyTorch or CPU fallback.
 """
-from .decode import GraphedDecode, parallax_attn_with_kvcache, parallax_decode
+from .decode import GraphedDecode, parallax_attn_with_kvcache, parallax_decode, parallax_decode_shared_prefix
 from .pages import parallax_compact_pages, parallax_copy_pages, parallax_fork_pages, parallax_free_pages
 from .train import parallax_bwd, parallax_func, parallax_fwd
 from .varlen import parallax_varlen_func
@@ -32,6 +32,7 @@ __all__ = [
     "parallax_attn_with_kvcache",
     "parallax_decode",
     "GraphedDecode",
+    "parallax_decode_shared_prefix",
     "parallax_copy_pages",
     "parallax_fork_pages",
     "parallax_compact_pages",

@@ -25,6 +25,8 @@ SYMBOLS = (
     "plx_train_workspace_bytes", "plx_train_fwd", "plx_train_extend", "plx_train_bwd", "plx_train_bwd_stages",
     "plx_decode_choose_splits", "plx_decode_choose_splits_gqa", "plx_decode_workspace_bytes", "plx_decode_stage", "plx_decode_step", "plx_decode", "plx_decode_static", "plx_decode_partial",
     "plx_decode_merge", "plx_decode_exchange_bytes", "plx_decode_exchange_merge", "plx_decode_partial_exchange",
+    "plx_train_workspace_bytes_sink", "plx_train_fwd_sink", "plx_train_extend_sink", "plx_train_bwd_sink",
+    "plx_decode_sink", "plx_decode_step_sink", "plx_decode_prefix_splits", "plx_decode_prefix_workspace_bytes", "plx_decode_prefix",
     "plx_pages_copy", "plx_pages_workspace_bytes", "plx_pages_fork", "plx_pages_compact", "plx_pages_free",
 )
 EXCHANGE_MAX_RANKS = 16
@@ -57,6 +59,12 @@ class Exchange(C.Structure):
         ("world", C.c_int32), ("rank", C.c_int32), ("n_records", C.c_int32), ("head_dim", C.c_int32),
         ("dtype", C.c_int32), ("wait_ms", C.c_uint32), ("status", C.c_void_p),
         ("inbox", C.c_void_p * EXCHANGE_MAX_RANKS),
+    ]
+
+
+class Prefix(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("stride_t", C.c_int64), ("stride_h", C.c_int64), ("len", C.c_int32), ("n_splits", C.c_int32),
     ]
 
 
@@ -127,7 +135,25 @@ def _declare(lib):
     lib.plx_decode_exchange_merge.argtypes = [C.POINTER(Exchange), vp, vp, vp]
     lib.plx_decode_partial_exchange.restype = C.c_int
     lib.plx_decode_partial_exchange.argtypes = [C.POINTER(DecodeProblem), C.POINTER(Exchange)] + [vp] * 7 + [vp, sz, vp]
-    pool = C.POINTER(PagePool)
+    train, decode, prefix, pool = C.POINTER(TrainProblem), C.POINTER(DecodeProblem), C.POINTER(Prefix), C.POINTER(PagePool)
+    lib.plx_train_workspace_bytes_sink.restype = C.c_int
+    lib.plx_train_workspace_bytes_sink.argtypes = [train, i32, C.POINTER(sz)]
+    lib.plx_train_fwd_sink.restype = C.c_int
+    lib.plx_train_fwd_sink.argtypes = [train, i32] + [vp] * 9 + [vp]
+    lib.plx_train_extend_sink.restype = C.c_int
+    lib.plx_train_extend_sink.argtypes = [train, i32] + [vp] * 7 + [i32, i32, i32, vp]
+    lib.plx_train_bwd_sink.restype = C.c_int
+    lib.plx_train_bwd_sink.argtypes = [train, i32] + [vp] * 14 + [vp, sz, vp]
+    lib.plx_decode_sink.restype = C.c_int
+    lib.plx_decode_sink.argtypes = [decode, i32] + [vp] * 7 + [vp, sz, vp]
+    lib.plx_decode_step_sink.restype = C.c_int
+    lib.plx_decode_step_sink.argtypes = [decode, i32] + [vp] * 9 + [vp, sz, vp]
+    lib.plx_decode_prefix_splits.restype = C.c_int
+    lib.plx_decode_prefix_splits.argtypes = [i32, i32, i32, i32, i32]
+    lib.plx_decode_prefix_workspace_bytes.restype = C.c_int
+    lib.plx_decode_prefix_workspace_bytes.argtypes = [decode, prefix, C.POINTER(sz)]
+    lib.plx_decode_prefix.restype = C.c_int
+    lib.plx_decode_prefix.argtypes = [decode, prefix] + [vp] * 6 + [vp, sz, vp]
     lib.plx_pages_copy.restype = C.c_int
     lib.plx_pages_copy.argtypes = [pool, vp, vp, i32, vp]
     lib.plx_pages_workspace_bytes.restype = C.c_int

@@ -83,6 +83,20 @@ static size_t train_ws_bytes(const plx_train_problem *p) {
     return train_stat_rows(p) * 12 * sizeof(float);
 }
 
+// Sinks of a problem into its arguments; none where no window hides a key.
+static void set_sinks(TrainArgs &a, int32_t sink_tokens) {
+    if (sink_tokens <= 0 || a.window < 0 || a.window >= a.len_k) return;
+    a.sink = sink_tokens < a.len_k ? sink_tokens : a.len_k;
+    a.sink_chunk = train_sink_chunk(a.window, a.len_q);
+    const int64_t longest = a.len_q;          // of a pack: one sequence may hold all tokens
+    if (longest > a.sink_chunk) a.sink_slots = static_cast<int>(a.cu ? 2 * longest / a.sink_chunk + 1 : (longest + a.sink_chunk - 1) / a.sink_chunk);
+}
+// bytes of the chunks' parts, behind the statistics
+static size_t train_sink_bytes(const TrainArgs &a, int head_dim) {
+    const size_t tiles = (static_cast<size_t>(a.sink) + 127) / 128;
+    return a.sink ? static_cast<size_t>(a.sink_slots) * tiles * a.batch * a.heads_kv * 2 * 128 * head_dim * sizeof(float) : 0;
+}
+
 static int check_decode(const plx_decode_problem *p) {
     if (!p) return PLX_ERR_BAD_ARG;
     if (p->batch <= 0 || p->heads_q <= 0 || p->heads_kv <= 0 || p->cache_len <= 0 || p->n_splits <= 0 ||
@@ -142,18 +156,32 @@ struct StepCopies {
     const int32_t *lens_src;   // host
 };
 
+// which keys a sweep takes and where its partial state goes, where that is not the ordinary way
+struct Sweep {
+    int sink = 0;              // keys in front that stay visible behind the window
+    int first_key = 0;         // keys before it are not looked at
+    int min_len = 1;           // shorter lengths count as it
+    int part_stride = 1;       // records between those of two (batch, head)
+};
+
 static int run_decode(const plx_decode_problem *p, const void *q, const void *r, const void *k, const void *v, void *out,
                       float *part, const int32_t *seqused_k, const int32_t *cache_start, void *workspace,
                       size_t workspace_bytes, cudaStream_t stream, const plx_exchange *xch = nullptr,
-                      const StepCopies *step = nullptr) {
+                      const StepCopies *step = nullptr, const Sweep &sweep = Sweep()) {
     int st = check_decode_args(p, q, r, k, v, out, part);
     if (st != PLX_OK) return st;
+    if (sweep.sink < 0) return PLX_ERR_BAD_ARG;
+    if (sweep.sink > 0 && (p->kv_offset != 0 || xch)) return PLX_ERR_UNSUPPORTED;   // sinks of a cache that is not key-sharded
     if (p->n_splits > 1 && (!workspace || workspace_bytes < decode_ws_bytes(p) || misaligned16(workspace)))
         return PLX_ERR_WORKSPACE;
     DecodeArgs a{};
     a.q = q; a.r = r; a.k = k; a.v = v;
     a.out = part ? nullptr : out;
     a.part_out = part;
+    a.part_stride = sweep.part_stride;
+    a.sink = p->window_left >= 0 && p->window_left < p->cache_len ? (sweep.sink < p->cache_len ? sweep.sink : p->cache_len) : 0;
+    a.first_key = sweep.first_key;
+    a.min_len = sweep.min_len;
     a.seqused = seqused_k;
     a.cache_start = cache_start;
     const size_t bh = static_cast<size_t>(p->batch) * p->heads_q;
@@ -197,6 +225,60 @@ static int run_decode(const plx_decode_problem *p, const void *q, const void *r,
         while ((1 << a.page_shift) < p->page_size) ++a.page_shift;
     }
     return launch_decode(a, p->dtype, p->head_dim, stream);
+}
+
+static size_t prefix_part_bytes(const plx_decode_problem *p, const plx_prefix *x) {
+    return static_cast<size_t>(p->batch) * p->heads_q * (x->n_splits + 1) * PLX_DECODE_PART_FLOATS(p->head_dim) * sizeof(float);
+}
+
+static int check_prefix(const plx_decode_problem *p, const plx_prefix *x) {
+    if (!x || x->len <= 0 || x->n_splits < 1 || x->n_splits > PLX_PREFIX_MAX_SPLITS || p->window_left >= 0 || p->kv_offset != 0) return PLX_ERR_BAD_ARG;
+    if (!x->k)        // in the pages of the cache
+        return p->page_table && p->n_pages > 0 && !x->v && x->len % p->page_size == 0 && x->len <= p->cache_len ? PLX_OK : PLX_ERR_BAD_ARG;
+    if (!x->v || misaligned16(x->k) || misaligned16(x->v)) return PLX_ERR_BAD_ARG;
+    return x->stride_t >= 0 && x->stride_h >= 0 && (x->stride_t & 7) == 0 && (x->stride_h & 7) == 0 ? PLX_OK : PLX_ERR_BAD_ARG;
+}
+
+// the backward: the chosen stages (all of them with sinks)
+static int run_train_bwd(const plx_train_problem *p, int32_t sink_tokens, int32_t stages, const void *q, const void *r, const void *k, const void *v,
+                         const void *o, const void *barv, const float *d1, const float *bart, const float *m, const void *grad_o, void *dq, void *dr,
+                         void *dk, void *dv, void *workspace, size_t workspace_bytes, plx_stream_t stream) {
+    int st = check_train(p);
+    if (st != PLX_OK) return st;
+    if (sink_tokens < 0) return PLX_ERR_BAD_ARG;
+    if (stages <= 0 || (stages & ~PLX_BWD_ALL) != 0) return PLX_ERR_BAD_ARG;
+    if (!q || !r || !k || !v || !o || !barv || !d1 || !bart || !m || !grad_o || !dq || !dr || !dk || !dv)
+        return PLX_ERR_BAD_ARG;
+    const void *ptrs[] = {q, r, k, v, o, barv, grad_o, dq, dr, dk, dv};
+    for (const void *x : ptrs)
+        if (misaligned16(x)) return PLX_ERR_BAD_ARG;
+    TrainArgs a = make_train_args(p);
+    set_sinks(a, sink_tokens);
+    if (!workspace || workspace_bytes < train_ws_bytes(p) + train_sink_bytes(a, p->head_dim) || misaligned16(workspace)) return PLX_ERR_WORKSPACE;
+    if ((st = check_device()) != PLX_OK) return st;
+    a.q = q; a.r = r; a.k = k; a.v = v; a.o_in = o; a.barv_in = barv; a.go = grad_o;
+    a.d1 = const_cast<float *>(d1); a.bart = const_cast<float *>(bart); a.m = const_cast<float *>(m);
+    a.dq = dq; a.dr = dr; a.dk = dk; a.dv = dv;
+    a.bst = static_cast<float *>(workspace);
+    a.cst = a.bst + train_stat_rows(p) * 8;
+    a.parts = a.bst + train_stat_rows(p) * 12;
+    cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
+    const bool tc = train_bwd_sm100_supported(a, p->head_dim);
+    // dk/dv before dq/dr: the two are independent, and the CTAs of the second start as those of the first, longer
+    // one leave their SMs.  (The three kernels, B = 2, H = 8, L = 1024: 62.9 us one after the other, 43.5 so; at B = 4,
+    // H = 16 174 against 145, at B = 8, H = 16, L = 4096 the same.)
+    int before = 0;
+    for (int stage : {PLX_BWD_STATS, PLX_BWD_DKV, PLX_BWD_DQR}) {
+        if (!(stages & stage)) continue;
+        const bool overlap = before == (stage == PLX_BWD_DKV ? PLX_BWD_STATS : PLX_BWD_DKV);
+        st = (tc && stage != PLX_BWD_STATS) ? launch_train_bwd_sm100(a, p->dtype, p->head_dim, stage, overlap, cs)
+                                            : launch_train_bwd_mma(a, p->dtype, p->head_dim, stage, cs);
+        if (st != PLX_OK) return st;
+        before = stage;
+    }
+    // (dq/dr waits for dk/dv at its end: what follows it follows both)
+    if (tc && a.sink && a.sink_slots > 0) return launch_train_bwd_join(a, p->dtype, p->head_dim, cs);
+    return PLX_OK;
 }
 
 }  // namespace plx
@@ -248,15 +330,32 @@ int plx_train_workspace_bytes(const plx_train_problem *p, size_t *bytes) {
     return PLX_OK;
 }
 
-int plx_train_fwd(const plx_train_problem *p, const void *q, const void *r, const void *k, const void *v, void *o,
-                  void *barv, float *d1, float *bart, float *m, plx_stream_t stream) {
+int plx_train_workspace_bytes_sink(const plx_train_problem *p, int32_t sink_tokens, size_t *bytes) {
     int st = check_train(p);
     if (st != PLX_OK) return st;
+    if (!bytes || sink_tokens < 0) return PLX_ERR_BAD_ARG;
+    TrainArgs a = make_train_args(p);
+    set_sinks(a, sink_tokens);
+    *bytes = train_ws_bytes(p) + train_sink_bytes(a, p->head_dim);
+    return PLX_OK;
+}
+
+int plx_train_fwd(const plx_train_problem *p, const void *q, const void *r, const void *k, const void *v, void *o,
+                  void *barv, float *d1, float *bart, float *m, plx_stream_t stream) {
+    return plx_train_fwd_sink(p, 0, q, r, k, v, o, barv, d1, bart, m, stream);
+}
+
+int plx_train_fwd_sink(const plx_train_problem *p, int32_t sink_tokens, const void *q, const void *r, const void *k, const void *v, void *o,
+                       void *barv, float *d1, float *bart, float *m, plx_stream_t stream) {
+    int st = check_train(p);
+    if (st != PLX_OK) return st;
+    if (sink_tokens < 0) return PLX_ERR_BAD_ARG;
     if (!q || !r || !k || !v || !o || !barv || !d1 || !bart || !m) return PLX_ERR_BAD_ARG;
     if (misaligned16(q) || misaligned16(r) || misaligned16(k) || misaligned16(v) || misaligned16(o) || misaligned16(barv))
         return PLX_ERR_BAD_ARG;
     if ((st = check_device()) != PLX_OK) return st;
     TrainArgs a = make_train_args(p);
+    set_sinks(a, sink_tokens);
     a.q = q; a.r = r; a.k = k; a.v = v; a.o = o; a.barv = barv; a.d1 = d1; a.bart = bart; a.m = m;
     if (train_fwd_sm100_supported(a, p->head_dim))
         return launch_train_fwd_sm100(a, p->dtype, p->head_dim, reinterpret_cast<cudaStream_t>(stream));
@@ -266,11 +365,19 @@ int plx_train_fwd(const plx_train_problem *p, const void *q, const void *r, cons
 int plx_train_extend(const plx_train_problem *p, const void *q, const void *r, const void *k, const void *v, void *o,
                      const int32_t *seqused_k, const int32_t *page_table, int32_t page_size, int32_t pages_per_seq,
                      int32_t n_pages, plx_stream_t stream) {
+    return plx_train_extend_sink(p, 0, q, r, k, v, o, seqused_k, page_table, page_size, pages_per_seq, n_pages, stream);
+}
+
+int plx_train_extend_sink(const plx_train_problem *p, int32_t sink_tokens, const void *q, const void *r, const void *k, const void *v, void *o,
+                          const int32_t *seqused_k, const int32_t *page_table, int32_t page_size, int32_t pages_per_seq,
+                          int32_t n_pages, plx_stream_t stream) {
     int st = check_train(p);
     if (st != PLX_OK) return st;
+    if (sink_tokens < 0) return PLX_ERR_BAD_ARG;
     if (!q || !r || !k || !v || !o || p->cu_seqlens || p->len_q > p->len_k) return PLX_ERR_BAD_ARG;
     if (misaligned16(q) || misaligned16(r) || misaligned16(k) || misaligned16(v) || misaligned16(o)) return PLX_ERR_BAD_ARG;
     TrainArgs a = make_train_args(p);
+    set_sinks(a, sink_tokens);
     a.q = q; a.r = r; a.k = k; a.v = v; a.o = o;
     a.seqused = seqused_k;
     if (page_table) {
@@ -291,37 +398,13 @@ int plx_train_bwd_stages(const plx_train_problem *p, int32_t stages, const void 
                          const void *v, const void *o, const void *barv, const float *d1, const float *bart,
                          const float *m, const void *grad_o, void *dq, void *dr, void *dk, void *dv, void *workspace,
                          size_t workspace_bytes, plx_stream_t stream) {
-    int st = check_train(p);
-    if (st != PLX_OK) return st;
-    if (stages <= 0 || (stages & ~PLX_BWD_ALL) != 0) return PLX_ERR_BAD_ARG;
-    if (!q || !r || !k || !v || !o || !barv || !d1 || !bart || !m || !grad_o || !dq || !dr || !dk || !dv)
-        return PLX_ERR_BAD_ARG;
-    const void *ptrs[] = {q, r, k, v, o, barv, grad_o, dq, dr, dk, dv};
-    for (const void *x : ptrs)
-        if (misaligned16(x)) return PLX_ERR_BAD_ARG;
-    if (!workspace || workspace_bytes < train_ws_bytes(p) || misaligned16(workspace)) return PLX_ERR_WORKSPACE;
-    if ((st = check_device()) != PLX_OK) return st;
-    TrainArgs a = make_train_args(p);
-    a.q = q; a.r = r; a.k = k; a.v = v; a.o_in = o; a.barv_in = barv; a.go = grad_o;
-    a.d1 = const_cast<float *>(d1); a.bart = const_cast<float *>(bart); a.m = const_cast<float *>(m);
-    a.dq = dq; a.dr = dr; a.dk = dk; a.dv = dv;
-    a.bst = static_cast<float *>(workspace);
-    a.cst = a.bst + train_stat_rows(p) * 8;
-    cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
-    const bool tc = train_bwd_sm100_supported(a, p->head_dim);
-    // dk/dv before dq/dr: the two are independent, and the CTAs of the second start as those of the first, longer
-    // one leave their SMs.  (The three kernels, B = 2, H = 8, L = 1024: 62.9 us one after the other, 43.5 so; at B = 4,
-    // H = 16 174 against 145, at B = 8, H = 16, L = 4096 the same.)
-    int before = 0;
-    for (int stage : {PLX_BWD_STATS, PLX_BWD_DKV, PLX_BWD_DQR}) {
-        if (!(stages & stage)) continue;
-        const bool overlap = before == (stage == PLX_BWD_DKV ? PLX_BWD_STATS : PLX_BWD_DKV);
-        st = (tc && stage != PLX_BWD_STATS) ? launch_train_bwd_sm100(a, p->dtype, p->head_dim, stage, overlap, cs)
-                                            : launch_train_bwd_mma(a, p->dtype, p->head_dim, stage, cs);
-        if (st != PLX_OK) return st;
-        before = stage;
-    }
-    return PLX_OK;
+    return run_train_bwd(p, 0, stages, q, r, k, v, o, barv, d1, bart, m, grad_o, dq, dr, dk, dv, workspace, workspace_bytes, stream);
+}
+
+int plx_train_bwd_sink(const plx_train_problem *p, int32_t sink_tokens, const void *q, const void *r, const void *k, const void *v, const void *o,
+                       const void *barv, const float *d1, const float *bart, const float *m, const void *grad_o, void *dq, void *dr, void *dk,
+                       void *dv, void *workspace, size_t workspace_bytes, plx_stream_t stream) {
+    return run_train_bwd(p, sink_tokens, PLX_BWD_ALL, q, r, k, v, o, barv, d1, bart, m, grad_o, dq, dr, dk, dv, workspace, workspace_bytes, stream);
 }
 
 int plx_train_bwd(const plx_train_problem *p, const void *q, const void *r, const void *k, const void *v, const void *o,
@@ -449,6 +532,12 @@ int plx_decode_stage(void *q, const void *q_src, void *r, const void *r_src, siz
 
 int plx_decode_step(const plx_decode_problem *p, void *q, const void *q_src, void *r, const void *r_src, const void *k, const void *v, void *out,
                     int32_t *seqused_k, const int32_t *seqused_src, void *workspace, size_t workspace_bytes, plx_stream_t stream) {
+    return plx_decode_step_sink(p, 0, q, q_src, r, r_src, k, v, out, seqused_k, seqused_src, workspace, workspace_bytes, stream);
+}
+
+int plx_decode_step_sink(const plx_decode_problem *p, int32_t sink_tokens, void *q, const void *q_src, void *r, const void *r_src, const void *k,
+                         const void *v, void *out, int32_t *seqused_k, const int32_t *seqused_src, void *workspace, size_t workspace_bytes,
+                         plx_stream_t stream) {
     if (!p || !out || !q || !r || (seqused_src && !seqused_k) || misaligned16(q) || misaligned16(r)) return PLX_ERR_BAD_ARG;
     if (p->batch > PLX_DECODE_STEP_ROWS) return PLX_ERR_UNSUPPORTED;
     const int st = check_decode(p);
@@ -463,7 +552,7 @@ int plx_decode_step(const plx_decode_problem *p, void *q, const void *q_src, voi
     }
     const StepCopies step{q_src ? q : nullptr, r_src ? r : nullptr, seqused_k, seqused_src};
     return run_decode(p, q_src ? q_src : q, r_src ? r_src : r, k, v, out, nullptr, seqused_src ? nullptr : seqused_k, nullptr, workspace,
-                      workspace_bytes, reinterpret_cast<cudaStream_t>(stream), nullptr, &step);
+                      workspace_bytes, reinterpret_cast<cudaStream_t>(stream), nullptr, &step, Sweep{sink_tokens});
 }
 
 int plx_decode(const plx_decode_problem *p, const void *q, const void *r, const void *k, const void *v, void *out,
@@ -472,6 +561,99 @@ int plx_decode(const plx_decode_problem *p, const void *q, const void *r, const 
     if (!out) return PLX_ERR_BAD_ARG;
     return run_decode(p, q, r, k, v, out, nullptr, seqused_k, cache_start, workspace, workspace_bytes,
                       reinterpret_cast<cudaStream_t>(stream));
+}
+
+int plx_decode_sink(const plx_decode_problem *p, int32_t sink_tokens, const void *q, const void *r, const void *k, const void *v, void *out,
+                    const int32_t *seqused_k, const int32_t *cache_start, void *workspace, size_t workspace_bytes, plx_stream_t stream) {
+    if (!out) return PLX_ERR_BAD_ARG;
+    return run_decode(p, q, r, k, v, out, nullptr, seqused_k, cache_start, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream), nullptr,
+                      nullptr, Sweep{sink_tokens});
+}
+
+int plx_decode_prefix_splits(int32_t batch, int32_t heads_q, int32_t heads_kv, int32_t len, int32_t sm_count) {
+    if (batch <= 0 || heads_kv <= 0 || heads_q % heads_kv != 0 || len <= 0 || sm_count <= 0) return 1;
+    // An item costs its key tiles and about four more for its start and its end; every SM takes the same number of items.
+    const int64_t units = static_cast<int64_t>(prefix_row_tiles(heads_q / heads_kv, batch)) * heads_kv, tiles = (len + 63) / 64;
+    int best = 1;
+    int64_t best_cost = INT64_MAX;
+    for (int n = 1; n <= PLX_PREFIX_MAX_SPLITS && n <= tiles; ++n) {
+        const int64_t cost = ((units * n + sm_count - 1) / sm_count) * ((tiles + n - 1) / n + 4);
+        if (cost < best_cost) {
+            best_cost = cost;
+            best = n;
+        }
+    }
+    return best;
+}
+
+int plx_decode_prefix_workspace_bytes(const plx_decode_problem *p, const plx_prefix *x, size_t *bytes) {
+    int st = check_decode(p);
+    if (st != PLX_OK) return st;
+    if (!x || !bytes || x->n_splits < 1 || x->n_splits > PLX_PREFIX_MAX_SPLITS) return PLX_ERR_BAD_ARG;
+    *bytes = prefix_part_bytes(p, x) + decode_ws_bytes(p);
+    return PLX_OK;
+}
+
+int plx_decode_prefix(const plx_decode_problem *p, const plx_prefix *x, const void *q, const void *r, const void *k, const void *v, void *out,
+                      const int32_t *seqused_k, void *workspace, size_t workspace_bytes, plx_stream_t stream) {
+    int st = check_decode_args(p, q, r, k, v, out, nullptr);
+    if (st == PLX_OK) st = check_prefix(p, x);
+    if (st != PLX_OK) return st;
+    const size_t part_bytes = prefix_part_bytes(p, x);
+    if (!workspace || misaligned16(workspace) || workspace_bytes < part_bytes + decode_ws_bytes(p)) return PLX_ERR_WORKSPACE;
+    const cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
+    float *parts = static_cast<float *>(workspace);
+    unsigned char *rest = static_cast<unsigned char *>(workspace) + part_bytes;
+    const size_t rest_bytes = workspace_bytes - part_bytes;
+    const bool in_cache = !x->k;                       // the rows' own page tables begin with the prefix
+    TrainArgs a{};
+    a.q = q; a.r = r;
+    a.k = in_cache ? k : x->k;
+    a.v = in_cache ? v : x->v;
+    a.batch = p->batch; a.heads_q = p->heads_q; a.heads_kv = p->heads_kv; a.n_rep = p->heads_q / p->heads_kv;
+    a.len_q = 1; a.len_k = x->len;
+    a.window = -1;
+    a.scale = p->qk_scale;
+    a.c2 = p->qk_scale * kLog2e;
+    a.q_st = p->head_dim; a.q_sh = static_cast<int64_t>(a.n_rep) * p->head_dim; a.q_sb = static_cast<int64_t>(p->heads_q) * p->head_dim;
+    a.kv_sb = in_cache ? p->kv_stride_b : x->stride_t; a.kv_st = in_cache ? p->kv_stride_t : x->stride_t; a.kv_sh = in_cache ? p->kv_stride_h : x->stride_h;
+    if (in_cache) {
+        a.page_table = p->page_table;
+        a.pages_per_seq = p->pages_per_seq;
+        a.n_pages = p->n_pages;
+        a.page_mask = p->page_size - 1;
+        while ((1 << a.page_shift) < p->page_size) ++a.page_shift;
+    }
+    a.parts = parts;
+    const Sweep own{0, in_cache ? x->len : 0, in_cache ? x->len : 0, 0};
+    auto sweep_own = [&](int n_parts) {
+        Sweep s = own;
+        s.part_stride = n_parts;
+        return run_decode(p, q, r, k, v, nullptr, parts + static_cast<size_t>(n_parts - 1) * PLX_DECODE_PART_FLOATS(p->head_dim), seqused_k, nullptr, rest,
+                          rest_bytes, cs, nullptr, nullptr, s);
+    };
+    int n_parts;
+    if (train_extend_sm100_supported(a, p->head_dim)) {
+        a.n_splits = x->n_splits;
+        a.n_parts = n_parts = x->n_splits + 1;
+        st = launch_prefix_sm100(a, p->dtype, p->head_dim, cs);
+    } else if (in_cache) {
+        return run_decode(p, q, r, k, v, out, nullptr, seqused_k, nullptr, rest, rest_bytes, cs);      // pages: the prefix is swept with the rest of each row
+    } else {
+        // a scale or strides that the tensor-core kernel does not take: every row sweeps the prefix
+        plx_decode_problem prefix = *p;
+        prefix.page_table = nullptr;
+        prefix.cache_len = x->len;
+        prefix.window_left = -1;
+        prefix.kv_offset = prefix.total_len = 0;
+        prefix.kv_stride_b = 0; prefix.kv_stride_t = x->stride_t; prefix.kv_stride_h = x->stride_h;
+        Sweep s;
+        s.part_stride = n_parts = 2;
+        st = run_decode(&prefix, q, r, x->k, x->v, nullptr, parts, nullptr, nullptr, rest, rest_bytes, cs, nullptr, nullptr, s);
+    }
+    if (st == PLX_OK) st = sweep_own(n_parts);
+    if (st != PLX_OK) return st;
+    return launch_prefix_merge(parts, n_parts, static_cast<int64_t>(p->batch) * p->heads_q, p->head_dim, p->dtype, out, cs);
 }
 
 int plx_decode_partial(const plx_decode_problem *p, const void *q, const void *r, const void *k, const void *v,

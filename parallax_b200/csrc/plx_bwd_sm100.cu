@@ -149,17 +149,80 @@ __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t x, uint32_t
 // and the range of 64-wide tiles of the other side that it streams.
 struct Item {
     int bos, nq, nk, m0, b, hy, hk, off, t_lo, n_t, n_iter;   // streamed tiles t_lo .. t_lo + n_t - 1, per q head
-    int valid;
+    int valid;                                                // sinks, DKV: from 2 on a chunk, which leaves part valid - 2
+    // DQR with sinks: the first n_iter - n_t tiles are 0, 1, .. instead.  The t-th tile of a q head:
+    template <bool SINK>
+    __device__ __forceinline__ int tile(int t) const {
+        const int front = SINK ? n_iter - n_t : 0;
+        return SINK && t < front ? t : t_lo + t - front;
+    }
 };
+
+// Sinks, DKV.  A key j < a.sink is seen by every row from j on, where another is seen by a.window: in sequences of more than
+// a.sink_chunk rows the key tiles that hold sinks are therefore cut into chunks of that many rows, which leave
+// their sums in 32 bits, and join_kernel adds those up (in the order of the rows: the same result every time).  A row that a chunk
+// cannot contribute to is neither written nor read (see chunk_keys).
+// Sequence i of a pack owns the chunk slots from 2 cu[i] / sink_chunk on: of a length above sink_chunk it has at most
+// 2 length / sink_chunk chunks, so slots are not shared and there are 2 total / sink_chunk + 1, whatever the sequences are.
+__device__ __forceinline__ bool locate_chunk(const TrainArgs &a, int slot, Seq &s, int &chunk) {
+    s = Seq{0, a.len_q, a.len_k};
+    chunk = slot;
+    if (a.cu) {
+        auto first = [&](int i) { return static_cast<int>(2ll * __ldg(a.cu + i) / a.sink_chunk); };
+        int lo = 0, hi = a.n_seqs - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (first(mid) <= slot) lo = mid;
+            else hi = mid - 1;
+        }
+        s.bos = __ldg(a.cu + lo);
+        s.nq = s.nk = __ldg(a.cu + lo + 1) - s.bos;
+        chunk = slot - first(lo);
+    }
+    return s.nq > a.sink_chunk && chunk >= 0 && static_cast<int64_t>(chunk) * a.sink_chunk < s.nq;
+}
+// the tiles of 64 rows that chunk `chunk` of key tile m0 streams (none: n_t = 0)
+__device__ __forceinline__ void chunk_rows(const TrainArgs &a, const Seq &s, int m0, int chunk, int &t_lo, int &n_t) {
+    const int lo = max(max(0, m0 - (s.nk - s.nq)), chunk * a.sink_chunk), hi = min(s.nq, (chunk + 1) * a.sink_chunk);
+    t_lo = lo / kBN;
+    n_t = lo < hi ? (hi + kBN - 1) / kBN - t_lo : 0;
+}
+// how many keys of the tile see a row of the tiles from t_lo on: all, or where those lie behind the windows the sinks
+__device__ __forceinline__ int chunk_keys(const TrainArgs &a, const Seq &s, int m0, int t_lo) {
+    const bool behind = t_lo * kBN > m0 + kBM - 1 - (s.nk - s.nq) + a.window - 1;
+    return min(kBM, (behind ? min(a.sink, s.nk) : s.nk) - m0);
+}
 
 // Work item `idx` of the launch.  Items are (batch, head)-major, so that CTAs running at the same time
 // share their streamed tiles in L2; inside a (batch, head) the 128-wide tiles alternate last, first,
 // last - 1, second, ...: under the causal mask any two neighbours add up to the same work.
 // With one item per CTA, and handed out by the hardware (group > 0), the longest items come first instead (see
 // longest_first): the CTAs of dq/dr take over the SMs that dk/dv leaves one by one.
-template <bool DQR>
+template <bool DQR, bool SINK>
 __device__ __forceinline__ Item get_item(const TrainArgs &a, int idx, int n_mt, int group) {
     Item it;
+    const int sink_tiles = SINK && !DQR ? (a.sink + kBM - 1) / kBM : 0;
+    if (SINK && !DQR) {
+        // the chunks first: (batch, head) fastest, so that all of them begin at once
+        const int n_bh = a.batch * a.heads_kv, n_chunks = a.sink_slots * sink_tiles * n_bh;
+        if (idx < n_chunks) {
+            const int bh = idx % n_bh, rest = idx / n_bh, slot = rest % a.sink_slots;
+            Seq s;
+            int chunk;
+            it.valid = locate_chunk(a, slot, s, chunk) ? 2 + idx : 0;
+            it.bos = s.bos; it.nq = s.nq; it.nk = s.nk;
+            it.off = s.nk - s.nq;
+            it.m0 = rest / a.sink_slots * kBM;
+            it.b = bh / a.heads_kv;
+            it.hy = it.hk = bh % a.heads_kv;
+            it.n_t = 0;
+            if (it.valid && it.m0 < it.nk) chunk_rows(a, s, it.m0, chunk, it.t_lo, it.n_t);
+            it.n_iter = it.n_t * a.n_rep;
+            if (it.n_t == 0) it.valid = 0;
+            return it;
+        }
+        idx -= n_chunks;
+    }
     int bh = idx / n_mt, k = idx % n_mt;
     int tile_id = (k & 1) ? (k >> 1) : n_mt - 1 - (k >> 1);
     if (group > 0) {
@@ -186,10 +249,18 @@ __device__ __forceinline__ Item get_item(const TrainArgs &a, int idx, int n_mt, 
         const int lo_col = a.window < 0 ? 0 : max(0, it.m0 + it.off - a.window + 1);
         it.t_lo = lo_col / kBN;
         n_t = hi_col > lo_col ? (hi_col + kBN - 1) / kBN - it.t_lo : 0;
+        if (SINK) {
+            const int sinks = hi_col > 0 ? (min(a.sink, hi_col) + kBN - 1) / kBN : 0;
+            it.n_t = it.valid ? n_t : 0;
+            it.n_iter = it.valid ? n_t + (n_t > 0 ? min(sinks, it.t_lo) : sinks) : 0;      // (a window of 0 may leave nothing but sinks)
+            return it;
+        }
     } else {
+        const bool sinks = SINK && it.m0 < a.sink;
+        if (sinks && a.sink_slots > 0 && it.nq > a.sink_chunk) it.valid = 0;               // its chunks do it
         // rows [i_lo, i_hi) see some key of the tile: key m is seen by rows m - off .. m - off + window - 1
         const int i_lo = max(0, it.m0 - it.off);
-        const int i_hi = a.window < 0 ? it.nq : min(it.nq, it.m0 + kBM - 1 - it.off + a.window);
+        const int i_hi = a.window < 0 || sinks ? it.nq : min(it.nq, it.m0 + kBM - 1 - it.off + a.window);
         it.t_lo = i_lo / kBN;
         n_t = i_hi > i_lo ? (i_hi + kBN - 1) / kBN - it.t_lo : 0;
     }
@@ -210,7 +281,7 @@ __device__ __forceinline__ int item_index(int n, int chunk_shift) {
 // accumulators, and the hand-overs for those are arranged so that the loads, the tensor-memory tile and
 // the first score products of the next item are under way while the element-wise warps write out the
 // accumulators of the current one.  TMEM allocation, barrier set-up and launch latency are paid once.
-template <typename T, int D, int MODE, bool SHORT>
+template <typename T, int D, int MODE, bool SHORT, bool SINK>
 __global__ void __launch_bounds__((4 + kEwWarps) * 32, 1)
 bwd_sm100_kernel(const TrainArgs a, int n_tok, const __grid_constant__ CUtensorMap tm_q,
                  const __grid_constant__ CUtensorMap tm_r, const __grid_constant__ CUtensorMap tm_go,
@@ -311,7 +382,7 @@ bwd_sm100_kernel(const TrainArgs a, int n_tok, const __grid_constant__ CUtensorM
                 clc_ask(base + L::kClc, bar(L::kClcFull));
                 src.asked = src.taken;
             }
-            it = get_item<DQR>(a, idx, n_mt, group);
+            it = get_item<DQR, SINK>(a, idx, n_mt, group);
             if (it.valid) return true;
         }
     };
@@ -374,7 +445,7 @@ bwd_sm100_kernel(const TrainArgs a, int n_tok, const __grid_constant__ CUtensorM
                         if (!ok) break;
                     }
                     mbar_expect_tx(bar(L::kNFull + s), L::kStageTx);
-                    const int row0 = it.bos + (it.t_lo + tt) * kBN;
+                    const int row0 = it.bos + it.template tile<SINK && DQR>(DQR ? t : tt) * kBN;
                     if (DQR) {
                         const CUtensorMap *maps[2] = {&tm_k, &tm_v};
                         for (int j = 0; j < 2; ++j)
@@ -660,13 +731,13 @@ bwd_sm100_kernel(const TrainArgs a, int n_tok, const __grid_constant__ CUtensorM
                 if (!ok) break;
                 tc_fence_after();
 
-                const int tile0 = (cur.t_lo + (DQR ? it : it % cur.n_t)) * kBN;   // first streamed index of the tile
+                const int tile0 = cur.template tile<SINK && DQR>(DQR ? it : it % cur.n_t) * kBN;   // first streamed index of the tile
                 const int win = a.window;
                 // tile-uniform: every element of the tile is visible
                 const bool full = DQR ? (tile0 + kBN - 1 <= m0 + off && tile0 + kBN <= nk && m0 + kBM <= nq &&
-                                         (win < 0 || tile0 >= m0 + kBM + off - win))
+                                         (win < 0 || tile0 >= m0 + kBM + off - win || (SINK && tile0 + kBN <= a.sink)))
                                       : (tile0 >= m0 + kBM - 1 - off && tile0 + kBN <= nq && m0 + kBM <= nk &&
-                                         (win < 0 || tile0 + kBN - 1 <= m0 - off + win - 1));
+                                         (win < 0 || tile0 + kBN - 1 <= m0 - off + win - 1 || (SINK && m0 + kBM <= a.sink)));
                 const float *stats = reinterpret_cast<const float *>(smem_raw + L::kStats + (g % kStatStages) * kStatBytes);
                 // One pair of adjacent columns: constants nml = -mL, nc1 = -(1 + bart), bb = b, ct = b - t (DKV: times
                 // scale; DKV: nc1 times scale too).  The third tile carries -W * scale = p un scale (DKV
@@ -692,7 +763,8 @@ bwd_sm100_kernel(const TrainArgs a, int n_tok, const __grid_constant__ CUtensorM
                     float2 gu = __fmul2_rn(p, dn);
                     float2 gl = __ffma2_rn(wn, dn, pc);
                     if (decltype(masked)::value) {
-                        const bool v0 = col >= lo && col <= hi, v1 = col + 1 >= lo && col + 1 <= hi;
+                        const int front = SINK && DQR ? a.sink : INT_MIN;           // columns before it are visible too
+                        const bool v0 = (col >= lo || col < front) && col <= hi, v1 = (col + 1 >= lo || col + 1 < front) && col + 1 <= hi;
                         gl = make_float2(v0 ? gl.x : 0.f, v1 ? gl.y : 0.f);
                         gu = make_float2(v0 ? gu.x : 0.f, v1 ? gu.y : 0.f);
                         wn = make_float2(v0 ? wn.x : 0.f, v1 ? wn.y : 0.f);
@@ -730,7 +802,7 @@ bwd_sm100_kernel(const TrainArgs a, int n_tok, const __grid_constant__ CUtensorM
                             for (int j = 0; j < 2; ++j) {
                                 const int key = m0 + quarter * 32 + 16 * h + 8 * j + gq;
                                 lo[j] = max(key - off, 0);
-                                hi[j] = key < nk ? (win < 0 ? nq - 1 : min(nq - 1, key - off + win - 1)) : -1;
+                                hi[j] = key < nk ? (win < 0 || (SINK && key < a.sink) ? nq - 1 : min(nq - 1, key - off + win - 1)) : -1;
                             }
 #pragma unroll
                             for (int k = 0; k < 8; ++k) {
@@ -755,7 +827,7 @@ bwd_sm100_kernel(const TrainArgs a, int n_tok, const __grid_constant__ CUtensorM
                     // one row (DQR) or key (DKV) a thread, CH columns at a time
                     const int lo = DQR ? (win < 0 ? INT_MIN : mg + off - win + 1) : max(mg - off, 0);      // visible columns
                     const int hi = DQR ? (mg < nq ? min(mg + off, nk - 1) : -1)
-                                       : (mg < nk ? (win < 0 ? nq - 1 : min(nq - 1, mg - off + win - 1)) : -1);
+                                       : (mg < nk ? (win < 0 || (SINK && mg < a.sink) ? nq - 1 : min(nq - 1, mg - off + win - 1)) : -1);
 #pragma unroll 1
                     for (int ch = 0; ch < GR; ++ch) {
                         const int col0 = (GR == 2 ? ch : sel) * CH;
@@ -831,6 +903,12 @@ bwd_sm100_kernel(const TrainArgs a, int n_tok, const __grid_constant__ CUtensorM
             const int rows_left = (DQR ? nq : nk) - m0;
             T *dst0;
             int64_t row_stride;
+            float *part = nullptr;             // of a chunk: [dk, dv][128 keys][D]
+            int part_rows = 0;
+            if (SINK && !DQR && cur.valid > 1) {
+                part = a.parts + (static_cast<int64_t>(cur.valid - 2) * 2 + sel) * (kBM * D);
+                part_rows = chunk_keys(a, Seq{cur.bos, cur.nq, cur.nk}, m0, cur.t_lo);
+            }
             if (DQR) {
                 dst0 = static_cast<T *>(sel == 0 ? a.dq : a.dr) + cur.b * a.q_sb + cur.hy * a.q_sh + static_cast<int64_t>(cur.bos + m0) * a.q_st;
                 row_stride = a.q_st;
@@ -864,6 +942,16 @@ bwd_sm100_kernel(const TrainArgs a, int n_tok, const __grid_constant__ CUtensorM
                     tc_fence_before();
                     mbar_arrive(bar(L::kAccFree));
                 }
+                if (SINK && !DQR && part) {
+#pragma unroll
+                    for (int hh = 0; hh < 2; ++hh)
+                        if (rl + 8 * hh < part_rows)
+#pragma unroll
+                            for (int k = 0; k < 8; ++k)
+                                __stcg(reinterpret_cast<float2 *>(part + (rl + 8 * hh) * D + 64 * cc + 8 * k + 2 * t),
+                                       make_float2(__uint_as_float(x[4 * k + 2 * hh]) * mul, __uint_as_float(x[4 * k + 2 * hh + 1]) * mul));
+                    continue;
+                }
 #pragma unroll
                 for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
@@ -891,10 +979,51 @@ bwd_sm100_kernel(const TrainArgs a, int n_tok, const __grid_constant__ CUtensorM
     if (DQR) grid_wait();
 }
 
+// dk, dv of the key tiles that were cut into chunks.  CTA (slot, key tile, (batch, kv head)); the CTAs of a sequence's slots share
+// its tile, 8 channels of a key per thread.  Bound by reading the parts: those of the first chunks whole, then the sinks' rows.
+constexpr int kJoinThreads = 256;
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const TrainArgs a) {
+    Seq s;
+    int chunk;
+    const int m0 = blockIdx.y * kBM;
+    if (!locate_chunk(a, blockIdx.x, s, chunk) || m0 >= s.nk) return;
+    const int n_bh = gridDim.z, first = blockIdx.x - chunk, n_chunks = (s.nq + a.sink_chunk - 1) / a.sink_chunk;
+    const int b = blockIdx.z / a.heads_kv, hk = blockIdx.z % a.heads_kv;
+    constexpr int kPerRow = D / 8;
+    for (int e = chunk * kJoinThreads + threadIdx.x; e < 2 * kBM * kPerRow; e += n_chunks * kJoinThreads) {
+        const int which = e / (kBM * kPerRow), row = e / kPerRow % kBM, c = e % kPerRow * 8;
+        if (m0 + row >= s.nk) continue;
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = 0.f;
+#pragma unroll 4
+        for (int j = 0; j < n_chunks; ++j) {
+            int t_lo, n_t;
+            chunk_rows(a, s, m0, j, t_lo, n_t);
+            if (n_t == 0 || row >= chunk_keys(a, s, m0, t_lo)) continue;
+            const int64_t idx = (static_cast<int64_t>(blockIdx.y) * a.sink_slots + first + j) * n_bh + blockIdx.z;      // of the item, see get_item
+            const float4 *src = reinterpret_cast<const float4 *>(a.parts + (idx * 2 + which) * (kBM * D) + row * D + c);
+            const float4 u = __ldcg(src), v = __ldcg(src + 1);
+            x[0] += u.x; x[1] += u.y; x[2] += u.z; x[3] += u.w;
+            x[4] += v.x; x[5] += v.y; x[6] += v.z; x[7] += v.w;
+        }
+        T *dst = static_cast<T *>(which == 0 ? a.dk : a.dv) + b * a.kv_sb + hk * a.kv_sh + static_cast<int64_t>(s.bos + m0 + row) * a.kv_st + c;
+        *reinterpret_cast<uint4 *>(dst) = make_uint4(Elem<T>::pack(x[0], x[1]), Elem<T>::pack(x[2], x[3]), Elem<T>::pack(x[4], x[5]), Elem<T>::pack(x[6], x[7]));
+    }
+}
+
 // ------------------------------------------------------------------------- //
 // host side
 // ------------------------------------------------------------------------- //
-template <typename T, int D, int MODE, bool SHORT>
+template <typename T, int D>
+int launch_join(const TrainArgs &a, cudaStream_t stream) {
+    join_kernel<T, D><<<dim3(a.sink_slots, (a.sink + kBM - 1) / kBM, a.batch * a.heads_kv), kJoinThreads, 0, stream>>>(a);
+    count_launch();
+    return cudaGetLastError() == cudaSuccess ? PLX_OK : PLX_ERR_LAUNCH;
+}
+
+template <typename T, int D, int MODE, bool SHORT, bool SINK>
 int launch_mode(const TrainArgs &a, int n_tok, const ErrSink &sink, bool overlap, cudaStream_t stream) {
     using L = Smem<D, MODE, SHORT>;
     constexpr bool DQR = MODE == kModeDQR;
@@ -907,16 +1036,17 @@ int launch_mode(const TrainArgs &a, int n_tok, const ErrSink &sink, bool overlap
         !tma::make_map(&tk, dt, a.k, D, a.len_k, a.heads_kv, a.batch, a.kv_st, a.kv_sh, a.kv_sb, kv_rows) ||
         !tma::make_map(&tv, dt, a.v, D, a.len_k, a.heads_kv, a.batch, a.kv_st, a.kv_sh, a.kv_sb, kv_rows))
         return PLX_ERR_LAUNCH;
-    auto kern = bwd_sm100_kernel<T, D, MODE, SHORT>;
+    auto kern = bwd_sm100_kernel<T, D, MODE, SHORT, SINK>;
     static std::mutex attr_mu;
     static bool attr_done[tma::kMaxDevices] = {};
     if (!tma::opt_in_smem(kern, static_cast<int>(L::kBytes), attr_done, attr_mu)) return PLX_ERR_LAUNCH;
     const int len = DQR ? a.len_q : a.len_k;
     const int tiles = a.cu ? (len + kBM - 1) / kBM + a.n_seqs : (len + kBM - 1) / kBM;
-    const int n_items = tiles * a.batch * (DQR ? a.heads_q : a.heads_kv), sms = tma::sm_count();
+    const int chunks = SINK && !DQR ? a.sink_slots * ((a.sink + kBM - 1) / kBM) * a.batch * a.heads_kv : 0;
+    const int n_items = chunks + tiles * a.batch * (DQR ? a.heads_q : a.heads_kv), sms = tma::sm_count();
     if (sms <= 0) return PLX_ERR_LAUNCH;
     // with plenty of items a CTA takes them in neighbouring pairs (a heavy and a light tile)
-    const bool dynamic = items_by_hardware(n_items, sms, a.cu != nullptr);
+    const bool dynamic = items_by_hardware(n_items, sms, a.cu != nullptr || chunks > 0);
     const int chunk_shift = dynamic ? -1 : n_items >= 2 * sms ? 1 : 0;
     const int units = dynamic ? n_items : (n_items + (1 << chunk_shift) - 1) >> chunk_shift;
     const int group = !dynamic && n_items > sms ? 0 : dynamic && a.cu ? 1 : item_group(a.batch * (DQR ? a.heads_q : a.heads_kv), tiles, sms);
@@ -948,41 +1078,53 @@ int launch_mode(const TrainArgs &a, int n_tok, const ErrSink &sink, bool overlap
 // short ones are on the wrong side of it: one of 16384 and 256 of 64 2445 / 2568, two of 8192 and 200 of 64 1257 / 1272.
 bool short_items(const TrainArgs &a) {
     int64_t keys = a.cu ? 2ll * a.len_q / (3ll * a.n_seqs) + kBM / 2 : a.len_k - a.len_q / 2 + std::min(a.len_q, kBM) / 2;
-    if (a.window > 0) keys = std::min<int64_t>(keys, a.window + kBM);
+    if (a.window > 0) keys = std::min<int64_t>(keys, static_cast<int64_t>(a.window) + kBM + (a.sink + kBN - 1) / kBN * kBN);
     return keys <= 14 * kBN;
 }
 
 }  // namespace
 
 bool train_bwd_sm100_supported(const TrainArgs &a, int head_dim) {
-    if ((head_dim != 64 && head_dim != 128) || a.window == 0 || !(a.c2 > 0.f)) return false;
+    if ((head_dim != 64 && head_dim != 128) || (a.window == 0 && a.sink == 0) || !(a.c2 > 0.f)) return false;
     const char *env = std::getenv("PLX_BWD_KERNEL");
     if (env && env[0] == 'm') return false;  // "mma": force the warp-level kernels
     return tma::encode_fn() != nullptr;
+}
+
+template <typename T, bool SINK>
+static int launch_stage(const TrainArgs &a, int head_dim, bool dqr, const ErrSink &err, bool overlap, cudaStream_t stream) {
+    const int n_tok = a.len_q;
+    if (head_dim == 64)
+        return dqr ? launch_mode<T, 64, kModeDQR, false, SINK>(a, n_tok, err, overlap, stream)
+                   : launch_mode<T, 64, kModeDKV, false, SINK>(a, n_tok, err, overlap, stream);
+    if (!dqr) return launch_mode<T, 128, kModeDKV, false, SINK>(a, n_tok, err, overlap, stream);
+    return short_items(a) ? launch_mode<T, 128, kModeDQR, true, SINK>(a, n_tok, err, overlap, stream)
+                          : launch_mode<T, 128, kModeDQR, false, SINK>(a, n_tok, err, overlap, stream);
 }
 
 int launch_train_bwd_sm100(const TrainArgs &a, int dtype, int head_dim, int stage, bool overlap, cudaStream_t stream) {
     const ErrorWords ew = sm100_error_words();
     if (!ew.word) return PLX_ERR_LAUNCH;
     const ErrSink err{ew.word, ew.mirror};
-    const int n_tok = a.len_q;
     const bool dqr = stage == PLX_BWD_DQR;
-    if (dtype == PLX_BF16) {
-        if (head_dim == 64)
-            return dqr ? launch_mode<__nv_bfloat16, 64, kModeDQR, false>(a, n_tok, err, overlap, stream)
-                       : launch_mode<__nv_bfloat16, 64, kModeDKV, false>(a, n_tok, err, overlap, stream);
-        return dqr ? (short_items(a) ? launch_mode<__nv_bfloat16, 128, kModeDQR, true>(a, n_tok, err, overlap, stream)
-                                     : launch_mode<__nv_bfloat16, 128, kModeDQR, false>(a, n_tok, err, overlap, stream))
-                   : launch_mode<__nv_bfloat16, 128, kModeDKV, false>(a, n_tok, err, overlap, stream);
-    }
-    if (dtype == PLX_FP16) {
-        if (head_dim == 64)
-            return dqr ? launch_mode<__half, 64, kModeDQR, false>(a, n_tok, err, overlap, stream)
-                       : launch_mode<__half, 64, kModeDKV, false>(a, n_tok, err, overlap, stream);
-        return dqr ? (short_items(a) ? launch_mode<__half, 128, kModeDQR, true>(a, n_tok, err, overlap, stream)
-                                     : launch_mode<__half, 128, kModeDQR, false>(a, n_tok, err, overlap, stream))
-                   : launch_mode<__half, 128, kModeDKV, false>(a, n_tok, err, overlap, stream);
-    }
+    if (dtype == PLX_BF16)
+        return a.sink ? launch_stage<__nv_bfloat16, true>(a, head_dim, dqr, err, overlap, stream)
+                      : launch_stage<__nv_bfloat16, false>(a, head_dim, dqr, err, overlap, stream);
+    if (dtype == PLX_FP16)
+        return a.sink ? launch_stage<__half, true>(a, head_dim, dqr, err, overlap, stream) : launch_stage<__half, false>(a, head_dim, dqr, err, overlap, stream);
+    return PLX_ERR_UNSUPPORTED;
+}
+
+// Rows of a chunk: about as much work as an item of other keys has, 512 at least (a chunk costs its sums in 32 bits), and some
+// 32 chunks in all at most, which bounds the workspace.
+int train_sink_chunk(int window, int len_q) {
+    const int64_t rows = std::max<int64_t>({512, static_cast<int64_t>(window) + kBM, len_q / 32});
+    return static_cast<int>((rows + kBN - 1) / kBN * kBN);
+}
+
+int launch_train_bwd_join(const TrainArgs &a, int dtype, int head_dim, cudaStream_t stream) {
+    if (dtype == PLX_BF16) return head_dim == 64 ? launch_join<__nv_bfloat16, 64>(a, stream) : launch_join<__nv_bfloat16, 128>(a, stream);
+    if (dtype == PLX_FP16) return head_dim == 64 ? launch_join<__half, 64>(a, stream) : launch_join<__half, 128>(a, stream);
     return PLX_ERR_UNSUPPORTED;
 }
 

@@ -139,6 +139,15 @@ struct TrainArgs {
     int pages_per_seq, page_shift, page_mask, n_pages;
     int batch, heads_q, heads_kv, n_rep, len_q, len_k, window;
     float scale, c2;  // c2 = scale * log2(e)
+    // The first `sink` keys of a sequence stay visible behind a sliding window (0: none, and where there is no window).
+    int sink;
+    // dk/dv with sinks: their key tiles see every row, `sink_chunk` rows an item, which leaves its part in `parts` (null: no
+    // sequence is longer than that)
+    int sink_chunk, sink_slots;
+    float *parts;
+    // all rows of a batch against a prefix that they share (see kPrefix in plx_fwd_sm100.cu): a tile is box_h q heads of a kv
+    // head by box_b batch rows, the keys are cut into n_splits; record (row of q, split) of `parts` is the state of a split
+    int box_h, box_b, n_splits, n_parts;
     int64_t q_sb, q_sh, q_st, kv_sb, kv_sh, kv_st, st_sb, st_sh, st_st;
 };
 
@@ -153,9 +162,10 @@ struct Seq {
 struct Mask {
     int off;     // nk - nq
     int window;  // -1 = off
+    int sink;    // keys in front that stay visible
     __device__ __forceinline__ bool operator()(int i, int j) const {
         int pos = i + off;
-        return j <= pos && (window < 0 || j > pos - window);
+        return j <= pos && (window < 0 || j > pos - window || j < sink);
     }
 };
 

@@ -13,6 +13,7 @@
 // Math: parallax/triton/parallax_decode.py:43-97 (per-key update and final
 // out = O1/d1 * (1 + d2/d1) - O2/d1); partial-state merge:
 // parallax/cute/parallax_decode.py:1107-1136.
+#include <climits>
 #include <atomic>
 #include <mutex>
 #include <type_traits>
@@ -269,11 +270,40 @@ __device__ __forceinline__ void exchange_merge_warp(const DecodeArgs &a, int64_t
 __device__ __forceinline__ void row_range(const DecodeArgs &a, int b, int &lo, int &hi) {
     int hi_g = a.total_len;
     if (a.n_lens) hi_g = min(max(a.lens[b], 1), a.total_len);
-    else if (a.seqused) hi_g = min(max(a.seqused[b], 1), a.total_len);
-    int lo_g = a.cache_start ? max(a.cache_start[b], 0) : 0;
+    else if (a.seqused) hi_g = min(max(a.seqused[b], a.min_len), a.total_len);
+    int lo_g = a.cache_start ? max(a.cache_start[b], 0) : a.first_key;
     if (a.window >= 0) lo_g = max(lo_g, hi_g - a.window);
     lo = min(max(lo_g - a.kv_offset, 0), a.cache_len);
     hi = min(max(hi_g - a.kv_offset, 0), a.cache_len);
+}
+
+// Sinks: the first a.sink keys of a row, from its first valid one on, stay visible behind the window.  A row is swept as ONE
+// range of virtual keys: the sinks are moved up to right in front of the window, and keys below `border` lie `gap` further
+// down in the cache.  With ALIGN = 16 sinks and window each start on a multiple of 16, so that a tile of 16 keys has keys of one kind
+// (and lies in one page); what is then in between, [sink_end, border) and [border, window_lo), is not visible.
+struct SinkMap {
+    int border, gap, sink_end, window_lo;
+};
+template <int ALIGN>
+__device__ __forceinline__ SinkMap sink_range(const DecodeArgs &a, int b, int &lo, int &hi) {
+    row_range(a, b, lo, hi);
+    const int start = min(a.cache_start ? max(a.cache_start[b], 0) : a.first_key, lo), n = min(a.sink, lo - start);
+    SinkMap m{INT_MIN, 0, INT_MIN, lo};
+    if (n == lo - start) {           // nothing is hidden
+        lo = m.window_lo = start;
+        return m;
+    }
+    m.border = lo / ALIGN * ALIGN;
+    lo = m.border - (n + ALIGN - 1) / ALIGN * ALIGN;
+    m.gap = lo - start;
+    m.sink_end = lo + n;
+    return m;
+}
+// the range that is cut into parts
+template <int G, bool SINK>
+__device__ __forceinline__ void sweep_range(const DecodeArgs &a, int b, int &lo, int &hi) {
+    if constexpr (SINK) sink_range<G == 16 ? 16 : 1>(a, b, lo, hi);
+    else row_range(a, b, lo, hi);
 }
 
 // What one of the batch * n_splits slots of a launch (per head) sweeps: part `part` of the `n_parts` into
@@ -291,10 +321,10 @@ __device__ __forceinline__ SplitPlan even_part(const DecodeArgs &a, int b, int p
     const int my_lo = min(lo + part * chunk, hi);
     return SplitPlan{b, part, a.n_splits, my_lo, min(my_lo + chunk, hi), static_cast<int64_t>(b) * a.n_splits * a.heads_q};
 }
-template <int G>
+template <int G, bool SINK>
 __device__ __forceinline__ SplitPlan plan_even(const DecodeArgs &a, int b, int part) {
     int lo, hi;
-    row_range(a, b, lo, hi);
+    sweep_range<G, SINK>(a, b, lo, hi);
     return even_part<G>(a, b, part, lo, hi);
 }
 
@@ -305,7 +335,7 @@ __device__ __forceinline__ SplitPlan plan_even(const DecodeArgs &a, int b, int p
 // ..: up to kBalancedRows rows.  `cap`: the most parts of a row that the merge takes.
 // Not so where the longest row is within a.balanced sixteenths of the mean (see balance_from): dealing out costs the
 // search and leaves parts and rows that no longer fall together with CTAs.
-template <int G>
+template <int G, bool SINK>
 __device__ __forceinline__ SplitPlan plan_slot(const DecodeArgs &a, int slot, int lane, int cap) {
     SplitPlan p{-1, 0, 1, 0, 0, 0};
     constexpr int kRows = kBalancedRows / 32;
@@ -315,7 +345,7 @@ __device__ __forceinline__ SplitPlan plan_slot(const DecodeArgs &a, int slot, in
         start[i] = n[i] = units[i] = 0;
         if (lane + 32 * i < a.batch) {
             int hi;
-            row_range(a, lane + 32 * i, start[i], hi);
+            sweep_range<G, SINK>(a, lane + 32 * i, start[i], hi);
             n[i] = max(hi - start[i], 0);
             units[i] = (n[i] + G - 1) / G;
         }
@@ -414,7 +444,9 @@ static cudaError_t launch_overlapped(void (*kern)(Params...), dim3 grid, int thr
 //
 // DEAL: the slots may be dealt out by length (a.balanced > 0).  A kernel of its own: with the plan of either kind in one,
 // launches without lengths were 0.3 to 0.6 us longer (32 rows of 300 down to 100 keys, 8 : 8 heads, 12.4 -> 13.0).
-template <typename T, int D, int HG, int U, bool SG, bool DEAL>
+//
+// SINK: a kernel of its own too, with the keys of a.sink in front of the window's (see SinkMap).
+template <typename T, int D, int HG, int U, bool SG, bool DEAL, bool SINK = false>
 __global__ void __launch_bounds__(HG * 32, U > 4 ? 1 : 512 / (HG * 32)) decode_kernel(const DecodeArgs a) {
     grid_wait();
     constexpr int LPK = D / 8;      // lanes per key row
@@ -429,12 +461,12 @@ __global__ void __launch_bounds__(HG * 32, U > 4 ? 1 : 512 / (HG * 32)) decode_k
     // the part of a batch row's keys that this warp sweeps
     SplitPlan plan;
     if constexpr (!DEAL) {
-        plan = plan_even<NS>(a, blockIdx.z, SG ? blockIdx.x * HG + warp : blockIdx.x);
+        plan = plan_even<NS, SINK>(a, blockIdx.z, SG ? blockIdx.x * HG + warp : blockIdx.x);
     } else {
         // the warps of a CTA have one slot: one of them plans (all eight, they queued for the divisions)
         __shared__ SplitPlan s_plan;
         if (warp == 0) {
-            plan = plan_slot<NS>(a, blockIdx.z * a.n_splits + blockIdx.x, lane, a.n_groups ? 32 * a.n_groups : 32);
+            plan = plan_slot<NS, SINK>(a, blockIdx.z * a.n_splits + blockIdx.x, lane, a.n_groups ? 32 * a.n_groups : 32);
             if (lane == 0) s_plan = plan;
         }
         __syncthreads();
@@ -443,6 +475,11 @@ __global__ void __launch_bounds__(HG * 32, U > 4 ? 1 : 512 / (HG * 32)) decode_k
     }
     const int b = plan.b, my_lo = plan.lo, my_hi = plan.hi;
     const int n_iter = (my_hi - my_lo + NS * U - 1) / (NS * U);
+    SinkMap sinks{INT_MIN, 0, 0, 0};
+    if constexpr (SINK) {
+        int lo, hi;
+        sinks = sink_range<1>(a, b, lo, hi);
+    }
 
     // this lane's 8 channels of q and r
     float qf[8], rf[8];
@@ -473,8 +510,9 @@ __global__ void __launch_bounds__(HG * 32, U > 4 ? 1 : 512 / (HG * 32)) decode_k
         const int base = my_lo + it * NS * U + sid;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int kj = base + u * NS;
+            int kj = base + u * NS;
             if (kj < my_hi) {
+                if (SINK && kj < sinks.border) kj -= sinks.gap;
                 const int64_t at = decltype(paged_tag)::value ? paged_key_offset(a, b, kj) : static_cast<int64_t>(kj) * a.kv_st;
                 const T *pk = kp + at, *pv = vp + at;
                 kr[u] = ld_stream16(pk);
@@ -579,7 +617,7 @@ __global__ void __launch_bounds__(HG * 32, U > 4 ? 1 : 512 / (HG * 32)) decode_k
     auto emit = [&](float M, float D1, float D2, const float (&O1)[8], const float (&O2)[8]) {
         if (!writer) return;
         if (a.part_out) {
-            float *rec = a.part_out + bh * REC;
+            float *rec = a.part_out + bh * a.part_stride * REC;
             if (lane == 0) {
                 rec[0] = M;
                 rec[1] = D1;
@@ -693,7 +731,7 @@ __global__ void __launch_bounds__(HG * 32, U > 4 ? 1 : 512 / (HG * 32)) decode_k
             if (c == 0) a.ws_counters[bh] = 0;  // ready for the next launch on this workspace
         }
         if (a.part_out) {
-            float *rec = a.part_out + bh * REC;
+            float *rec = a.part_out + bh * a.part_stride * REC;
             if (c == 0) *reinterpret_cast<float4 *>(rec) = make_float4(M, S1, S2, 0.f);
             if (active) rec[4 + c] = A;
         } else {
@@ -766,7 +804,7 @@ __global__ void __launch_bounds__(HG * 32, U > 4 ? 1 : 512 / (HG * 32)) decode_k
     if (a.xch.world > 0) {
         exchange_merge_warp<T, D>(a, bh, lane, big, D1, D2, O1, O2);
     } else if (a.part_out) {
-        float *rec = a.part_out + bh * REC;
+        float *rec = a.part_out + bh * a.part_stride * REC;
         if (lane == 0) *reinterpret_cast<float4 *>(rec) = make_float4(big, D1, D2, 0.f);
 #pragma unroll
         for (int e = 0; e < CH; ++e) {
@@ -955,7 +993,9 @@ struct GqaSmem {
 // MMAs, with none of them on rows of zeros, and half the registers for accumulators and fragments (in all 190 to 201 at
 // head_dim 128, where the other form fills 255); a movmatrix per 8 x 8 block turns P^T around.
 // B = 16, 1024 keys, 32 : 8 heads 16.7 -> 16.0 us, B = 8, 4000 keys, rows of different lengths 40.8 -> 34.0.
-template <typename T, int D, bool PAGED, bool FEW>
+//
+// SINK: see SinkMap; a tile holds sinks or keys of the window, and rows of it that are not visible are zeroed and masked.
+template <typename T, int D, bool PAGED, bool FEW, bool SINK = false>
 __global__ void __launch_bounds__(kGqaWarps * 32, 1) decode_gqa_kernel(const DecodeArgs a, int n_hgroups) {
     grid_wait();
     constexpr int LD = D + 8;                       // padded row: ldmatrix without bank conflicts
@@ -974,7 +1014,7 @@ __global__ void __launch_bounds__(kGqaWarps * 32, 1) decode_gqa_kernel(const Dec
     const int hunit = blockIdx.x % n_hunits, cta = blockIdx.x / n_hunits, slot = cta * kGqaWarps + warp;
     const int hk = hunit / n_hgroups, hgrp = hunit % n_hgroups;
     SplitPlan plan{-1, 0, 0, 0, 0, 0};
-    if (slot < n_slots) plan = a.balanced ? plan_slot<kGqaTile>(a, slot, lane, n_slots) : plan_even<kGqaTile>(a, slot / a.n_splits, slot % a.n_splits);
+    if (slot < n_slots) plan = a.balanced ? plan_slot<kGqaTile, SINK>(a, slot, lane, n_slots) : plan_even<kGqaTile, SINK>(a, slot / a.n_splits, slot % a.n_splits);
     const int b = max(plan.b, 0), my_lo = plan.lo, my_hi = plan.b < 0 ? plan.lo : plan.hi;
     const int n_tiles = (my_hi - my_lo + kGqaTile - 1) / kGqaTile;
     const int hq0 = hk * a.n_rep + hgrp * 16;       // first q head of this CTA's rows
@@ -983,6 +1023,15 @@ __global__ void __launch_bounds__(kGqaWarps * 32, 1) decode_gqa_kernel(const Dec
     auto sK = [&](int st) -> uint32_t { return sbase + st * 2 * kTileBytes; };
     auto sV = [&](int st) -> uint32_t { return sbase + st * 2 * kTileBytes + kTileBytes; };
     if (lane == 0) s_row[warp] = plan.b;
+    SinkMap sinks{INT_MIN, 0, 0, 0};
+    if constexpr (SINK) {
+        int lo, hi;
+        sinks = sink_range<kGqaTile>(a, b, lo, hi);
+    }
+    // visible keys of a tile
+    auto first_of = [&](int tile0) { return SINK && tile0 >= sinks.border ? sinks.window_lo : INT_MIN; };
+    auto end_of = [&](int tile0) { return SINK && tile0 < sinks.border ? min(my_hi, sinks.sink_end) : my_hi; };
+    auto visible = [&](int key, int first, int end) { return key < end && (!SINK || key >= first); };
 
     // Tile i of this warp -> stage i % kGqaStages.  A lane copies the same 16-byte column of every
     // (32 / CPR)-th row, so its source and destination advance by constants; rows past my_hi (last tile
@@ -991,7 +1040,7 @@ __global__ void __launch_bounds__(kGqaWarps * 32, 1) decode_gqa_kernel(const Dec
     // read ahead.
     constexpr int RPI = 32 / CPR;                                  // rows covered by one instruction of the warp
     const int my_row = lane / CPR, my_col = lane % CPR;
-    const bool page_per_tile = PAGED && a.page_mask + 1 >= kGqaTile && my_lo % kGqaTile == 0;
+    const bool page_per_tile = PAGED && a.page_mask + 1 >= kGqaTile && my_lo % kGqaTile == 0 && (!SINK || sinks.gap % kGqaTile == 0);
     const T *kp = static_cast<const T *>(a.k) + (PAGED ? 0 : b * a.kv_sb) + hk * a.kv_sh + my_col * 8;
     const T *vp = static_cast<const T *>(a.v) + (PAGED ? 0 : b * a.kv_sb) + hk * a.kv_sh + my_col * 8;
     const uint32_t my_dst = (my_row * LD + my_col * 8) * 2;
@@ -999,19 +1048,24 @@ __global__ void __launch_bounds__(kGqaWarps * 32, 1) decode_gqa_kernel(const Dec
     // two where registers are short (B = 64, 4096 keys, 16 : 1 heads, pages, 34.0 us, three 35.8).
     constexpr int kPages = FEW ? kGqaStages : 2;
     uint32_t next_page[kPages];
-    auto page_of_tile = [&](int i) -> uint32_t { return page_per_tile && i < n_tiles ? paged_key_page(a, b, my_lo + i * kGqaTile) : 0u; };
+    auto in_cache = [&](int key, int tile0) { return SINK && tile0 < sinks.border ? key - sinks.gap : key; };
+    auto page_of_tile = [&](int i) -> uint32_t {
+        const int tile0 = my_lo + i * kGqaTile;
+        return page_per_tile && i < n_tiles ? paged_key_page(a, b, in_cache(tile0, tile0)) : 0u;
+    };
     if (PAGED)
 #pragma unroll
         for (int i = 0; i < kPages; ++i) next_page[i] = page_of_tile(i);
     auto load_tile = [&](int i) {
         if (i < n_tiles) {
-            const int st = i % kGqaStages, tile0 = my_lo + i * kGqaTile, key0 = tile0 + my_row;
+            const int st = i % kGqaStages, tile0 = my_lo + i * kGqaTile, key0 = tile0 + my_row, first = first_of(tile0), end = end_of(tile0);
             const uint32_t dk = sK(st) + my_dst, dv = sV(st) + my_dst;
-            const bool whole = tile0 + kGqaTile <= my_hi;
+            const bool whole = tile0 + kGqaTile <= end && (!SINK || tile0 >= first);
+            const int at0 = in_cache(key0, tile0);           // of the lane's first key
             if (!PAGED || page_per_tile) {
                 const int64_t step = static_cast<int64_t>(RPI) * a.kv_st;
-                const int64_t at = page_per_tile ? static_cast<int64_t>(next_page[0]) * a.kv_sb + static_cast<int64_t>(key0 & a.page_mask) * a.kv_st
-                                                 : static_cast<int64_t>(key0) * a.kv_st;
+                const int64_t at = page_per_tile ? static_cast<int64_t>(next_page[0]) * a.kv_sb + static_cast<int64_t>(at0 & a.page_mask) * a.kv_st
+                                                 : static_cast<int64_t>(at0) * a.kv_st;
                 if (PAGED) {
 #pragma unroll
                     for (int n = 1; n < kPages; ++n) next_page[n - 1] = next_page[n];
@@ -1026,7 +1080,7 @@ __global__ void __launch_bounds__(kGqaWarps * 32, 1) decode_gqa_kernel(const Dec
                 } else {
 #pragma unroll
                     for (int j = 0; j < kGqaTile / RPI; ++j) {
-                        const bool in = key0 + j * RPI < my_hi;
+                        const bool in = visible(key0 + j * RPI, first, end);
                         cp_async16(dk + j * RPI * LD * 2, kp + (in ? at + j * step : 0), in ? 16 : 0);
                         cp_async16(dv + j * RPI * LD * 2, vp + (in ? at + j * step : 0), in ? 16 : 0);
                     }
@@ -1034,8 +1088,8 @@ __global__ void __launch_bounds__(kGqaWarps * 32, 1) decode_gqa_kernel(const Dec
             } else {
 #pragma unroll
                 for (int j = 0; j < kGqaTile / RPI; ++j) {
-                    const bool in = whole || key0 + j * RPI < my_hi;
-                    const int64_t at = in ? paged_key_offset(a, b, key0 + j * RPI) : 0;
+                    const bool in = whole || visible(key0 + j * RPI, first, end);
+                    const int64_t at = in ? paged_key_offset(a, b, at0 + j * RPI) : 0;
                     cp_async16(dk + j * RPI * LD * 2, kp + at, in ? 16 : 0);
                     cp_async16(dv + j * RPI * LD * 2, vp + at, in ? 16 : 0);
                 }
@@ -1105,7 +1159,7 @@ __global__ void __launch_bounds__(kGqaWarps * 32, 1) decode_gqa_kernel(const Dec
         for (int e = 0; e < 4; ++e) o1[i][e] = o2[i][e] = 0.f;
 
     for (int i = 0; i < n_tiles; ++i) {
-        const int st = i % kGqaStages, key0 = my_lo + i * kGqaTile;
+        const int st = i % kGqaStages, key0 = my_lo + i * kGqaTile, first = first_of(key0), end = end_of(key0);
         cp_async_wait<kGqaStages - 1>();
         __syncwarp();                    // tile i has landed for every lane
 
@@ -1123,8 +1177,8 @@ __global__ void __launch_bounds__(kGqaWarps * 32, 1) decode_gqa_kernel(const Dec
             float alpha[2], m_safe[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                s1[e] = key0 + g < my_hi ? s1[e] * a.c2 : -INFINITY;
-                s1[2 + e] = key0 + g + 8 < my_hi ? s1[2 + e] * a.c2 : -INFINITY;
+                s1[e] = visible(key0 + g, first, end) ? s1[e] * a.c2 : -INFINITY;
+                s1[2 + e] = visible(key0 + g + 8, first, end) ? s1[2 + e] * a.c2 : -INFINITY;
                 float mx = fmaxf(s1[e], s1[2 + e]);
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
@@ -1191,7 +1245,7 @@ __global__ void __launch_bounds__(kGqaWarps * 32, 1) decode_gqa_kernel(const Dec
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int key = key0 + nb * 8 + 2 * t + (e & 1);
-                s1[nb][e] = key < my_hi ? s1[nb][e] * a.c2 : -INFINITY;
+                s1[nb][e] = visible(key, first, end) ? s1[nb][e] * a.c2 : -INFINITY;
                 mx[e >> 1] = fmaxf(mx[e >> 1], s1[nb][e]);
             }
         uint32_t pa1[4], pa2[4];
@@ -1301,7 +1355,7 @@ __global__ void __launch_bounds__(kGqaWarps * 32, 1) decode_gqa_kernel(const Dec
     float big = -INFINITY, D1 = 0.f, D2 = 0.f, O1[CH], O2[CH];
     auto emit = [&](int64_t bh) {
         if (a.part_out) {
-            float *rec = a.part_out + bh * REC;
+            float *rec = a.part_out + bh * a.part_stride * REC;
             if (lane == 0) *reinterpret_cast<float4 *>(rec) = make_float4(big, D1, D2, 0.f);
 #pragma unroll
             for (int e = 0; e < CH; ++e) {
@@ -1384,11 +1438,11 @@ __global__ void __launch_bounds__(kGqaWarps * 32, 1) decode_gqa_kernel(const Dec
     if (warp == w0 && lane == 0) a.ws_counters[bh_of(0)] = 0;   // ready for the next launch on this workspace
 }
 
-template <typename T, int D, bool PAGED, bool FEW>
+template <typename T, int D, bool PAGED, bool FEW, bool SINK>
 static int launch_decode_gqa(const DecodeArgs &a, cudaStream_t stream) {
     const int n_hgroups = (a.n_rep + 15) / 16;
     constexpr int kSmem = kGqaWarps * GqaSmem<D>::kPerWarp;
-    auto kern = decode_gqa_kernel<T, D, PAGED, FEW>;
+    auto kern = decode_gqa_kernel<T, D, PAGED, FEW, SINK>;
     {   // the shared-memory opt-in is a per-device function attribute: set it once per device
         constexpr int kMaxDevices = 64;
         static std::mutex mu;
@@ -1414,7 +1468,10 @@ template <typename T, int D, int HG>
 static int launch_decode_hg(const DecodeArgs &a, cudaStream_t stream) {
     constexpr int U = 4;  // key rows per stream and register buffer (two buffers: 8 rows of K and of V in flight)
     dim3 grid(a.n_splits, a.heads_q / HG, a.batch);
-    auto kern = a.balanced ? decode_kernel<T, D, HG, U, false, true> : decode_kernel<T, D, HG, U, false, false>;
+    // (with sinks the rows are as long as the window, most of them: never dealt out by length)
+    auto kern = a.sink       ? decode_kernel<T, D, HG, U, false, false, true>
+                : a.balanced ? decode_kernel<T, D, HG, U, false, true>
+                             : decode_kernel<T, D, HG, U, false, false>;
     const cudaError_t st = launch_overlapped(kern, grid, HG * 32, 0, stream, a);
     count_launch();
     return st == cudaSuccess && cudaGetLastError() == cudaSuccess ? PLX_OK : PLX_ERR_LAUNCH;
@@ -1441,7 +1498,7 @@ static int tma_free_sm_count() {
 // split, whose CTAs read contiguous memory.
 static bool decode_split_groups(const DecodeArgs &a) {
     const int64_t bh = static_cast<int64_t>(a.batch) * a.heads_q;
-    const int64_t n_keys = a.window >= 0 && a.window < a.cache_len ? a.window : a.cache_len;
+    const int64_t n_keys = a.active_keys();
     return a.n_rep == 1 && a.n_splits >= 8 && a.n_splits % 8 == 0 && a.n_splits <= 256 &&
            bh <= PLX_DECODE_SPLIT_GROUP_MAX_BH && bh * n_keys <= (static_cast<int64_t>(1) << 19);
 }
@@ -1489,19 +1546,26 @@ static int launch_decode_sg(const DecodeArgs &a, cudaStream_t stream) {
         }
         roomy = roomy && units <= n;
     }
-    auto kern = roomy ? decode_kernel<T, D, 8, 8, true, false> : decode_kernel<T, D, 8, 4, true, false>;
+    auto kern = a.sink  ? (roomy ? decode_kernel<T, D, 8, 8, true, false, true> : decode_kernel<T, D, 8, 4, true, false, true>)
+                : roomy ? decode_kernel<T, D, 8, 8, true, false>
+                        : decode_kernel<T, D, 8, 4, true, false>;
     cfg.numAttrs = cluster ? 2 : 1;
     cudaError_t st = cudaLaunchKernelEx(&cfg, kern, a);
     count_launch();
     return st == cudaSuccess && cudaGetLastError() == cudaSuccess ? PLX_OK : PLX_ERR_LAUNCH;
 }
 
+template <typename T, int D, bool SINK>
+static int launch_decode_grouped(const DecodeArgs &a, cudaStream_t stream) {
+    if (a.n_rep > 8)
+        return a.page_table ? launch_decode_gqa<T, D, true, false, SINK>(a, stream) : launch_decode_gqa<T, D, false, false, SINK>(a, stream);
+    return a.page_table ? launch_decode_gqa<T, D, true, true, SINK>(a, stream) : launch_decode_gqa<T, D, false, true, SINK>(a, stream);
+}
+
 template <typename T, int D>
 static int launch_decode_t(const DecodeArgs &a, cudaStream_t stream) {
-    if (a.n_rep > 8)    // grouped heads: tensor-core kernel
-        return a.page_table ? launch_decode_gqa<T, D, true, false>(a, stream) : launch_decode_gqa<T, D, false, false>(a, stream);
-    if (a.n_rep >= 2)
-        return a.page_table ? launch_decode_gqa<T, D, true, true>(a, stream) : launch_decode_gqa<T, D, false, true>(a, stream);
+    if (a.n_rep >= 2)    // grouped heads: tensor-core kernel
+        return a.sink ? launch_decode_grouped<T, D, true>(a, stream) : launch_decode_grouped<T, D, false>(a, stream);
     if (decode_split_groups(a)) return launch_decode_sg<T, D>(a, stream);
     // adjacent q heads share a CTA (one warp each): the largest group that divides the head count
     if (a.heads_q % 8 == 0) return launch_decode_hg<T, D, 8>(a, stream);
@@ -1531,12 +1595,12 @@ static int balance_from(const DecodeArgs &a, int head_dim) {
     if ((!a.seqused && !a.n_lens && !a.cache_start) || a.batch < 2 || a.batch > kBalancedRows || a.n_splits < 2 || a.part_out || a.xch.world != 0 ||
         decode_split_groups(a))
         return 0;
-    const int64_t n_keys = a.window >= 0 && a.window < a.cache_len ? a.window : a.cache_len, part = n_keys / a.n_splits * head_dim;
+    const int64_t n_keys = a.active_keys(), part = n_keys / a.n_splits * head_dim;
     if (a.n_rep > 1) {
         const bool rows_end_with_ctas = a.n_splits % kGqaWarps == 0 || kGqaWarps % a.n_splits == 0;
         return part < 384 * 128 && rows_end_with_ctas ? 32 : 17;
     }
-    if (part < 64 * 128) return 0;
+    if (part < 64 * 128 || a.sink) return 0;
     const bool one_wave = static_cast<int64_t>(a.batch) * a.heads_q * a.n_splits <= 16 * static_cast<int64_t>(tma_free_sm_count());
     return part < 100 * 128 || a.n_splits < 4 || !one_wave ? 32 : 17;
 }
@@ -1603,6 +1667,40 @@ int launch_decode_merge(const float *parts, int n_parts, int n_records, int head
         if (head_dim == 64) return launch_merge_t<__half, 64>(parts, n_parts, n_records, out, stream);
     }
     return PLX_ERR_UNSUPPORTED;
+}
+
+// ========================================================================= //
+// A batch behind a shared prefix: the states of the prefix's splits and of the row's own keys, n_parts <= 32 records in a row for
+// each (batch, head), -> out.  One warp each; bound by one round trip to the L2.
+// ========================================================================= //
+template <typename T, int D>
+__global__ void __launch_bounds__(128) prefix_merge_kernel(const float *parts, int n_parts, int64_t n_rows, void *out) {
+    constexpr int REC = 2 * D + 4, CH = D / 32;
+    grid_wait();
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (row >= n_rows) return;
+    float big, D1, D2, O1[CH], O2[CH];
+    warp_merge<D, 8, true>(parts + row * n_parts * REC, n_parts, lane, big, D1, D2, O1, O2);
+    T *dst = static_cast<T *>(out) + row * D + lane * CH;
+#pragma unroll
+    for (int e = 0; e < CH; e += 2)
+        *reinterpret_cast<uint32_t *>(dst + e) = Elem<T>::pack(finalize(D1, D2, O1[e], O2[e]), finalize(D1, D2, O1[e + 1], O2[e + 1]));
+}
+
+template <typename T, int D>
+static int launch_prefix_merge_t(const float *parts, int n_parts, int64_t n_rows, void *out, cudaStream_t stream) {
+    const cudaError_t st = launch_overlapped(prefix_merge_kernel<T, D>, dim3(static_cast<unsigned>((n_rows + 3) / 4)), 128, 0, stream, parts, n_parts, n_rows, out);
+    count_launch();
+    return st == cudaSuccess && cudaGetLastError() == cudaSuccess ? PLX_OK : PLX_ERR_LAUNCH;
+}
+
+int launch_prefix_merge(const float *parts, int n_parts, int64_t n_rows, int head_dim, int dtype, void *out, cudaStream_t stream) {
+    if (dtype == PLX_BF16)
+        return head_dim == 128 ? launch_prefix_merge_t<__nv_bfloat16, 128>(parts, n_parts, n_rows, out, stream)
+                               : launch_prefix_merge_t<__nv_bfloat16, 64>(parts, n_parts, n_rows, out, stream);
+    return head_dim == 128 ? launch_prefix_merge_t<__half, 128>(parts, n_parts, n_rows, out, stream)
+                           : launch_prefix_merge_t<__half, 64>(parts, n_parts, n_rows, out, stream);
 }
 
 }  // namespace plx

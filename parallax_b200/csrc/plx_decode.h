@@ -20,7 +20,8 @@ constexpr int kBalancedRows = 128;   // most batch rows whose splits are dealt o
 struct DecodeArgs {
     const void *q, *r, *k, *v;
     void *out;         // (batch, heads_q, D) or nullptr
-    float *part_out;   // nullptr, or one partial-state record per (batch, head) instead of `out`
+    float *part_out;   // nullptr, or one partial-state record per (batch, head) instead of `out`,
+    int part_stride;   // every part_stride-th one
     const int32_t *seqused, *cache_start;
     float *ws_parts;   // (batch * heads_q, n_splits) partial records
     int *ws_counters;  // (batch * heads_q) arrival counters, zero between launches
@@ -29,6 +30,8 @@ struct DecodeArgs {
     int n_groups;      // 0: single-level merge
     int balanced;      // splits dealt out to the batch rows by length, from this skew on; 0: never (see plan_slot)
     int batch, heads_q, heads_kv, n_rep, cache_len, window, n_splits, kv_offset, total_len;
+    int sink;          // keys in front that stay visible behind the window (0 without one)
+    int first_key, min_len;   // keys before first_key are another launch's (0); lengths below min_len count as it (1)
     float c2;  // qk_scale * log2(e)
     int64_t kv_sb, kv_st, kv_sh;   // paged: kv_sb is the stride between pages
     // paged cache (page_table != nullptr): key j of batch row b lives in page
@@ -45,6 +48,11 @@ struct DecodeArgs {
     // Fused sweep + exchange (xch.world >= 1): the warp that holds the merged state of a (batch, head) does
     // not write a partial record but pushes it to every rank's inbox, waits for the peers' and merges.
     ExchangeArgs xch;
+    // the most keys that a row sweeps
+    int active_keys() const {
+        const int64_t n = window >= 0 ? static_cast<int64_t>(window) + sink : cache_len;
+        return static_cast<int>((n < cache_len ? n : cache_len) - (window >= 0 ? 0 : first_key));
+    }
 };
 
 }  // namespace plx

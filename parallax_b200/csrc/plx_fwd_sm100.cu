@@ -62,6 +62,14 @@ constexpr uint32_t kQPanel = kBM * 128;       // bytes of one 64-channel panel o
 constexpr uint32_t kKVPanel = kBN * 128;
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleThreshold = 8.f;
+// What a launch is.  The training forward; several query rows per sequence against a KV cache; both with sinks (the first
+// a.sink keys stay visible behind the window: an item streams their tiles, then those of its window); a batch's rows against a
+// prefix that they share, which leaves the un-normalised state of its share of the keys.
+constexpr int kTrain = 0, kExtend = 1, kTrainSink = 2, kExtendSink = 3, kPrefix = 4;
+template <int MODE>
+constexpr bool kIsExtend = MODE == kExtend || MODE == kExtendSink || MODE == kPrefix;
+template <int MODE>
+constexpr bool kHasSinks = MODE == kTrainSink || MODE == kExtendSink;
 constexpr int kMinPage = 8;                   // smallest page a tile can be copied from: boxes start on 1024-byte boundaries (8 rows)
 
 template <typename T>
@@ -99,20 +107,42 @@ struct Smem {
 // One unit of work: a 128-row query tile of one (batch, q head).
 struct Item {
     int bos, nq, nk, r0, b, h, hk, off, t_lo, n_tiles;   // key tiles t_lo .. t_lo + n_tiles - 1
-    int valid, pad;
+    int valid;
+    int extra;      // sinks: the first `extra` tiles are 0 .. extra - 1 instead; prefix: the split
 };
+
+// first key of the j-th tile of an item
+template <int MODE>
+__device__ __forceinline__ int tile_key(const Item &it, int j) {
+    return (kHasSinks<MODE> ? (j < it.extra ? j : it.t_lo + j - it.extra) : it.t_lo + j) * kBN;
+}
 
 // Work item `idx` of the launch.  Items are ordered (batch, head)-major so that CTAs running at the
 // same time share K / V in L2; inside a (batch, head) the row tiles alternate last, first, last - 1,
 // second, ... so that under a causal mask any two neighbours add up to the same work.
 // (Handed out by the hardware, DYN, they go from last to first: see longest_first.)
-template <bool EXT, bool DYN>
+template <int MODE, bool DYN>
 __device__ __forceinline__ Item get_item(const TrainArgs &a, int idx, int n_rt, int group) {
     Item it;
+    if (MODE == kPrefix) {
+        // tiles of rows fastest: those that run together read the same keys
+        const int rt = idx % n_rt, n_rt_h = (a.n_rep + a.box_h - 1) / a.box_h, rest = idx / n_rt, tiles = (a.len_k + kBN - 1) / kBN;
+        it.bos = it.r0 = 0;
+        it.nq = kBM;
+        it.nk = it.off = a.len_k;
+        it.h = rt % n_rt_h * a.box_h;
+        it.b = rt / n_rt_h * a.box_b;
+        it.hk = rest % a.heads_kv;
+        it.extra = rest / a.heads_kv;
+        it.t_lo = static_cast<int>(static_cast<int64_t>(it.extra) * tiles / a.n_splits);
+        it.n_tiles = static_cast<int>(static_cast<int64_t>(it.extra + 1) * tiles / a.n_splits) - it.t_lo;
+        it.valid = 1;
+        return it;
+    }
     int bh = idx / n_rt, k = idx % n_rt;
     if (DYN) longest_first(idx, n_rt, a.batch * a.heads_q, group, bh, k);
     const int tile_id = DYN ? n_rt - 1 - k : (k & 1) ? (k >> 1) : n_rt - 1 - (k >> 1);
-    it.pad = 0;
+    it.extra = 0;
     Seq s;
     int tis = 0;
     it.valid = locate_tile(a, tile_id, kBM, s, tis);
@@ -123,7 +153,7 @@ __device__ __forceinline__ Item get_item(const TrainArgs &a, int idx, int n_rt, 
     if (it.valid && it.r0 >= it.nq) it.valid = false;
     it.b = bh / a.heads_q;
     // a row's own active length, kept inside what the tensor map (or the page table) covers
-    if (EXT && a.seqused) it.nk = min(max(__ldg(a.seqused + it.b), it.nq), a.len_k);
+    if (kIsExtend<MODE> && a.seqused) it.nk = min(max(__ldg(a.seqused + it.b), it.nq), a.len_k);
     it.h = bh % a.heads_q;
     it.hk = it.h / a.n_rep;
     it.off = it.nk - it.nq;
@@ -132,6 +162,11 @@ __device__ __forceinline__ Item get_item(const TrainArgs &a, int idx, int n_rt, 
     const int lo_col = a.window < 0 ? 0 : max(0, it.r0 + it.off - a.window + 1);
     it.t_lo = lo_col / kBN;
     it.n_tiles = (it.valid && hi_col > lo_col) ? (hi_col + kBN - 1) / kBN - it.t_lo : 0;
+    if (kHasSinks<MODE> && it.valid && hi_col > 0) {
+        const int sinks = (min(a.sink, hi_col) + kBN - 1) / kBN;
+        it.extra = it.n_tiles > 0 ? min(sinks, it.t_lo) : sinks;      // (a window of 0 may leave nothing but sinks)
+        it.n_tiles += it.extra;
+    }
     return it;
 }
 
@@ -153,13 +188,14 @@ __device__ __forceinline__ int item_index(int n, int chunk_shift) {
 // Dealt out in advance every role finds its items by itself, in a kernel of its own without ring and launch control: a
 // launch of one small item per CTA is bound by latency, and through the ring it was slower (B = 16, H = 8, L = 100, D = 64:
 // 8.9 -> 9.5 us).
-template <typename T, int D, int NS, bool EXT, bool DYN>
+template <typename T, int D, int NS, int MODE, bool DYN>
 __global__ void __launch_bounds__(352, 1)
 fwd_sm100_kernel(const TrainArgs a, const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_r,
                  const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const ErrSink sink, int n_rt,
                  int n_items, int chunk_shift, int group) {
     using L = Smem<D, NS>;
     constexpr uint32_t kQBytes = L::kQBytes, kKVBytes = L::kKVBytes;
+    constexpr bool EXT = kIsExtend<MODE>, SINK = kHasSinks<MODE>, PART = MODE == kPrefix;
     extern __shared__ unsigned char smem_raw[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -226,7 +262,7 @@ fwd_sm100_kernel(const TrainArgs a, const __grid_constant__ CUtensorMap tm_q, co
             }
             clc_ask(base + L::kClc, bar(L::kClcFull));
             src.asked = src.taken;
-            it = get_item<EXT, DYN>(a, idx, n_rt, group);
+            it = get_item<MODE, DYN>(a, idx, n_rt, group);
             if (it.valid) return true;
         }
     };
@@ -243,7 +279,7 @@ fwd_sm100_kernel(const TrainArgs a, const __grid_constant__ CUtensorMap tm_q, co
                 const int idx = item_index(taken++, chunk_shift);
                 it.valid = 0;
                 if (idx >= n_items) return true;
-                it = get_item<EXT, DYN>(a, idx, n_rt, group);
+                it = get_item<MODE, DYN>(a, idx, n_rt, group);
                 if (it.valid) return true;
             }
         }
@@ -282,16 +318,19 @@ fwd_sm100_kernel(const TrainArgs a, const __grid_constant__ CUtensorMap tm_q, co
                     // the q / r tiles of the previous item are free once its last score product has completed
                     ok = mbar_wait(bar(L::kQEmpty), (n_items_done & 1) ^ 1, err, 1);
                     if (!ok) break;
-                    mbar_expect_tx(bar(L::kQFull), 2 * kQBytes);
+                    mbar_expect_tx(bar(L::kQFull), PART ? 2u * L::kPanels * 128u * a.box_h * a.box_b : 2 * kQBytes);
 #pragma unroll
                     for (int pn = 0; pn < L::kPanels; ++pn) {
-                        tma_load_4d(sQ + pn * kQPanel, &tm_q, bar(L::kQFull), 64 * pn, it.bos + it.r0, it.h, it.b);
-                        tma_load_4d(sR + pn * kQPanel, &tm_r, bar(L::kQFull), 64 * pn, it.bos + it.r0, it.h, it.b);
+                        // (prefix: box_h heads by box_b batch rows, heads first; what rows of the tile are left over hold
+                        // anything, and only they see it)
+                        const int c1 = PART ? it.h : it.bos + it.r0, c2 = PART ? it.hk : it.h;
+                        tma_load_4d(sQ + pn * kQPanel, &tm_q, bar(L::kQFull), 64 * pn, c1, c2, it.b);
+                        tma_load_4d(sR + pn * kQPanel, &tm_r, bar(L::kQFull), 64 * pn, c1, c2, it.b);
                     }
                 }
                 ++n_items_done;
                 for (int j = 0; j < it.n_tiles; ++j) {
-                    const int key0 = (it.t_lo + j) * kBN;
+                    const int key0 = tile_key<MODE>(it, j), kb = PART ? 0 : it.b;
                     int page[kMaxBoxes];
                     if (EXT && a.page_table) {
                         // the tile's page numbers, read before the wait so that their latency is hidden by it
@@ -299,7 +338,7 @@ fwd_sm100_kernel(const TrainArgs a, const __grid_constant__ CUtensorMap tm_q, co
                         for (int i = 0; i < kMaxBoxes; ++i) {
                             const int key = key0 + (i << box_shift);
                             page[i] = (i << box_shift) < kBN && key < it.nk
-                                          ? __ldg(a.page_table + static_cast<int64_t>(it.b) * a.pages_per_seq + (key >> a.page_shift)) : 0;
+                                          ? __ldg(a.page_table + static_cast<int64_t>(kb) * a.pages_per_seq + (key >> a.page_shift)) : 0;
                         }
                     }
                     ok = mbar_wait(bar(empty0 + s), ph ^ 1, err, is_k ? 2 : 3);
@@ -323,7 +362,7 @@ fwd_sm100_kernel(const TrainArgs a, const __grid_constant__ CUtensorMap tm_q, co
                         mbar_expect_tx(full, kKVBytes);
 #pragma unroll
                         for (int pn = 0; pn < L::kPanels; ++pn)
-                            tma_load_4d(dst + pn * kKVPanel, map, full, 64 * pn, it.bos + key0, it.hk, it.b);
+                            tma_load_4d(dst + pn * kKVPanel, map, full, 64 * pn, it.bos + key0, it.hk, kb);
                     }
                     if (tail) {
                         ok = mbar_wait(full, n_tails & 1, err, is_k ? 17 : 18);
@@ -520,7 +559,7 @@ fwd_sm100_kernel(const TrainArgs a, const __grid_constant__ CUtensorMap tm_q, co
             // multiply V, so that bart * barv - O2 / d1 = sum_j P2_j (barv - v_j) / d1 cancels as in exact
             // arithmetic (a row with a single key returns v exactly).  The saved statistics are always the
             // fp32 sums, which is what the backward recomputes.
-            const bool exact_norm = (r0 + off < kBN) || (a.window >= 0 && a.window <= 2 * kBN);
+            const bool exact_norm = PART ? nk <= 2 * kBN : (r0 + off < kBN) || (a.window >= 0 && a.window + (SINK ? a.sink : 0) <= 2 * kBN);
             float d1r[2] = {0.f, 0.f}, d2r[2] = {0.f, 0.f};
 
             for (int j = 0; j < it.n_tiles; ++j, ++g) {
@@ -538,21 +577,22 @@ fwd_sm100_kernel(const TrainArgs a, const __grid_constant__ CUtensorMap tm_q, co
                     mbar_arrive(bar(L::kSFree));                 // the next score products may overwrite S1 / S2
                 }
 
-                const int c0 = (it.t_lo + j) * kBN;
-                const bool need_mask = (c0 + kBN - 1 > r0 + off) || (c0 + kBN > nk) ||
-                                       (a.window >= 0 && c0 < r0 + kBM + off - a.window);
+                const int c0 = tile_key<MODE>(it, j);
+                const bool need_mask = PART ? c0 + kBN > nk
+                                            : (c0 + kBN - 1 > r0 + off) || (c0 + kBN > nk) ||
+                                                  (a.window >= 0 && c0 < r0 + kBM + off - a.window && !(SINK && c0 + kBN <= a.sink));
                 if (need_mask) {
 #pragma unroll
                     for (int hh = 0; hh < 2; ++hh) {
                         const int pos = r0 + rl0 + 8 * hh + off;
-                        const int last = min(pos, nk - 1);                        // last visible key of the row
-                        const int first = a.window < 0 ? 0 : pos - a.window + 1;  // first visible key of the row
+                        const int last = PART ? nk - 1 : min(pos, nk - 1);        // last visible key of the row
+                        const int first = PART || a.window < 0 ? 0 : pos - a.window + 1;   // first visible key of the row
 #pragma unroll
                         for (int k = 0; k < 8; ++k)
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
                                 const int c = c0 + 8 * k + 2 * t + e;
-                                if (c > last || c < first) s1[4 * k + 2 * hh + e] = 0xff800000u;  // -inf
+                                if (c > last || (c < first && !(SINK && c < a.sink))) s1[4 * k + 2 * hh + e] = 0xff800000u;  // -inf
                             }
                     }
                 }
@@ -684,6 +724,10 @@ fwd_sm100_kernel(const TrainArgs a, const __grid_constant__ CUtensorMap tm_q, co
                 }
                 inv[hh] = r1f > 0.f ? 1.f / r1f : 0.f;                           // normaliser of the output
                 bart_o[hh] = r2f * inv[hh];                                      // bart used for the output
+                if (PART) {
+                    inv[hh] = r1f;                                               // the state goes out as it is
+                    bart_o[hh] = r2f;
+                }
                 const int row = r0 + rl0 + 8 * hh;
                 if (!EXT && t == 0 && row < it.nq) {
                     const int64_t si = it.b * a.st_sb + it.h * a.st_sh + static_cast<int64_t>(it.bos + row) * a.st_st;
@@ -697,6 +741,36 @@ fwd_sm100_kernel(const TrainArgs a, const __grid_constant__ CUtensorMap tm_q, co
             ok = __all_sync(0xffffffffu, mbar_wait(bar(L::kPVDone + (g - 1) % kPBufs), ((g - 1) / kPBufs) & 1, err, 11));
             if (!ok) break;
             tc_fence_after();
+            if constexpr (PART) {
+                float *rec[2];
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {
+                    const int rl = rl0 + 8 * hh, bi = it.b + rl / a.box_h, hr = it.h + rl % a.box_h;
+                    const bool in = rl < a.box_h * a.box_b && bi < a.batch && hr < a.n_rep;
+                    const int64_t row = static_cast<int64_t>(bi) * a.heads_q + it.hk * a.n_rep + hr;
+                    rec[hh] = in ? a.parts + (row * a.n_parts + it.extra) * (2 * D + 4) : nullptr;
+                    if (in && t == 0) __stcg(reinterpret_cast<float4 *>(rec[hh]), make_float4(m_ref[hh], inv[hh], bart_o[hh], 0.f));
+                }
+#pragma unroll 1
+                for (int c = 0; c < 2 * D; c += 64) {      // O1 then O2, 64 columns at a time
+                    uint32_t o[32];
+                    tmem_ld_16x256b_x8(tO1 + frag_base + c, o);
+                    tmem_wait_ld();
+                    if (c == 2 * D - 64) {
+                        tc_fence_before();
+                        mbar_arrive(bar(L::kOFree));
+                    }
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+#pragma unroll
+                        for (int hh = 0; hh < 2; ++hh)
+                            if (rec[hh])
+                                __stcg(reinterpret_cast<float2 *>(rec[hh] + 4 + c + 8 * k + 2 * t),
+                                       make_float2(__uint_as_float(o[4 * k + 2 * hh]), __uint_as_float(o[4 * k + 2 * hh + 1])));
+                }
+                ++n_items_done;
+                continue;
+            }
             const int64_t q_base = it.b * a.q_sb + it.h * a.q_sh + static_cast<int64_t>(it.bos + r0 + rl0) * a.q_st + 8 * t;
             T *go = static_cast<T *>(a.o) + q_base;
             T *gb = EXT ? nullptr : static_cast<T *>(a.barv) + q_base;
@@ -793,36 +867,50 @@ int *mirror_host_view() {
     return w.word ? h : nullptr;
 }
 
-template <typename T, int D, bool EXT>
+template <typename T, int D, int MODE>
 int launch_t(const TrainArgs &a, cudaStream_t stream) {
     constexpr int NS = 4;
+    constexpr bool EXT = kIsExtend<MODE>, PART = MODE == kPrefix;
     using L = Smem<D, NS>;
     const ErrorWords ew = error_words();
     if (!ew.word) return PLX_ERR_LAUNCH;
     const ErrSink sink{ew.word, ew.mirror};
     // keys: (batch, len_k) of a dense cache or of the training op, (page, key of the page) of a paged one
     const bool paged = EXT && a.page_table;
-    const int kv_rows = paged ? a.page_mask + 1 : a.len_k, kv_batch = paged ? a.n_pages : a.batch;
+    const int kv_rows = paged ? a.page_mask + 1 : a.len_k, kv_batch = paged ? a.n_pages : PART ? 1 : a.batch;
     const int kv_box = paged && a.page_mask + 1 < kBN ? a.page_mask + 1 : kBN;
     CUtensorMap tq, tr, tk, tv;
     const CUtensorMapDataType dt = Fmt<T>::kTma;
-    if (!make_map(&tq, dt, a.q, D, a.len_q, a.heads_q, a.batch, a.q_st, a.q_sh, a.q_sb, kBM) ||
-        !make_map(&tr, dt, a.r, D, a.len_q, a.heads_q, a.batch, a.q_st, a.q_sh, a.q_sb, kBM) ||
+    // prefix: the rows of a tile are q heads of a kv head (heads first) and batch rows
+    const int rows = PART ? a.n_rep : a.len_q, outer = PART ? a.heads_kv : a.heads_q, box_h = PART ? a.box_h : kBM, box_b = PART ? a.box_b : 1;
+    if (!make_map(&tq, dt, a.q, D, rows, outer, a.batch, a.q_st, a.q_sh, a.q_sb, box_h, box_b) ||
+        !make_map(&tr, dt, a.r, D, rows, outer, a.batch, a.q_st, a.q_sh, a.q_sb, box_h, box_b) ||
         !make_map(&tk, dt, a.k, D, kv_rows, a.heads_kv, kv_batch, a.kv_st, a.kv_sh, a.kv_sb, kv_box) ||
         !make_map(&tv, dt, a.v, D, kv_rows, a.heads_kv, kv_batch, a.kv_st, a.kv_sh, a.kv_sb, kv_box))
         return PLX_ERR_LAUNCH;
-    const int tiles = a.cu ? (a.len_q + kBM - 1) / kBM + a.n_seqs : (a.len_q + kBM - 1) / kBM;
-    const int n_items = tiles * a.batch * a.heads_q, sms = sm_count();
+    const int sms = sm_count();
     if (sms <= 0) return PLX_ERR_LAUNCH;
+    if constexpr (PART) {
+        static std::mutex mu;
+        static bool done[tma::kMaxDevices] = {};
+        auto kern = fwd_sm100_kernel<T, D, NS, MODE, false>;
+        if (!tma::opt_in_smem(kern, static_cast<int>(L::kBytes), done, mu)) return PLX_ERR_LAUNCH;
+        const int n_rt = ((a.n_rep + a.box_h - 1) / a.box_h) * ((a.batch + a.box_b - 1) / a.box_b), n = n_rt * a.heads_kv * a.n_splits;
+        kern<<<n < sms ? n : sms, 352, L::kBytes, stream>>>(a, tq, tr, tk, tv, sink, n_rt, n, 0, 0);
+        count_launch();
+        return cudaGetLastError() == cudaSuccess ? PLX_OK : PLX_ERR_LAUNCH;
+    } else {
+    const int tiles = a.cu ? (a.len_q + kBM - 1) / kBM + a.n_seqs : (a.len_q + kBM - 1) / kBM;
+    const int n_items = tiles * a.batch * a.heads_q;
     static std::mutex attr_mu;
     static bool attr_done[2][tma::kMaxDevices] = {};
     if (items_by_hardware(n_items, sms, a.cu || EXT)) {
-        auto kern = fwd_sm100_kernel<T, D, NS, EXT, true>;
+        auto kern = fwd_sm100_kernel<T, D, NS, MODE, true>;
         if (!tma::opt_in_smem(kern, static_cast<int>(L::kBytes), attr_done[1], attr_mu)) return PLX_ERR_LAUNCH;
         const int group = a.cu || EXT ? 1 : item_group(a.batch * a.heads_q, tiles, sms);
         kern<<<n_items, 352, L::kBytes, stream>>>(a, tq, tr, tk, tv, sink, tiles, n_items, 0, group);
     } else {
-        auto kern = fwd_sm100_kernel<T, D, NS, EXT, false>;
+        auto kern = fwd_sm100_kernel<T, D, NS, MODE, false>;
         if (!tma::opt_in_smem(kern, static_cast<int>(L::kBytes), attr_done[0], attr_mu)) return PLX_ERR_LAUNCH;
         // with plenty of items a CTA takes them in neighbouring pairs (a heavy and a light row tile)
         const int chunk_shift = n_items >= 2 * sms ? 1 : 0, units = (n_items + (1 << chunk_shift) - 1) >> chunk_shift;
@@ -830,22 +918,28 @@ int launch_t(const TrainArgs &a, cudaStream_t stream) {
     }
     count_launch();
     return cudaGetLastError() == cudaSuccess ? PLX_OK : PLX_ERR_LAUNCH;
+    }
 }
 
 }  // namespace
 
 bool train_fwd_sm100_supported(const TrainArgs &a, int head_dim) {
-    if ((head_dim != 64 && head_dim != 128) || a.window == 0 || !(a.c2 > 0.f)) return false;
+    if ((head_dim != 64 && head_dim != 128) || (a.window == 0 && a.sink == 0) || !(a.c2 > 0.f)) return false;
     // TMA needs 16-byte aligned strides; the ABI already guarantees multiples of 8 elements
     const char *env = std::getenv("PLX_FWD_KERNEL");
     if (env && env[0] == 'm') return false;  // "mma": force the warp-level kernels
     return tma::encode_fn() != nullptr;
 }
 
-int launch_train_fwd_sm100(const TrainArgs &a, int dtype, int head_dim, cudaStream_t stream) {
-    if (dtype == PLX_BF16) return head_dim == 64 ? launch_t<__nv_bfloat16, 64, false>(a, stream) : launch_t<__nv_bfloat16, 128, false>(a, stream);
-    if (dtype == PLX_FP16) return head_dim == 64 ? launch_t<__half, 64, false>(a, stream) : launch_t<__half, 128, false>(a, stream);
+template <int MODE>
+static int launch_mode(const TrainArgs &a, int dtype, int head_dim, cudaStream_t stream) {
+    if (dtype == PLX_BF16) return head_dim == 64 ? launch_t<__nv_bfloat16, 64, MODE>(a, stream) : launch_t<__nv_bfloat16, 128, MODE>(a, stream);
+    if (dtype == PLX_FP16) return head_dim == 64 ? launch_t<__half, 64, MODE>(a, stream) : launch_t<__half, 128, MODE>(a, stream);
     return PLX_ERR_UNSUPPORTED;
+}
+
+int launch_train_fwd_sm100(const TrainArgs &a, int dtype, int head_dim, cudaStream_t stream) {
+    return a.sink ? launch_mode<kTrainSink>(a, dtype, head_dim, stream) : launch_mode<kTrain>(a, dtype, head_dim, stream);
 }
 
 // Against a cache: any key range the forward takes; pages from 8 keys on (below that a box would not start on
@@ -856,9 +950,15 @@ bool train_extend_sm100_supported(const TrainArgs &a, int head_dim) {
 }
 
 int launch_train_extend_sm100(const TrainArgs &a, int dtype, int head_dim, cudaStream_t stream) {
-    if (dtype == PLX_BF16) return head_dim == 64 ? launch_t<__nv_bfloat16, 64, true>(a, stream) : launch_t<__nv_bfloat16, 128, true>(a, stream);
-    if (dtype == PLX_FP16) return head_dim == 64 ? launch_t<__half, 64, true>(a, stream) : launch_t<__half, 128, true>(a, stream);
-    return PLX_ERR_UNSUPPORTED;
+    return a.sink ? launch_mode<kExtendSink>(a, dtype, head_dim, stream) : launch_mode<kExtend>(a, dtype, head_dim, stream);
+}
+
+// A prefix: as against a cache.  `a` holds q, r, the keys (dense: one row of len_k; paged: a row of the page table), `parts` and
+// n_parts; n_splits is the caller's (see prefix_splits), box_h and box_b follow from the heads.
+int launch_prefix_sm100(const TrainArgs &problem, int dtype, int head_dim, cudaStream_t stream) {
+    TrainArgs a = problem;
+    prefix_boxes(a.n_rep, a.batch, a.box_h, a.box_b);
+    return launch_mode<kPrefix>(a, dtype, head_dim, stream);
 }
 
 ErrorWords sm100_error_words() { return error_words(); }

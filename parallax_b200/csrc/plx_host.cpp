@@ -45,15 +45,15 @@ enum Layout { kBHLD = 0, kBTHD = 1 };
 // entry points of the loaded libplx_sm100.so (the one ops.py calls; set once by bind())
 struct Api {
     decltype(&plx_device_error_peek) device_error_peek;
-    decltype(&plx_train_workspace_bytes) train_workspace_bytes;
-    decltype(&plx_train_fwd) train_fwd;
-    decltype(&plx_train_bwd) train_bwd;
-    decltype(&plx_train_extend) train_extend;
+    decltype(&plx_train_workspace_bytes_sink) train_workspace_bytes;
+    decltype(&plx_train_fwd_sink) train_fwd;
+    decltype(&plx_train_bwd_sink) train_bwd;
+    decltype(&plx_train_extend_sink) train_extend;
     decltype(&plx_decode_choose_splits_gqa) decode_choose_splits_gqa;
     decltype(&plx_decode_workspace_bytes) decode_workspace_bytes;
-    decltype(&plx_decode) decode;
+    decltype(&plx_decode_sink) decode;
     decltype(&plx_decode_stage) decode_stage;
-    decltype(&plx_decode_step) decode_step;
+    decltype(&plx_decode_step_sink) decode_step;
 };
 Api api;
 
@@ -63,15 +63,15 @@ void bind_one(F &slot, const py::dict &addresses, const char *name) {
 }
 void bind(const py::dict &addresses) {
     bind_one(api.device_error_peek, addresses, "plx_device_error_peek");
-    bind_one(api.train_workspace_bytes, addresses, "plx_train_workspace_bytes");
-    bind_one(api.train_fwd, addresses, "plx_train_fwd");
-    bind_one(api.train_bwd, addresses, "plx_train_bwd");
-    bind_one(api.train_extend, addresses, "plx_train_extend");
+    bind_one(api.train_workspace_bytes, addresses, "plx_train_workspace_bytes_sink");
+    bind_one(api.train_fwd, addresses, "plx_train_fwd_sink");
+    bind_one(api.train_bwd, addresses, "plx_train_bwd_sink");
+    bind_one(api.train_extend, addresses, "plx_train_extend_sink");
     bind_one(api.decode_choose_splits_gqa, addresses, "plx_decode_choose_splits_gqa");
     bind_one(api.decode_workspace_bytes, addresses, "plx_decode_workspace_bytes");
-    bind_one(api.decode, addresses, "plx_decode");
+    bind_one(api.decode, addresses, "plx_decode_sink");
     bind_one(api.decode_stage, addresses, "plx_decode_stage");
-    bind_one(api.decode_step, addresses, "plx_decode_step");
+    bind_one(api.decode_step, addresses, "plx_decode_step_sink");
 }
 
 // ------------------------------------------------------------------------- //
@@ -107,6 +107,14 @@ bool take_window(const py::object &o, int64_t &window) {
     int overflow = 0;
     window = PyLong_AsLongLongAndOverflow(o.ptr(), &overflow);
     return overflow == 0 && window >= -1 && window <= INT32_MAX;
+}
+
+// sink_tokens as a plain Python number
+bool take_sinks(const py::object &o, int32_t &sinks) {
+    int64_t n;
+    if (!take_window(o, n) || n < 0) return false;
+    sinks = static_cast<int32_t>(n);
+    return true;
 }
 
 // No dispatch key beyond those of an ordinary dense CUDA tensor and its autograd, and no forward-mode tangent.
@@ -185,14 +193,14 @@ struct Refused {};   // a status of the library that the Python path has to repo
 // One node for forward and backward, as the custom op plx::train_fwd registers it.
 struct Train : torch::autograd::Function<Train> {
     static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &q, const Tensor &r, const Tensor &k, const Tensor &v,
-                          double scale, int64_t window, int64_t layout, const OptTensor &cu) {
+                          double scale, int64_t window, int64_t layout, const OptTensor &cu, int64_t sinks) {
         at::AutoDispatchBelowADInplaceOrView below;
         const c10::cuda::CUDAGuard device(q.device());
         Tensor o = at::empty_like(q), barv = at::empty_like(q);
         const auto stat = [&] { return at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat)); };
         Tensor d1 = stat(), bart = stat(), m = stat();
         const plx_train_problem p = train_problem(q, k, d1, scale, window, layout, cu);
-        if (api.train_fwd(&p, q.data_ptr(), r.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), barv.data_ptr(),
+        if (api.train_fwd(&p, static_cast<int32_t>(sinks), q.data_ptr(), r.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), barv.data_ptr(),
                           d1.data_ptr<float>(), bart.data_ptr<float>(), m.data_ptr<float>(), c10::cuda::getCurrentCUDAStream().stream()) != PLX_OK)
             throw Refused();
         ctx->save_for_backward({q, r, k, v, o, barv, d1, bart, m, cu ? *cu : Tensor()});
@@ -200,6 +208,7 @@ struct Train : torch::autograd::Function<Train> {
         ctx->saved_data["scale"] = scale;
         ctx->saved_data["window"] = window;
         ctx->saved_data["layout"] = layout;
+        ctx->saved_data["sinks"] = sinks;
         return {o, barv, d1, bart, m};
     }
 
@@ -209,7 +218,8 @@ struct Train : torch::autograd::Function<Train> {
                      &bart = saved[7], &m = saved[8];
         const OptTensor cu = saved[9].defined() ? OptTensor(saved[9]) : std::nullopt;
         const double scale = ctx->saved_data["scale"].toDouble();
-        const int64_t window = ctx->saved_data["window"].toInt(), layout = ctx->saved_data["layout"].toInt();
+        const int64_t window = ctx->saved_data["window"].toInt(), layout = ctx->saved_data["layout"].toInt(),
+                      sinks = ctx->saved_data["sinks"].toInt();
         Tensor go = grads[0].defined() ? grads[0] : at::zeros_like(o);
         if (go.strides() != q.strides()) go = at::empty_like(q).copy_(go);   // one stride set for all q-like tensors
         Tensor dq, dr, dk, dv;
@@ -229,13 +239,13 @@ struct Train : torch::autograd::Function<Train> {
             const c10::cuda::CUDAGuard device(q.device());
             const plx_train_problem p = train_problem(q, k, d1, scale, window, layout, cu);
             size_t need = 0;
-            if (!device_error_waiting() && api.train_workspace_bytes(&p, &need) == PLX_OK) {
+            if (!device_error_waiting() && api.train_workspace_bytes(&p, static_cast<int32_t>(sinks), &need) == PLX_OK) {
                 dq = at::empty_like(q);
                 dr = at::empty_like(q);
                 dk = at::empty_like(k);
                 dv = at::empty_like(k);
                 const Tensor ws = at::empty({static_cast<int64_t>(need)}, q.options().dtype(at::kByte));
-                done = api.train_bwd(&p, q.data_ptr(), r.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), barv.data_ptr(),
+                done = api.train_bwd(&p, static_cast<int32_t>(sinks), q.data_ptr(), r.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), barv.data_ptr(),
                                      d1.data_ptr<float>(), bart.data_ptr<float>(), m.data_ptr<float>(), go.data_ptr(), dq.data_ptr(), dr.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), need,
                                      c10::cuda::getCurrentCUDAStream().stream()) == PLX_OK;
             }
@@ -244,10 +254,10 @@ struct Train : torch::autograd::Function<Train> {
             static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("plx::train_bwd", "")
                 .typed<std::tuple<Tensor, Tensor, Tensor, Tensor>(const Tensor &, const Tensor &, const Tensor &, const Tensor &,
                     const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &, double, int64_t, int64_t,
-                    const OptTensor &)>();
-            std::tie(dq, dr, dk, dv) = op.call(q, r, k, v, o, barv, d1, bart, m, go, scale, window, layout, cu);
+                    const OptTensor &, int64_t)>();
+            std::tie(dq, dr, dk, dv) = op.call(q, r, k, v, o, barv, d1, bart, m, go, scale, window, layout, cu, sinks);
         }
-        return {dq, dr, dk, dv, Tensor(), Tensor(), Tensor(), Tensor()};
+        return {dq, dr, dk, dv, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
 
@@ -270,7 +280,7 @@ bool train_ready(const py::object &q_, const py::object &r_, const py::object &k
 
 // o, barv, d1, bart, m
 py::object train(const py::object &q_, const py::object &r_, const py::object &k_, const py::object &v_, const py::object &scale_,
-                 const py::object &window_, int64_t layout, const py::object &cu_) {
+                 const py::object &window_, int64_t layout, const py::object &cu_, const py::object &sinks_) {
     bool ok = true;
     const Tensor q = take(q_, ok), r = take(r_, ok), k = take(k_, ok), v = take(v_, ok);
     const OptTensor cu = take_optional(cu_, ok);
@@ -280,14 +290,15 @@ py::object train(const py::object &q_, const py::object &r_, const py::object &k
         return py::none();
     double scale;
     int64_t window;
-    if (!take_scale(scale_, q.size(3), scale) || !take_window(window_, window)) return py::none();
+    int32_t sinks;
+    if (!take_scale(scale_, q.size(3), scale) || !take_window(window_, window) || !take_sinks(sinks_, sinks)) return py::none();
     const c10::cuda::CUDAGuard device(q.device());
     if (device_error_waiting()) return py::none();
     torch::autograd::variable_list res;
     RECORD_FUNCTION("plx::train_fwd", Values({q, r, k, v}));
     try {
         py::gil_scoped_release nogil;
-        res = Train::apply(q, r, k, v, scale, window, static_cast<int64_t>(layout), cu);
+        res = Train::apply(q, r, k, v, scale, window, static_cast<int64_t>(layout), cu, static_cast<int64_t>(sinks));
     } catch (const Refused &) {
         return py::none();
     }
@@ -510,7 +521,7 @@ plx_decode_problem decode_problem(const Tensor &q, const Tensor &k, int64_t ceil
 }
 
 py::object decode(const py::object &q_, const py::object &r_, const py::object &k_, const py::object &v_, const py::object &scale_,
-                  const py::object &window_, const py::object &lens_, const py::object &start_, const py::object &table_) {
+                  const py::object &window_, const py::object &lens_, const py::object &start_, const py::object &table_, const py::object &sinks_) {
     bool ok = true;
     const Tensor q = take(q_, ok), r = take(r_, ok), k = take(k_, ok), v = take(v_, ok);
     const OptTensor lens = take_optional(lens_, ok), start = take_optional(start_, ok), table = take_optional(table_, ok);
@@ -519,22 +530,23 @@ py::object decode(const py::object &q_, const py::object &r_, const py::object &
         return py::none();
     double scale;
     int64_t window;
+    int32_t sinks;
     const int64_t ceiling = table ? table->size(1) * k.size(1) : k.size(1);
-    if (!take_scale(scale_, q.size(3), scale) || !take_window(window_, window) || ceiling > INT32_MAX) return py::none();
+    if (!take_scale(scale_, q.size(3), scale) || !take_window(window_, window) || !take_sinks(sinks_, sinks) || ceiling > INT32_MAX) return py::none();
     at::AutoDispatchBelowADInplaceOrView below;
     const c10::cuda::CUDAGuard device(q.device());
     if (capturing()) return py::none();
     RECORD_FUNCTION("plx::decode_out", Values({q, r, k, v}));
     const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream();
     plx_decode_problem p = decode_problem(q, k, ceiling, table, scale, window, 1);
-    const int32_t n_keys = window < 0 ? p.cache_len : std::max(1, std::min(p.cache_len, p.window_left));
+    const int32_t n_keys = window < 0 ? p.cache_len : static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(p.cache_len, window + sinks)));
     p.n_splits = api.decode_choose_splits_gqa(p.batch, p.heads_q, p.heads_kv, n_keys, at::cuda::getDeviceProperties(q.get_device())->multiProcessorCount);
     size_t need = 0;
     if (api.decode_workspace_bytes(&p, &need) != PLX_OK) return py::none();
     const Tensor ws = workspaces().get(stream, q, p.n_splits, static_cast<int64_t>(need / sizeof(float)));
     Tensor out = at::empty(q.sizes(), q.options());
     LengthCheck check(lens, stream, decode_lasts(q, k, n_keys));
-    if (api.decode(&p, q.data_ptr(), r.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), int_ptr(lens), int_ptr(start), ws.data_ptr(), need,
+    if (api.decode(&p, sinks, q.data_ptr(), r.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), int_ptr(lens), int_ptr(start), ws.data_ptr(), need,
                    stream.stream()) != PLX_OK ||
         !check.within(1, ceiling))
         return py::none();
@@ -543,15 +555,16 @@ py::object decode(const py::object &q_, const py::object &r_, const py::object &
 
 // L_q > 1: one launch of the training forward kernel against the cache.
 py::object extend(const py::object &q_, const py::object &r_, const py::object &k_, const py::object &v_, const py::object &scale_,
-                  const py::object &window_, const py::object &lens_, const py::object &table_) {
+                  const py::object &window_, const py::object &lens_, const py::object &table_, const py::object &sinks_) {
     bool ok = true;
     const Tensor q = take(q_, ok), r = take(r_, ok), k = take(k_, ok), v = take(v_, ok);
     const OptTensor lens = take_optional(lens_, ok), table = take_optional(table_, ok);
     if (!ok || !plain_thread() || !cache_call_ok(q, r, k, v, lens, table)) return py::none();
     double scale;
     int64_t window;
+    int32_t sinks;
     const int64_t ceiling = table ? table->size(1) * k.size(1) : k.size(1);
-    if (!take_scale(scale_, q.size(3), scale) || !take_window(window_, window) || ceiling > INT32_MAX || q.size(1) > ceiling) return py::none();
+    if (!take_scale(scale_, q.size(3), scale) || !take_window(window_, window) || !take_sinks(sinks_, sinks) || ceiling > INT32_MAX || q.size(1) > ceiling) return py::none();
     at::AutoDispatchBelowADInplaceOrView below;
     const c10::cuda::CUDAGuard device(q.device());
     if (capturing() || device_error_waiting()) return py::none();
@@ -561,7 +574,7 @@ py::object extend(const py::object &q_, const py::object &r_, const py::object &
     p.len_k = static_cast<int32_t>(ceiling);
     Tensor out = at::empty(q.sizes(), q.options());
     LengthCheck check(lens, stream, prefill_lasts(q, ceiling));
-    if (api.train_extend(&p, q.data_ptr(), r.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), int_ptr(lens), int_ptr(table),
+    if (api.train_extend(&p, sinks, q.data_ptr(), r.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), int_ptr(lens), int_ptr(table),
                          table ? static_cast<int32_t>(k.size(1)) : 0, table ? static_cast<int32_t>(table->size(1)) : 0,
                          table ? static_cast<int32_t>(k.size(0)) : 0, stream.stream()) != PLX_OK ||
         !check.within(q.size(1), ceiling))
@@ -570,10 +583,11 @@ py::object extend(const py::object &q_, const py::object &r_, const py::object &
 }
 
 py::object attend(const py::object &q, const py::object &r, const py::object &k, const py::object &v, const py::object &scale,
-                  const py::object &window, const py::object &lens, const py::object &table) {
+                  const py::object &window, const py::object &lens, const py::object &table, const py::object &sinks) {
     if (!plain_object(q.ptr())) return py::none();
     const Tensor &t = THPVariable_Unpack(q.ptr());
-    return t.dim() == 4 && t.size(1) == 1 ? decode(q, r, k, v, scale, window, lens, py::none(), table) : extend(q, r, k, v, scale, window, lens, table);
+    return t.dim() == 4 && t.size(1) == 1 ? decode(q, r, k, v, scale, window, lens, py::none(), table, sinks)
+                                            : extend(q, r, k, v, scale, window, lens, table, sinks);
 }
 
 // No address of the sources (tensors or None) lies in one of the buffers; false where that cannot be told.
@@ -610,7 +624,7 @@ bool apart(const py::tuple &sources, const py::tuple &buffers) {
 enum Step { kNothing = 0, kStaged = 1, kDone = 2 };
 int step(const py::object &q_, const py::object &q_src_, const py::object &r_, const py::object &r_src_, const py::object &lens_,
          const py::object &lens_src, int64_t most, const py::object &k_, const py::object &v_, const py::object &out_, const py::object &ws_,
-         double scale, int64_t window, int64_t n_splits) {
+         double scale, int64_t window, int64_t n_splits, int64_t sinks) {
     bool ok = true;
     const Tensor q = take(q_, ok), r = take(r_, ok);
     const OptTensor q_src = take_optional(q_src_, ok), r_src = take_optional(r_src_, ok), lens = take_optional(lens_, ok);
@@ -645,7 +659,7 @@ int step(const py::object &q_, const py::object &q_src_, const py::object &r_, c
     if (ok && q.dim() == 4 && q.size(0) <= PLX_DECODE_STEP_ROWS && cache_call_ok(q, r, k, v, lens, std::nullopt) && plain_tensor(out) && plain_tensor(ws) &&
         out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.device() == q.device() && out.is_contiguous()) {
         const plx_decode_problem p = decode_problem(q, k, k.size(1), std::nullopt, scale, window, static_cast<int32_t>(n_splits));
-        if (api.decode_step(&p, q.data_ptr(), q_from, r.data_ptr(), r_from, k.data_ptr(), v.data_ptr(), out.data_ptr(), lens_to, n ? values : nullptr,
+        if (api.decode_step(&p, static_cast<int32_t>(sinks), q.data_ptr(), q_from, r.data_ptr(), r_from, k.data_ptr(), v.data_ptr(), out.data_ptr(), lens_to, n ? values : nullptr,
                             ws.data_ptr(), ws.nbytes(), stream) == PLX_OK)
             return kDone;
     }
@@ -659,10 +673,10 @@ PYBIND11_MODULE(_plx_host, m) {
     m.attr("abi_version") = PLX_ABI_VERSION;
     m.def("bind", &bind);
     m.def("train_ready", &train_ready);
-    m.def("train", &train);
-    m.def("decode", &decode);
-    m.def("attend", &attend);
+    m.def("train", &train, py::arg("q"), py::arg("r"), py::arg("k"), py::arg("v"), py::arg("scale"), py::arg("window"), py::arg("layout"), py::arg("cu_seqlens"), py::arg("sink_tokens") = 0);
+    m.def("decode", &decode, py::arg("q"), py::arg("r"), py::arg("k"), py::arg("v"), py::arg("scale"), py::arg("window"), py::arg("seqused_k"), py::arg("cache_start"), py::arg("page_table"), py::arg("sink_tokens") = 0);
+    m.def("attend", &attend, py::arg("q"), py::arg("r"), py::arg("k"), py::arg("v"), py::arg("scale"), py::arg("window"), py::arg("seqused_k"), py::arg("page_table"), py::arg("sink_tokens") = 0);
     m.def("apart", &apart);
-    m.def("step", &step);
+    m.def("step", &step, py::arg("q"), py::arg("q_src"), py::arg("r"), py::arg("r_src"), py::arg("lens"), py::arg("lens_src"), py::arg("most"), py::arg("k"), py::arg("v"), py::arg("out"), py::arg("workspace"), py::arg("scale"), py::arg("window"), py::arg("n_splits"), py::arg("sink_tokens") = 0);
     m.def("side_streams_made", [] { return side_streams().made(); });
 }

@@ -50,6 +50,18 @@ int launch_train_fwd_sm100(const TrainArgs &a, int dtype, int head_dim, cudaStre
 // the same kernel for several query rows per sequence against a dense or paged KV cache (writes `o` only)
 bool train_extend_sm100_supported(const TrainArgs &a, int head_dim);
 int launch_train_extend_sm100(const TrainArgs &a, int dtype, int head_dim, cudaStream_t stream);
+// Rows of a tile of the prefix kernel: box_h q heads of a kv head by box_b batch rows, 128 at most.
+inline void prefix_boxes(int n_rep, int batch, int &box_h, int &box_b) {
+    box_h = n_rep < 128 ? n_rep : 128;
+    box_b = 128 / box_h < batch ? 128 / box_h : batch;
+}
+inline int prefix_row_tiles(int n_rep, int batch) {
+    int h, b;
+    prefix_boxes(n_rep, batch, h, b);
+    return ((n_rep + h - 1) / h) * ((batch + b - 1) / b);
+}
+// the same kernel for the rows of a batch (one token each) against a prefix that they share: partial states only
+int launch_prefix_sm100(const TrainArgs &a, int dtype, int head_dim, cudaStream_t stream);
 // Error words of the current device (see sm100::ErrSink): `word` in device memory, `mirror` in mapped
 // pinned host memory.  Both null on failure.  The first call on a device allocates the mirror.
 struct ErrorWords {
@@ -63,6 +75,9 @@ bool train_bwd_sm100_supported(const TrainArgs &a, int head_dim);
 // `overlap`: the kernel launched just before on this stream is the row statistics (dk/dv) or dk/dv (dq/dr) of the
 // same call, and this one may start under its end
 int launch_train_bwd_sm100(const TrainArgs &a, int dtype, int head_dim, int stage, bool overlap, cudaStream_t stream);
+// sinks: rows of a chunk of dk/dv, and the launch that adds the chunks up (behind dk/dv, where a.sink_slots > 0)
+int train_sink_chunk(int window, int len_q);
+int launch_train_bwd_join(const TrainArgs &a, int dtype, int head_dim, cudaStream_t stream);
 
 constexpr int kDecodeGqaWarps = 8;   // warps (independent splits) per CTA of the grouped-query decode kernel
 int launch_decode(const DecodeArgs &a, int dtype, int head_dim, cudaStream_t stream);
@@ -73,6 +88,8 @@ int launch_decode_stage(void *q, const void *q_src, void *r, const void *r_src, 
                         cudaStream_t stream);
 int launch_decode_merge(const float *parts, int n_parts, int n_records, int head_dim, int dtype, void *out,
                         cudaStream_t stream);
+
+int launch_prefix_merge(const float *parts, int n_parts, int64_t n_rows, int head_dim, int dtype, void *out, cudaStream_t stream);
 
 // pages of a cache (see plx_pages.cu)
 int launch_pages_copy(const plx_page_pool *p, const int32_t *src, const int32_t *dst, int n, cudaStream_t stream);

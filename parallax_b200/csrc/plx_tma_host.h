@@ -32,18 +32,18 @@ inline EncodeFn encode_fn() {
 }
 
 // What a map of these kernels depends on: a (head_dim, tokens, heads, batch) view of a 16-bit tensor
-// with a box of 64 channels x `rows` tokens, 128-byte swizzle.
+// with a box of 64 channels x `rows` tokens (x box_b batch rows), 128-byte swizzle.
 struct MapKey {
     const void *ptr;
     int64_t st, sh, sb;
-    int32_t head_dim, tokens, heads, batch, rows, dtype;
+    int32_t head_dim, tokens, heads, batch, rows, box_b, dtype;
 };
 
 // Encoding a map is pure host arithmetic on the key, so maps are kept in a small direct-mapped
 // cache: a training loop that calls with the same buffers (or a CUDA-graph capture loop) encodes
 // each map once.  A changed pointer, shape or stride is simply a different key.
 inline bool make_map(CUtensorMap *map, CUtensorMapDataType dt, const void *ptr, int head_dim, int tokens, int heads, int batch,
-                     int64_t st, int64_t sh, int64_t sb, int rows) {
+                     int64_t st, int64_t sh, int64_t sb, int rows, int box_b = 1) {
     constexpr int kSlots = 64;
     struct Slot {
         MapKey key;
@@ -55,7 +55,7 @@ inline bool make_map(CUtensorMap *map, CUtensorMapDataType dt, const void *ptr, 
     MapKey key;
     memset(&key, 0, sizeof(key));
     key.ptr = ptr; key.st = st; key.sh = sh; key.sb = sb;
-    key.head_dim = head_dim; key.tokens = tokens; key.heads = heads; key.batch = batch; key.rows = rows;
+    key.head_dim = head_dim; key.tokens = tokens; key.heads = heads; key.batch = batch; key.rows = rows; key.box_b = box_b;
     key.dtype = static_cast<int32_t>(dt);
     uint64_t h = reinterpret_cast<uintptr_t>(ptr) >> 4;
     h = (h ^ (h >> 17)) * 0x9E3779B97F4A7C15ull + static_cast<uint64_t>(rows) * 31u + static_cast<uint64_t>(tokens);
@@ -73,7 +73,7 @@ inline bool make_map(CUtensorMap *map, CUtensorMapDataType dt, const void *ptr, 
                                 static_cast<cuuint64_t>(batch)};
     const cuuint64_t strides[3] = {static_cast<cuuint64_t>(st) * 2, static_cast<cuuint64_t>(sh) * 2,
                                    static_cast<cuuint64_t>(sb) * 2};
-    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(rows), 1, 1};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(rows), 1, static_cast<cuuint32_t>(box_b)};
     const cuuint32_t elem[4] = {1, 1, 1, 1};
     if (fn(map, dt, 4, const_cast<void *>(ptr), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)

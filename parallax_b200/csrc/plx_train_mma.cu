@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(NW * 32) fwd_mma_kernel(const TrainArgs a) {
     const int bos = s_loc[0], nq = s_loc[1], nk = s_loc[2], r0 = s_loc[3] * BM;
     if (r0 >= nq) return;
     const int b = blockIdx.y / a.heads_q, h = blockIdx.y % a.heads_q, hk = h / a.n_rep;
-    const Mask mask{nk - nq, a.window};
+    const Mask mask{nk - nq, a.window, a.sink};
 
     const int64_t q_base = b * a.q_sb + h * a.q_sh + static_cast<int64_t>(bos) * a.q_st;
     const int64_t kv_base = b * a.kv_sb + hk * a.kv_sh + static_cast<int64_t>(bos) * a.kv_st;
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(NW * 32) fwd_mma_kernel(const TrainArgs a) {
 
     // visible key range of this row tile
     int hi_col = min(nk, r0 + BM + mask.off);
-    int lo_col = a.window >= 0 ? max(0, r0 + mask.off - a.window + 1) : 0;
+    int lo_col = a.window >= 0 && a.sink == 0 ? max(0, r0 + mask.off - a.window + 1) : 0;
     const int jlo = lo_col / BN;
     const int jhi = hi_col > lo_col ? (hi_col + BN - 1) / BN : jlo;
 
@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(NW * 32) bwd_dqr_mma_kernel(const TrainArgs a,
     const int bos = s_loc[0], nq = s_loc[1], nk = s_loc[2], r0 = s_loc[3] * BM;
     if (r0 >= nq) return;
     const int b = blockIdx.y / a.heads_q, h = blockIdx.y % a.heads_q, hk = h / a.n_rep;
-    const Mask mask{nk - nq, a.window};
+    const Mask mask{nk - nq, a.window, a.sink};
 
     const int64_t q_base = b * a.q_sb + h * a.q_sh + static_cast<int64_t>(bos) * a.q_st;
     const int64_t kv_base = b * a.kv_sb + hk * a.kv_sh + static_cast<int64_t>(bos) * a.kv_st;
@@ -499,7 +499,7 @@ __global__ void __launch_bounds__(NW * 32) bwd_dqr_mma_kernel(const TrainArgs a,
     const T *gv = static_cast<const T *>(a.v) + kv_base;
 
     int hi_col = min(nk, r0 + BM + mask.off);
-    int lo_col = a.window >= 0 ? max(0, r0 + mask.off - a.window + 1) : 0;
+    int lo_col = a.window >= 0 && a.sink == 0 ? max(0, r0 + mask.off - a.window + 1) : 0;
     const int jlo = lo_col / BN;
     const int jhi = hi_col > lo_col ? (hi_col + BN - 1) / BN : jlo;
 
@@ -638,12 +638,12 @@ __global__ void __launch_bounds__(NW * 32) bwd_dkv_mma_kernel(const TrainArgs a,
     const int bos = s_loc[0], nq = s_loc[1], nk = s_loc[2], c0 = s_loc[3] * BN;
     if (c0 >= nk) return;
     const int b = blockIdx.y / a.heads_kv, hk = blockIdx.y % a.heads_kv;
-    const Mask mask{nk - nq, a.window};
+    const Mask mask{nk - nq, a.window, a.sink};
     const int64_t kv_base = b * a.kv_sb + hk * a.kv_sh + static_cast<int64_t>(bos) * a.kv_st;
 
     // query rows that can see any key of this tile
     const int i_lo = max(0, c0 - mask.off);
-    const int i_hi = a.window >= 0 ? min(nq, min(nk, c0 + BN) - mask.off + a.window - 1) : nq;
+    const int i_hi = a.window >= 0 && c0 >= a.sink ? min(nq, min(nk, c0 + BN) - mask.off + a.window - 1) : nq;
     const int tlo = i_lo / BR;
     const int thi = i_hi > i_lo ? (i_hi + BR - 1) / BR : tlo;
     const int ntile = thi - tlo;

@@ -79,6 +79,14 @@ def _train_problem(q: Tensor, k: Tensor, stats: Tensor, qk_scale: float, window_
     return p
 
 
+def _entry(name: str, sink_tokens: int):
+    """Entry point `name`, or its form with sinks: what follows the problem is the same."""
+    if not sink_tokens:
+        return getattr(_cabi.lib(), name)
+    fn = getattr(_cabi.lib(), name + "_sink")
+    return lambda p, *rest: fn(p, int(sink_tokens), *rest)
+
+
 def _stats_shape(q: Tensor, layout: int):
     return q.shape[:3]
 
@@ -95,7 +103,7 @@ def _with_strides_of(like: Tensor, *tensors: Tensor):
 # --------------------------------------------------------------------------- #
 @torch.library.custom_op("plx::train_fwd", mutates_args=(), device_types="cuda")
 def train_fwd_op(q: Tensor, r: Tensor, k: Tensor, v: Tensor, qk_scale: float, window_left: int, layout: int,
-                 cu_seqlens: Optional[Tensor]) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+                 cu_seqlens: Optional[Tensor], sink_tokens: int = 0) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
     o = torch.empty_like(q)
     barv = torch.empty_like(q)
     q, r = _with_strides_of(o, q, r)
@@ -105,21 +113,21 @@ def train_fwd_op(q: Tensor, r: Tensor, k: Tensor, v: Tensor, qk_scale: float, wi
     p = _train_problem(q, k, d1, qk_scale, window_left, layout, cu_seqlens)
     with torch.cuda.device(q.device):
         _cabi.raise_if_device_error("plx_train_fwd")
-        st = _cabi.lib().plx_train_fwd(C.byref(p), _ptr(q), _ptr(r), _ptr(k), _ptr(v), _ptr(o), _ptr(barv),
-                                       _ptr(d1), _ptr(bart), _ptr(m), _stream(q.device))
+        st = _entry("plx_train_fwd", sink_tokens)(C.byref(p), _ptr(q), _ptr(r), _ptr(k), _ptr(v), _ptr(o), _ptr(barv),
+                                                  _ptr(d1), _ptr(bart), _ptr(m), _stream(q.device))
     _cabi.check(st, "plx_train_fwd")
     return o, barv, d1, bart, m
 
 
 @train_fwd_op.register_fake
-def _(q, r, k, v, qk_scale, window_left, layout, cu_seqlens):
+def _(q, r, k, v, qk_scale, window_left, layout, cu_seqlens, sink_tokens=0):
     stats = q.new_empty(q.shape[:3], dtype=torch.float32)
     return torch.empty_like(q), torch.empty_like(q), stats, torch.empty_like(stats), torch.empty_like(stats)
 
 
 @torch.library.custom_op("plx::train_extend", mutates_args=("out",), device_types="cuda")
 def train_extend(q: Tensor, r: Tensor, k: Tensor, v: Tensor, out: Tensor, qk_scale: float, window_left: int,
-                 seqused_k: Optional[Tensor], page_table: Optional[Tensor]) -> None:
+                 seqused_k: Optional[Tensor], page_table: Optional[Tensor], sink_tokens: int = 0) -> None:
     """Several query rows per sequence against a cache, all rows in one launch (BTHD; `out` strided like q).
     Raises PlxError with status PLX_ERR_UNSUPPORTED, having enqueued nothing, where no kernel takes the problem."""
     p = _train_problem(q, k, q, qk_scale, window_left, BTHD, None)
@@ -129,24 +137,25 @@ def train_extend(q: Tensor, r: Tensor, k: Tensor, v: Tensor, out: Tensor, qk_sca
         p.len_k = pages_per_seq * page_size
     with torch.cuda.device(q.device):
         _cabi.raise_if_device_error("plx_train_extend")
-        st = _cabi.lib().plx_train_extend(C.byref(p), _ptr(q), _ptr(r), _ptr(k), _ptr(v), _ptr(out), _ptr(seqused_k),
-                                          _ptr(page_table), page_size, pages_per_seq, n_pages, _stream(q.device))
+        st = _entry("plx_train_extend", sink_tokens)(C.byref(p), _ptr(q), _ptr(r), _ptr(k), _ptr(v), _ptr(out), _ptr(seqused_k),
+                                                     _ptr(page_table), page_size, pages_per_seq, n_pages, _stream(q.device))
     _cabi.check(st, "plx_train_extend")
 
 
 @train_extend.register_fake
-def _(q, r, k, v, out, qk_scale, window_left, seqused_k, page_table):
+def _(q, r, k, v, out, qk_scale, window_left, seqused_k, page_table, sink_tokens=0):
     return None
 
 
 BWD_STATS, BWD_DQR, BWD_DKV, BWD_ALL = 1, 2, 4, 7
 
 
-def train_bwd_workspace(q: Tensor, k: Tensor, d1: Tensor, layout: int, cu_seqlens: Optional[Tensor]) -> Tensor:
-    """Scratch for the backward row statistics (sized by plx_train_workspace_bytes)."""
-    p = _train_problem(q, k, d1, 1.0, -1, layout, cu_seqlens)
+def train_bwd_workspace(q: Tensor, k: Tensor, d1: Tensor, layout: int, cu_seqlens: Optional[Tensor], window_left: int = -1,
+                        sink_tokens: int = 0) -> Tensor:
+    """Scratch for the backward: row statistics, with sinks the parts of their keys' gradients (plx_train_workspace_bytes_sink)."""
+    p = _train_problem(q, k, d1, 1.0, window_left, layout, cu_seqlens)
     need = C.c_size_t(0)
-    _cabi.check(_cabi.lib().plx_train_workspace_bytes(C.byref(p), C.byref(need)), "plx_train_workspace_bytes")
+    _cabi.check(_entry("plx_train_workspace_bytes", sink_tokens)(C.byref(p), C.byref(need)), "plx_train_workspace_bytes")
     return torch.empty(max(need.value, 16), device=q.device, dtype=torch.uint8)
 
 
@@ -166,28 +175,37 @@ def train_bwd_stages(stages: int, q, r, k, v, o, barv, d1, bart, m, grad_o, dq, 
 @torch.library.custom_op("plx::train_bwd", mutates_args=(), device_types="cuda")
 def train_bwd(q: Tensor, r: Tensor, k: Tensor, v: Tensor, o: Tensor, barv: Tensor, d1: Tensor, bart: Tensor,
               m: Tensor, grad_o: Tensor, qk_scale: float, window_left: int, layout: int,
-              cu_seqlens: Optional[Tensor]) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+              cu_seqlens: Optional[Tensor], sink_tokens: int = 0) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
     dq, dr = torch.empty_like(q), torch.empty_like(q)
     dk, dv = torch.empty_like(k), torch.empty_like(k)
     q, r, o, barv, grad_o = _with_strides_of(dq, q, r, o, barv, grad_o)
     k, v = _with_strides_of(dk, k, v)
     d1, bart, m = d1.contiguous(), bart.contiguous(), m.contiguous()
-    ws = train_bwd_workspace(q, k, d1, layout, cu_seqlens)
-    train_bwd_stages(BWD_ALL, q, r, k, v, o, barv, d1, bart, m, grad_o, dq, dr, dk, dv, ws, qk_scale, window_left,
-                     layout, cu_seqlens)
+    ws = train_bwd_workspace(q, k, d1, layout, cu_seqlens, window_left, sink_tokens)
+    if not sink_tokens:
+        train_bwd_stages(BWD_ALL, q, r, k, v, o, barv, d1, bart, m, grad_o, dq, dr, dk, dv, ws, qk_scale, window_left,
+                         layout, cu_seqlens)
+        return dq, dr, dk, dv
+    p = _train_problem(q, k, d1, qk_scale, window_left, layout, cu_seqlens)
+    with torch.cuda.device(q.device):
+        _cabi.raise_if_device_error("plx_train_bwd_sink")
+        st = _cabi.lib().plx_train_bwd_sink(C.byref(p), int(sink_tokens), _ptr(q), _ptr(r), _ptr(k), _ptr(v), _ptr(o), _ptr(barv), _ptr(d1),
+                                            _ptr(bart), _ptr(m), _ptr(grad_o), _ptr(dq), _ptr(dr), _ptr(dk), _ptr(dv), _ptr(ws),
+                                            C.c_size_t(ws.numel()), _stream(q.device))
+    _cabi.check(st, "plx_train_bwd_sink")
     return dq, dr, dk, dv
 
 
 @train_bwd.register_fake
-def _(q, r, k, v, o, barv, d1, bart, m, grad_o, qk_scale, window_left, layout, cu_seqlens):
+def _(q, r, k, v, o, barv, d1, bart, m, grad_o, qk_scale, window_left, layout, cu_seqlens, sink_tokens=0):
     return torch.empty_like(q), torch.empty_like(q), torch.empty_like(k), torch.empty_like(k)
 
 
 def _setup_ctx(ctx, inputs, output):
-    q, r, k, v, qk_scale, window_left, layout, cu_seqlens = inputs
+    q, r, k, v, qk_scale, window_left, layout, cu_seqlens, sink_tokens = inputs
     o, barv, d1, bart, m = output
     ctx.save_for_backward(q, r, k, v, o, barv, d1, bart, m, cu_seqlens)
-    ctx.qk_scale, ctx.window_left, ctx.layout = qk_scale, window_left, layout
+    ctx.qk_scale, ctx.window_left, ctx.layout, ctx.sink_tokens = qk_scale, window_left, layout, sink_tokens
 
 
 def _backward(ctx, grad_o, *_unused):
@@ -195,19 +213,19 @@ def _backward(ctx, grad_o, *_unused):
     if grad_o.stride() != q.stride():          # one stride set for all q-like tensors: bring grad_o to q's layout
         grad_o = torch.empty_like(q).copy_(grad_o)
     dq, dr, dk, dv = train_bwd(q, r, k, v, o, barv, d1, bart, m, grad_o, ctx.qk_scale, ctx.window_left,
-                               ctx.layout, cu_seqlens)
-    return dq, dr, dk, dv, None, None, None, None
+                               ctx.layout, cu_seqlens, ctx.sink_tokens)
+    return dq, dr, dk, dv, None, None, None, None, None
 
 
 train_fwd_op.register_autograd(_backward, setup_context=_setup_ctx)
 
 
 def train_fwd(q: Tensor, r: Tensor, k: Tensor, v: Tensor, qk_scale: float, window_left: int, layout: int,
-              cu_seqlens: Optional[Tensor]) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+              cu_seqlens: Optional[Tensor], sink_tokens: int = 0) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
     """(o, barv, d1, bart, m): plx::train_fwd, a plainly eager call through the C++ host side."""
     host = eager_host()
-    res = None if host is None else host.train(q, r, k, v, qk_scale, window_left, layout, cu_seqlens)
-    return train_fwd_op(q, r, k, v, qk_scale, window_left, layout, cu_seqlens) if res is None else res
+    res = None if host is None else host.train(q, r, k, v, qk_scale, window_left, layout, cu_seqlens, sink_tokens)
+    return train_fwd_op(q, r, k, v, qk_scale, window_left, layout, cu_seqlens, sink_tokens) if res is None else res
 
 
 # --------------------------------------------------------------------------- #
@@ -252,13 +270,45 @@ def decode_workspace_floats(batch: int, heads_q: int, head_dim: int, n_splits: i
 @torch.library.custom_op("plx::decode_out", mutates_args=("out", "workspace"), device_types="cuda")
 def decode_out(q: Tensor, r: Tensor, k: Tensor, v: Tensor, out: Tensor, workspace: Tensor, qk_scale: float,
                window_left: int, n_splits: int, seqused_k: Optional[Tensor], cache_start: Optional[Tensor],
-               page_table: Optional[Tensor] = None) -> None:
+               page_table: Optional[Tensor] = None, sink_tokens: int = 0) -> None:
     p = _decode_problem(q, k, qk_scale, window_left, n_splits, 0, 0, page_table)
     with torch.cuda.device(q.device):
-        st = _cabi.lib().plx_decode(C.byref(p), _ptr(q), _ptr(r), _ptr(k), _ptr(v), _ptr(out), _ptr(seqused_k),
-                                    _ptr(cache_start), _ptr(workspace), C.c_size_t(workspace.numel() * 4),
-                                    _stream(q.device))
+        st = _entry("plx_decode", sink_tokens)(C.byref(p), _ptr(q), _ptr(r), _ptr(k), _ptr(v), _ptr(out), _ptr(seqused_k),
+                                               _ptr(cache_start), _ptr(workspace), C.c_size_t(workspace.numel() * 4),
+                                               _stream(q.device))
     _cabi.check(st, "plx_decode")
+
+
+def _prefix(k_prefix: Optional[Tensor], v_prefix: Optional[Tensor], prefix_len: int, n_splits: int) -> _cabi.Prefix:
+    """`prefix_len` keys of their own (P, H_kv, D), or without tensors the first ones of the paged cache."""
+    x = _cabi.Prefix()
+    if k_prefix is not None:
+        x.k, x.v, x.stride_t, x.stride_h = k_prefix.data_ptr(), v_prefix.data_ptr(), k_prefix.stride(0), k_prefix.stride(1)
+    x.len, x.n_splits = int(prefix_len), int(n_splits)
+    return x
+
+
+def choose_prefix_splits(batch: int, heads_q: int, heads_kv: int, prefix_len: int, device: torch.device) -> int:
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    return int(_cabi.lib().plx_decode_prefix_splits(batch, heads_q, heads_kv, prefix_len, sm_count(idx)))
+
+
+def decode_prefix_workspace_bytes(q: Tensor, k: Tensor, n_splits: int, prefix_splits: int, page_table: Optional[Tensor]) -> int:
+    p, x, need = _decode_problem(q, k, 1.0, -1, n_splits, 0, 0, page_table), _prefix(None, None, 1, prefix_splits), C.c_size_t(0)
+    _cabi.check(_cabi.lib().plx_decode_prefix_workspace_bytes(C.byref(p), C.byref(x), C.byref(need)), "plx_decode_prefix_workspace_bytes")
+    return int(need.value)
+
+
+@torch.library.custom_op("plx::decode_prefix", mutates_args=("out", "workspace"), device_types="cuda")
+def decode_prefix(q: Tensor, r: Tensor, k_prefix: Optional[Tensor], v_prefix: Optional[Tensor], prefix_len: int, k: Tensor, v: Tensor,
+                  out: Tensor, workspace: Tensor, qk_scale: float, n_splits: int, prefix_splits: int, seqused_k: Optional[Tensor],
+                  page_table: Optional[Tensor]) -> None:
+    p, x = _decode_problem(q, k, qk_scale, -1, n_splits, 0, 0, page_table), _prefix(k_prefix, v_prefix, prefix_len, prefix_splits)
+    with torch.cuda.device(q.device):
+        _cabi.raise_if_device_error("plx_decode_prefix")
+        st = _cabi.lib().plx_decode_prefix(C.byref(p), C.byref(x), _ptr(q), _ptr(r), _ptr(k), _ptr(v), _ptr(out), _ptr(seqused_k),
+                                           _ptr(workspace), C.c_size_t(workspace.numel() * 4), _stream(q.device))
+    _cabi.check(st, "plx_decode_prefix")
 
 
 @torch.library.custom_op("plx::decode_partial", mutates_args=("part", "workspace"), device_types="cuda")

@@ -22,6 +22,11 @@ def _check_cuda(name: str, *tensors: torch.Tensor) -> None:
             raise RuntimeError(f"{name}: tensors must live on a CUDA device (there is no CPU path)")
 
 
+def check_sinks(name: str, sink_tokens: int) -> None:
+    if sink_tokens < 0 or sink_tokens > 2 ** 31 - 1:
+        raise ValueError(f"{name}: sink_tokens must be a number of tokens, got {sink_tokens}")
+
+
 def _dense(x: torch.Tensor) -> bool:
     """True if x covers its memory without gaps or overlap in SOME axis order (a permuted view of a
     contiguous tensor), which is what ``torch.empty_like`` reproduces stride for stride."""
@@ -55,16 +60,18 @@ def kernel_ready(x: torch.Tensor, like: torch.Tensor | None = None) -> torch.Ten
 
 
 def parallax_func(q: torch.Tensor, r: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
-                  qk_scale: float | None = None, window_size_left: int = -1) -> torch.Tensor:
+                  qk_scale: float | None = None, window_size_left: int = -1, sink_tokens: int = 0) -> torch.Tensor:
     """Causal Parallax with autograd (reference: ``parallax_func``,
     parallax/triton/parallax_train.py:1039-1087).
 
     q, r: ``(B, H_q, L_q, D)``; k, v: ``(B, H_kv, L_kv, D)``, bf16 or fp16,
     ``H_q % H_kv == 0``.  ``qk_scale`` defaults to ``D ** -0.5`` and scales
-    ``q.k`` only.  ``window_size_left >= 0`` keeps keys ``[i - W + 1, i]``.
+    ``q.k`` only.  ``window_size_left >= 0`` keeps keys ``[i - W + 1, i]``; ``sink_tokens = S`` keeps the first S keys visible behind
+    it (to the rows from them on; without a window it changes nothing, and the reference has no such argument).
     For ``L_q != L_kv`` the causal diagonal is aligned to the END of the keys,
     as in ``parallax/reference.py:64-68``.  Returns ``(B, H_q, L_q, D)``.
     """
+    check_sinks("parallax_func", sink_tokens)
     host = ops.eager_host()
     if host is None or not host.train_ready(q, r, k, v, ops.BHLD):
         _check_dtype("parallax_func", q)
@@ -77,7 +84,7 @@ def parallax_func(q: torch.Tensor, r: torch.Tensor, k: torch.Tensor, v: torch.Te
         r, v = kernel_ready(r, q), kernel_ready(v, k)
     if qk_scale is None:
         qk_scale = q.shape[-1] ** -0.5
-    o, _, _, _, _ = ops.train_fwd(q, r, k, v, float(qk_scale), int(window_size_left), ops.BHLD, None)
+    o, _, _, _, _ = ops.train_fwd(q, r, k, v, float(qk_scale), int(window_size_left), ops.BHLD, None, int(sink_tokens))
     return o
 
 
