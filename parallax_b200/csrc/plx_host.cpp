@@ -52,6 +52,14 @@ struct Api {
     decltype(&plx_decode_choose_splits_gqa) decode_choose_splits_gqa;
     decltype(&plx_decode_workspace_bytes) decode_workspace_bytes;
     decltype(&plx_decode_sink) decode;
+    decltype(&plx_decode_prefix_splits) decode_prefix_splits;
+    decltype(&plx_decode_prefix_workspace_bytes) decode_prefix_workspace_bytes;
+    decltype(&plx_decode_prefix) decode_prefix;
+    decltype(&plx_pages_workspace_bytes) pages_workspace_bytes;
+    decltype(&plx_pages_copy) pages_copy;
+    decltype(&plx_pages_fork) pages_fork;
+    decltype(&plx_pages_compact) pages_compact;
+    decltype(&plx_pages_free) pages_free;
     decltype(&plx_decode_stage) decode_stage;
     decltype(&plx_decode_step_sink) decode_step;
 };
@@ -70,6 +78,14 @@ void bind(const py::dict &addresses) {
     bind_one(api.decode_choose_splits_gqa, addresses, "plx_decode_choose_splits_gqa");
     bind_one(api.decode_workspace_bytes, addresses, "plx_decode_workspace_bytes");
     bind_one(api.decode, addresses, "plx_decode_sink");
+    bind_one(api.decode_prefix_splits, addresses, "plx_decode_prefix_splits");
+    bind_one(api.decode_prefix_workspace_bytes, addresses, "plx_decode_prefix_workspace_bytes");
+    bind_one(api.decode_prefix, addresses, "plx_decode_prefix");
+    bind_one(api.pages_workspace_bytes, addresses, "plx_pages_workspace_bytes");
+    bind_one(api.pages_copy, addresses, "plx_pages_copy");
+    bind_one(api.pages_fork, addresses, "plx_pages_fork");
+    bind_one(api.pages_compact, addresses, "plx_pages_compact");
+    bind_one(api.pages_free, addresses, "plx_pages_free");
     bind_one(api.decode_stage, addresses, "plx_decode_stage");
     bind_one(api.decode_step, addresses, "plx_decode_step_sink");
 }
@@ -315,8 +331,10 @@ py::object train(const py::object &q_, const py::object &r_, const py::object &k
 // workspace is only ever used on the stream it was allocated on, so the allocator reuses its memory in stream order.
 class Workspaces {
 public:
-    Tensor get(const c10::cuda::CUDAStream &stream, const Tensor &q, int n_splits, int64_t floats) {
-        const Key key{q.get_device(), static_cast<int64_t>(reinterpret_cast<uintptr_t>(stream.stream())), q.size(0), q.size(2), q.size(3), n_splits};
+    // prefix_splits: of a call behind a shared prefix, whose workspace is another; else 0
+    Tensor get(const c10::cuda::CUDAStream &stream, const Tensor &q, int n_splits, int64_t floats, int prefix_splits = 0) {
+        const Key key{q.get_device(), static_cast<int64_t>(reinterpret_cast<uintptr_t>(stream.stream())), q.size(0), q.size(2), q.size(3), n_splits,
+                      prefix_splits};
         std::lock_guard<std::mutex> lock(mu_);
         for (auto it = list_.begin(); it != list_.end(); ++it)
             if (it->first == key) {
@@ -329,7 +347,7 @@ public:
     }
 
 private:
-    using Key = std::array<int64_t, 6>;
+    using Key = std::array<int64_t, 7>;
     static constexpr size_t kMax = 32;
     std::mutex mu_;
     std::list<std::pair<Key, Tensor>> list_;
@@ -553,6 +571,54 @@ py::object decode(const py::object &q_, const py::object &r_, const py::object &
     return py::reinterpret_steal<py::object>(THPVariable_Wrap(out));
 }
 
+// Behind a shared prefix of its own tensors (P, H_kv, D), or (those None) of `prefix_len` keys in the pages of the cache.
+py::object decode_prefix(const py::object &q_, const py::object &r_, const py::object &kp_, const py::object &vp_, int64_t prefix_len, const py::object &k_,
+                         const py::object &v_, const py::object &scale_, const py::object &lens_, const py::object &table_) {
+    bool ok = true;
+    const Tensor q = take(q_, ok), r = take(r_, ok), k = take(k_, ok), v = take(v_, ok);
+    const OptTensor kp = take_optional(kp_, ok), vp = take_optional(vp_, ok), lens = take_optional(lens_, ok), table = take_optional(table_, ok);
+    if (!ok || !plain_thread() || !cache_call_ok(q, r, k, v, lens, table) || q.size(1) != 1 || std::getenv("PLX_DECODE_SPLITS")) return py::none();
+    plx_prefix x{};
+    if (kp) {
+        if (!vp || table || !plain_tensor(*kp) || !plain_tensor(*vp) || recorded({&*kp, &*vp}) || kp->dim() != 3 || vp->sizes() != kp->sizes() ||
+            vp->strides() != kp->strides())
+            return py::none();
+        for (const Tensor *t : Tensors{&*kp, &*vp})
+            if (t->scalar_type() != q.scalar_type() || t->device() != q.device() || t->size(0) != prefix_len || prefix_len == 0 ||
+                t->size(1) != k.size(2) || t->size(2) != k.size(3) || t->stride(2) != 1 || t->stride(0) % 8 != 0 || t->stride(1) % 8 != 0 || !aligned16(*t))
+                return py::none();
+        x.k = kp->data_ptr();
+        x.v = vp->data_ptr();
+        x.stride_t = kp->stride(0);
+        x.stride_h = kp->stride(1);
+    } else if (!table || prefix_len <= 0 || prefix_len % k.size(1) != 0) {
+        return py::none();
+    }
+    double scale;
+    const int64_t ceiling = table ? table->size(1) * k.size(1) : k.size(1), least = kp ? 0 : prefix_len;
+    if (!take_scale(scale_, q.size(3), scale) || ceiling > INT32_MAX || prefix_len > INT32_MAX || least > ceiling) return py::none();
+    at::AutoDispatchBelowADInplaceOrView below;
+    const c10::cuda::CUDAGuard device(q.device());
+    if (capturing() || device_error_waiting()) return py::none();
+    RECORD_FUNCTION("plx::decode_prefix", Values({q, r, k, v}));
+    const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream();
+    const int sms = at::cuda::getDeviceProperties(q.get_device())->multiProcessorCount;
+    plx_decode_problem p = decode_problem(q, k, ceiling, table, scale, -1, 1);
+    p.n_splits = api.decode_choose_splits_gqa(p.batch, p.heads_q, p.heads_kv, static_cast<int32_t>(std::max<int64_t>(1, ceiling - least)), sms);
+    x.len = static_cast<int32_t>(prefix_len);
+    x.n_splits = api.decode_prefix_splits(p.batch, p.heads_q, p.heads_kv, x.len, sms);
+    size_t need = 0;
+    if (api.decode_prefix_workspace_bytes(&p, &x, &need) != PLX_OK) return py::none();
+    const Tensor ws = workspaces().get(stream, q, p.n_splits, static_cast<int64_t>(need / sizeof(float)), x.n_splits);
+    Tensor out = at::empty(q.sizes(), q.options());
+    LengthCheck check(lens, stream, true);
+    if (api.decode_prefix(&p, &x, q.data_ptr(), r.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), int_ptr(lens), ws.data_ptr(), need,
+                          stream.stream()) != PLX_OK ||
+        !check.within(least, ceiling))
+        return py::none();
+    return py::reinterpret_steal<py::object>(THPVariable_Wrap(out));
+}
+
 // L_q > 1: one launch of the training forward kernel against the cache.
 py::object extend(const py::object &q_, const py::object &r_, const py::object &k_, const py::object &v_, const py::object &scale_,
                   const py::object &window_, const py::object &lens_, const py::object &table_, const py::object &sinks_) {
@@ -667,6 +733,123 @@ int step(const py::object &q_, const py::object &q_src_, const py::object &r_, c
                ? kStaged : kNothing;
 }
 
+// ------------------------------------------------------------------------- //
+// pages of a cache (pages.py)
+// ------------------------------------------------------------------------- //
+bool take_pool(const Tensor &k, const Tensor &v, plx_page_pool &p) {
+    for (const Tensor *t : Tensors{&k, &v}) {
+        if (!plain_tensor(*t) || t->dim() != 4 || dtype_code(*t) < 0 || t->numel() == 0 || t->stride(3) != 1 || !aligned16(*t)) return false;
+        for (int i = 0; i < 3; ++i)
+            if (t->stride(i) % 8 != 0 || (t->stride(i) == 0 && t->size(i) > 1)) return false;
+    }
+    const int64_t page = k.size(1);
+    if (v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type() || v.device() != k.device() || (page & (page - 1)) != 0 || k.size(3) % 8 != 0 ||
+        k.size(0) > INT32_MAX || recorded({&k, &v}))
+        return false;
+    p = plx_page_pool{};
+    p.k = k.data_ptr();
+    p.v = v.data_ptr();
+    p.n_pages = static_cast<int32_t>(k.size(0));
+    p.page_size = static_cast<int32_t>(page);
+    p.heads_kv = static_cast<int32_t>(k.size(2));
+    p.head_dim = static_cast<int32_t>(k.size(3));
+    p.k_stride_p = k.stride(0); p.k_stride_t = k.stride(1); p.k_stride_h = k.stride(2);
+    p.v_stride_p = v.stride(0); p.v_stride_t = v.stride(1); p.v_stride_h = v.stride(2);
+    return true;
+}
+bool int32_list(const Tensor &t, const at::Device &device) { return t.dim() == 1 && int32_vector(t, t.size(0), device); }
+bool tables_ok(const Tensor &table, const Tensor &lens, const at::Device &device) {
+    return plain_tensor(table) && table.dim() == 2 && table.numel() > 0 && page_table_ok(table, table.size(0), 1, device) &&
+           int32_vector(lens, table.size(0), device);
+}
+int32_t *ints(const Tensor &t) { return static_cast<int32_t *>(t.data_ptr()); }
+// scratch needs no contents, so it comes from the allocator, in stream order (and in a capture from the graph's own pool)
+Tensor pages_scratch(const Tensor &like, int64_t n_pages, int64_t batch, int64_t n_forks) {
+    size_t need = 0;
+    if (api.pages_workspace_bytes(static_cast<int32_t>(n_pages), static_cast<int32_t>(batch), static_cast<int32_t>(n_forks), &need) != PLX_OK) return Tensor();
+    return at::empty({static_cast<int64_t>(need)}, like.options().dtype(at::kByte));
+}
+// written in place: as a mutating op would, tell autograd's version counters
+void written(const Tensor &k, const Tensor &v) {
+    for (const Tensor *t : Tensors{&k, &v})
+        if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
+bool pages_copy(const py::object &k_, const py::object &v_, const py::object &src_, const py::object &dst_) {
+    bool ok = true;
+    const Tensor k = take(k_, ok), v = take(v_, ok), src = take(src_, ok), dst = take(dst_, ok);
+    plx_page_pool p;
+    if (!ok || !plain_thread() || !take_pool(k, v, p) || !int32_list(src, k.device()) || !int32_list(dst, k.device()) || src.numel() != dst.numel() ||
+        src.numel() == 0 || src.numel() > INT32_MAX)
+        return false;
+    const c10::cuda::CUDAGuard device(k.device());
+    RECORD_FUNCTION("plx::pages_copy", Values({k, v, src, dst}));
+    if (api.pages_copy(&p, ints(src), ints(dst), static_cast<int32_t>(src.numel()), c10::cuda::getCurrentCUDAStream().stream()) != PLX_OK) return false;
+    written(k, v);
+    return true;
+}
+
+py::object wrap(const Tensor &t) { return py::reinterpret_steal<py::object>(THPVariable_Wrap(t)); }
+
+py::object pages_fork(const py::object &k_, const py::object &v_, const py::object &table_, const py::object &lens_, const py::object &parents_,
+                      const py::object &children_) {
+    bool ok = true;
+    const Tensor k = take(k_, ok), v = take(v_, ok), table = take(table_, ok), lens = take(lens_, ok), parents = take(parents_, ok), children = take(children_, ok);
+    plx_page_pool p;
+    if (!ok || !plain_thread() || !take_pool(k, v, p) || !tables_ok(table, lens, k.device()) || !int32_list(parents, k.device()) ||
+        !int32_list(children, k.device()) || parents.numel() != children.numel() || parents.numel() == 0 || parents.numel() > INT32_MAX)
+        return py::none();
+    at::AutoDispatchBelowADInplaceOrView below;
+    const c10::cuda::CUDAGuard device(k.device());
+    RECORD_FUNCTION("plx::pages_fork", Values({k, v, table, lens, parents, children}));
+    const Tensor ws = pages_scratch(k, p.n_pages, table.size(0), parents.numel());
+    if (!ws.defined()) return py::none();
+    Tensor new_table = at::empty(table.sizes(), table.options()), new_lens = at::empty(lens.sizes(), lens.options()), missing = at::empty({1}, lens.options());
+    if (api.pages_fork(&p, ints(table), ints(lens), static_cast<int32_t>(table.size(0)), static_cast<int32_t>(table.size(1)), ints(parents), ints(children),
+                       static_cast<int32_t>(parents.numel()), ints(new_table), ints(new_lens), ints(missing), ws.data_ptr(), ws.nbytes(),
+                       c10::cuda::getCurrentCUDAStream().stream()) != PLX_OK)
+        return py::none();
+    written(k, v);
+    return py::make_tuple(wrap(new_table), wrap(new_lens), wrap(missing));
+}
+
+py::object pages_compact(const py::object &k_, const py::object &v_, const py::object &table_, const py::object &lens_) {
+    bool ok = true;
+    const Tensor k = take(k_, ok), v = take(v_, ok), table = take(table_, ok), lens = take(lens_, ok);
+    plx_page_pool p;
+    if (!ok || !plain_thread() || !take_pool(k, v, p) || !tables_ok(table, lens, k.device())) return py::none();
+    at::AutoDispatchBelowADInplaceOrView below;
+    const c10::cuda::CUDAGuard device(k.device());
+    RECORD_FUNCTION("plx::pages_compact", Values({k, v, table, lens}));
+    const Tensor ws = pages_scratch(k, p.n_pages, table.size(0), 0);
+    if (!ws.defined()) return py::none();
+    Tensor new_table = at::empty(table.sizes(), table.options()), n_live = at::empty({1}, lens.options());
+    if (api.pages_compact(&p, ints(table), ints(lens), static_cast<int32_t>(table.size(0)), static_cast<int32_t>(table.size(1)), ints(new_table),
+                          ints(n_live), ws.data_ptr(), ws.nbytes(), c10::cuda::getCurrentCUDAStream().stream()) != PLX_OK)
+        return py::none();
+    written(k, v);
+    return py::make_tuple(wrap(new_table), wrap(n_live));
+}
+
+py::object pages_free(const py::object &table_, const py::object &lens_, const py::object &rows_, int64_t n_pages, int64_t page_size) {
+    bool ok = true;
+    const Tensor table = take(table_, ok), lens = take(lens_, ok), rows = take(rows_, ok);
+    if (!ok || !plain_thread() || !tables_ok(table, lens, table.device()) || !int32_list(rows, table.device()) || n_pages < 1 || n_pages > INT32_MAX ||
+        page_size < 1 || page_size > INT32_MAX)
+        return py::none();
+    at::AutoDispatchBelowADInplaceOrView below;
+    const c10::cuda::CUDAGuard device(table.device());
+    RECORD_FUNCTION("plx::pages_free", Values({table, lens, rows}));
+    const Tensor ws = pages_scratch(table, n_pages, table.size(0), 0);
+    if (!ws.defined()) return py::none();
+    Tensor new_lens = at::empty(lens.sizes(), lens.options()), free_list = at::empty({n_pages}, lens.options()), n_free = at::empty({1}, lens.options());
+    if (api.pages_free(ints(table), ints(lens), static_cast<int32_t>(table.size(0)), static_cast<int32_t>(table.size(1)), ints(rows),
+                       static_cast<int32_t>(rows.numel()), static_cast<int32_t>(n_pages), static_cast<int32_t>(page_size), ints(new_lens), ints(free_list),
+                       ints(n_free), ws.data_ptr(), ws.nbytes(), c10::cuda::getCurrentCUDAStream().stream()) != PLX_OK)
+        return py::none();
+    return py::make_tuple(wrap(new_lens), wrap(free_list), wrap(n_free));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_plx_host, m) {
@@ -676,6 +859,11 @@ PYBIND11_MODULE(_plx_host, m) {
     m.def("train", &train, py::arg("q"), py::arg("r"), py::arg("k"), py::arg("v"), py::arg("scale"), py::arg("window"), py::arg("layout"), py::arg("cu_seqlens"), py::arg("sink_tokens") = 0);
     m.def("decode", &decode, py::arg("q"), py::arg("r"), py::arg("k"), py::arg("v"), py::arg("scale"), py::arg("window"), py::arg("seqused_k"), py::arg("cache_start"), py::arg("page_table"), py::arg("sink_tokens") = 0);
     m.def("attend", &attend, py::arg("q"), py::arg("r"), py::arg("k"), py::arg("v"), py::arg("scale"), py::arg("window"), py::arg("seqused_k"), py::arg("page_table"), py::arg("sink_tokens") = 0);
+    m.def("decode_prefix", &decode_prefix);
+    m.def("pages_copy", &pages_copy);
+    m.def("pages_fork", &pages_fork);
+    m.def("pages_compact", &pages_compact);
+    m.def("pages_free", &pages_free);
     m.def("apart", &apart);
     m.def("step", &step, py::arg("q"), py::arg("q_src"), py::arg("r"), py::arg("r_src"), py::arg("lens"), py::arg("lens_src"), py::arg("most"), py::arg("k"), py::arg("v"), py::arg("out"), py::arg("workspace"), py::arg("scale"), py::arg("window"), py::arg("n_splits"), py::arg("sink_tokens") = 0);
     m.def("side_streams_made", [] { return side_streams().made(); });

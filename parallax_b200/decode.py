@@ -262,6 +262,11 @@ def _prefix_workspace(q, k, n_splits: int, prefix_splits: int, page_table) -> to
 
 
 def _prefix_core(q, r, k_prefix, v_prefix, prefix_len: int, k, v, scale, *, seqused_k, page_table, out) -> torch.Tensor:
+    host = ops.eager_host() if out is None else None
+    if host is not None:
+        res = host.decode_prefix(q, r, k_prefix, v_prefix, prefix_len, k, v, scale, seqused_k, page_table)
+        if res is not None:
+            return res
     name = "parallax_decode_shared_prefix" if page_table is None else "parallax_attn_with_kvcache"
     if q.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"{name} requires bf16 or fp16 input, got {q.dtype}")

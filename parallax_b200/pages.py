@@ -19,7 +19,7 @@ import torch
 from torch import Tensor
 
 from . import _cabi
-from .ops import _ptr, _stream
+from .ops import _ptr, _stream, eager_host
 
 
 def _pool(k: Tensor, v: Tensor) -> _cabi.PagePool:
@@ -162,6 +162,9 @@ def parallax_copy_pages(k_cache: Tensor, v_cache: Tensor, src: Tensor, dst: Tens
     ``src``, ``dst``: int32 vectors of one length.  Entries out of range (-1, say, to pad a list to a fixed length) are passed
     over.  No page may be a target twice, or a source and a target: what such a page holds afterwards is not defined.
     """
+    host = eager_host()
+    if host is not None and host.pages_copy(k_cache, v_cache, src, dst):
+        return
     _check_pool("parallax_copy_pages", k_cache, v_cache)
     _check_lists("parallax_copy_pages", src=src, dst=dst)
     _check_cuda("parallax_copy_pages", k_cache, src, dst)
@@ -179,6 +182,10 @@ def parallax_fork_pages(k_cache: Tensor, v_cache: Tensor, page_table: Tensor, se
     before the call, in the order of the lists.  ``n_missing`` (one int32 on the device) counts the children for which there was
     none: their rows end with the whole pages (and the entry behind those is -1).
     """
+    host = eager_host()
+    res = None if host is None else host.pages_fork(k_cache, v_cache, page_table, seqused_k, parents, children)
+    if res is not None:
+        return res
     name = "parallax_fork_pages"
     _check_pool(name, k_cache, v_cache)
     _check_table(name, page_table, seqused_k)
@@ -195,6 +202,10 @@ def parallax_compact_pages(k_cache: Tensor, v_cache: Tensor, page_table: Tensor,
     Of ``n_live`` live pages (one int32 on the device) the i-th from page ``n_live`` on goes to the i-th free page below it, and the
     tables follow; pages that are in place stay there, shared pages stay shared.  All pages from ``n_live`` on are free afterwards.
     """
+    host = eager_host()
+    res = None if host is None else host.pages_compact(k_cache, v_cache, page_table, seqused_k)
+    if res is not None:
+        return res
     name = "parallax_compact_pages"
     _check_pool(name, k_cache, v_cache)
     _check_table(name, page_table, seqused_k)
@@ -209,6 +220,10 @@ def parallax_free_pages(page_table: Tensor, seqused_k: Tensor, rows: Tensor, n_p
     that are not live then, ascending, -1 behind the last; ``n_free`` (one int32 on the device) is their number.  A page that another
     row shares stays live.
     """
+    host = eager_host()
+    res = None if host is None else host.pages_free(page_table, seqused_k, rows, n_pages, page_size)
+    if res is not None:
+        return res
     name = "parallax_free_pages"
     _check_table(name, page_table, seqused_k)
     _check_lists(name, rows=rows)
