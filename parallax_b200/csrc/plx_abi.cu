@@ -162,6 +162,7 @@ struct Sweep {
     int first_key = 0;         // keys before it are not looked at
     int min_len = 1;           // shorter lengths count as it
     int part_stride = 1;       // records between those of two (batch, head)
+    int let_next_in = 0;       // the next launch may begin under this one
 };
 
 static int run_decode(const plx_decode_problem *p, const void *q, const void *r, const void *k, const void *v, void *out,
@@ -182,6 +183,7 @@ static int run_decode(const plx_decode_problem *p, const void *q, const void *r,
     a.sink = p->window_left >= 0 && p->window_left < p->cache_len ? (sweep.sink < p->cache_len ? sweep.sink : p->cache_len) : 0;
     a.first_key = sweep.first_key;
     a.min_len = sweep.min_len;
+    a.let_next_in = sweep.let_next_in;
     a.seqused = seqused_k;
     a.cache_start = cache_start;
     const size_t bh = static_cast<size_t>(p->batch) * p->heads_q;
@@ -625,33 +627,33 @@ int plx_decode_prefix(const plx_decode_problem *p, const plx_prefix *x, const vo
         while ((1 << a.page_shift) < p->page_size) ++a.page_shift;
     }
     a.parts = parts;
-    const Sweep own{0, in_cache ? x->len : 0, in_cache ? x->len : 0, 0};
-    auto sweep_own = [&](int n_parts) {
-        Sweep s = own;
-        s.part_stride = n_parts;
-        return run_decode(p, q, r, k, v, nullptr, parts + static_cast<size_t>(n_parts - 1) * PLX_DECODE_PART_FLOATS(p->head_dim), seqused_k, nullptr, rest,
-                          rest_bytes, cs, nullptr, nullptr, s);
-    };
-    int n_parts;
-    if (train_extend_sm100_supported(a, p->head_dim)) {
+    const bool tensor_cores = train_extend_sm100_supported(a, p->head_dim);
+    // pages that the tensor-core kernel does not take: the prefix is swept with the rest of each row
+    if (!tensor_cores && in_cache) return run_decode(p, q, r, k, v, out, nullptr, seqused_k, nullptr, rest, rest_bytes, cs);
+    const int n_parts = tensor_cores ? x->n_splits + 1 : 2;
+    // Each row's own keys first: the items of the prefix, all alike, are handed out to the SMs as the sweep leaves them.
+    Sweep own;
+    own.first_key = own.min_len = in_cache ? x->len : 0;
+    own.part_stride = n_parts;
+    own.let_next_in = tensor_cores;
+    st = run_decode(p, q, r, k, v, nullptr, parts + static_cast<size_t>(n_parts - 1) * PLX_DECODE_PART_FLOATS(p->head_dim), seqused_k, nullptr, rest, rest_bytes,
+                    cs, nullptr, nullptr, own);
+    if (st != PLX_OK) return st;
+    if (tensor_cores) {
         a.n_splits = x->n_splits;
-        a.n_parts = n_parts = x->n_splits + 1;
+        a.n_parts = n_parts;
         st = launch_prefix_sm100(a, p->dtype, p->head_dim, cs);
-    } else if (in_cache) {
-        return run_decode(p, q, r, k, v, out, nullptr, seqused_k, nullptr, rest, rest_bytes, cs);      // pages: the prefix is swept with the rest of each row
     } else {
-        // a scale or strides that the tensor-core kernel does not take: every row sweeps the prefix
+        // a scale or strides that it does not take either: every row sweeps the prefix
         plx_decode_problem prefix = *p;
         prefix.page_table = nullptr;
         prefix.cache_len = x->len;
-        prefix.window_left = -1;
         prefix.kv_offset = prefix.total_len = 0;
         prefix.kv_stride_b = 0; prefix.kv_stride_t = x->stride_t; prefix.kv_stride_h = x->stride_h;
         Sweep s;
-        s.part_stride = n_parts = 2;
+        s.part_stride = n_parts;
         st = run_decode(&prefix, q, r, x->k, x->v, nullptr, parts, nullptr, nullptr, rest, rest_bytes, cs, nullptr, nullptr, s);
     }
-    if (st == PLX_OK) st = sweep_own(n_parts);
     if (st != PLX_OK) return st;
     return launch_prefix_merge(parts, n_parts, static_cast<int64_t>(p->batch) * p->heads_q, p->head_dim, p->dtype, out, cs);
 }

@@ -449,6 +449,7 @@ static cudaError_t launch_overlapped(void (*kern)(Params...), dim3 grid, int thr
 template <typename T, int D, int HG, int U, bool SG, bool DEAL, bool SINK = false>
 __global__ void __launch_bounds__(HG * 32, U > 4 ? 1 : 512 / (HG * 32)) decode_kernel(const DecodeArgs a) {
     grid_wait();
+    if (a.let_next_in) launch_dependents();
     constexpr int LPK = D / 8;      // lanes per key row
     constexpr int NS = 32 / LPK;    // streams per warp
     constexpr int REC = 2 * D + 4;  // floats per partial record
@@ -998,6 +999,7 @@ struct GqaSmem {
 template <typename T, int D, bool PAGED, bool FEW, bool SINK = false>
 __global__ void __launch_bounds__(kGqaWarps * 32, 1) decode_gqa_kernel(const DecodeArgs a, int n_hgroups) {
     grid_wait();
+    if (a.let_next_in) launch_dependents();
     constexpr int LD = D + 8;                       // padded row: ldmatrix without bank conflicts
     constexpr int REC = 2 * D + 4, CH = D / 32;
     constexpr int KS = D / 16;                      // k-steps of the score products

@@ -32,6 +32,7 @@ struct DecodeArgs {
     int batch, heads_q, heads_kv, n_rep, cache_len, window, n_splits, kv_offset, total_len;
     int sink;          // keys in front that stay visible behind the window (0 without one)
     int first_key, min_len;   // keys before first_key are another launch's (0); lengths below min_len count as it (1)
+    int let_next_in;          // the next launch may begin under this one (it waits for its end by itself)
     float c2;  // qk_scale * log2(e)
     int64_t kv_sb, kv_st, kv_sh;   // paged: kv_sb is the stride between pages
     // paged cache (page_table != nullptr): key j of batch row b lives in page

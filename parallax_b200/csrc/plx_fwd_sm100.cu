@@ -312,8 +312,8 @@ fwd_sm100_kernel(const TrainArgs a, const __grid_constant__ CUtensorMap tm_q, co
                     if (DYN && n_items_done > 0)
 #pragma unroll
                         for (int pn = 0; pn < L::kPanels; ++pn) {
-                            tma_prefetch_4d(&tm_q, 64 * pn, it.bos + it.r0, it.h, it.b);
-                            tma_prefetch_4d(&tm_r, 64 * pn, it.bos + it.r0, it.h, it.b);
+                            tma_prefetch_4d(&tm_q, 64 * pn, PART ? it.h : it.bos + it.r0, PART ? it.hk : it.h, it.b);
+                            tma_prefetch_4d(&tm_r, 64 * pn, PART ? it.h : it.bos + it.r0, PART ? it.hk : it.h, it.b);
                         }
                     // the q / r tiles of the previous item are free once its last score product has completed
                     ok = mbar_wait(bar(L::kQEmpty), (n_items_done & 1) ^ 1, err, 1);
@@ -337,8 +337,8 @@ fwd_sm100_kernel(const TrainArgs a, const __grid_constant__ CUtensorMap tm_q, co
 #pragma unroll
                         for (int i = 0; i < kMaxBoxes; ++i) {
                             const int key = key0 + (i << box_shift);
-                            page[i] = (i << box_shift) < kBN && key < it.nk
-                                          ? __ldg(a.page_table + static_cast<int64_t>(kb) * a.pages_per_seq + (key >> a.page_shift)) : 0;
+                            const int32_t *entry = a.page_table + static_cast<int64_t>(kb) * a.pages_per_seq + (key >> a.page_shift);
+                            page[i] = (i << box_shift) < kBN && key < it.nk ? (PART ? __ldcg(entry) : __ldg(entry)) : 0;
                         }
                     }
                     ok = mbar_wait(bar(empty0 + s), ph ^ 1, err, is_k ? 2 : 3);
@@ -815,6 +815,9 @@ fwd_sm100_kernel(const TrainArgs a, const __grid_constant__ CUtensorMap tm_q, co
     tc_fence_before();
     __syncthreads();
     if (warp == 1) tmem_dealloc(tmem_base, kTmemCols);
+    // A prefix is launched under the end of the sweep of the rows' own keys.  What it reads was complete before that let it in; it
+    // ends behind it, so that whatever follows on the stream follows both.
+    if (PART) grid_wait();
 }
 
 // ------------------------------------------------------------------------- //
@@ -893,12 +896,25 @@ int launch_t(const TrainArgs &a, cudaStream_t stream) {
     if constexpr (PART) {
         static std::mutex mu;
         static bool done[tma::kMaxDevices] = {};
+        // A CTA per item: they take the SMs as the sweep before leaves them.  (Handed on from item to item a CTA asks for the next
+        // one when it begins one, and with about an item per SM the first SMs to be free keep two: 32 rows, 32 : 8 heads, 8192 keys
+        // 40 us against 24.)
         auto kern = fwd_sm100_kernel<T, D, NS, MODE, false>;
         if (!tma::opt_in_smem(kern, static_cast<int>(L::kBytes), done, mu)) return PLX_ERR_LAUNCH;
-        const int n_rt = ((a.n_rep + a.box_h - 1) / a.box_h) * ((a.batch + a.box_b - 1) / a.box_b), n = n_rt * a.heads_kv * a.n_splits;
-        kern<<<n < sms ? n : sms, 352, L::kBytes, stream>>>(a, tq, tr, tk, tv, sink, n_rt, n, 0, 0);
+        const int n_rt = prefix_row_tiles(a.n_rep, a.batch), n = n_rt * a.heads_kv * a.n_splits;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(n);
+        cfg.blockDim = dim3(352);
+        cfg.dynamicSmemBytes = L::kBytes;
+        cfg.stream = stream;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        const cudaError_t st = cudaLaunchKernelEx(&cfg, kern, a, tq, tr, tk, tv, sink, n_rt, n, 0, 0);
         count_launch();
-        return cudaGetLastError() == cudaSuccess ? PLX_OK : PLX_ERR_LAUNCH;
+        return st == cudaSuccess && cudaGetLastError() == cudaSuccess ? PLX_OK : PLX_ERR_LAUNCH;
     } else {
     const int tiles = a.cu ? (a.len_q + kBM - 1) / kBM + a.n_seqs : (a.len_q + kBM - 1) / kBM;
     const int n_items = tiles * a.batch * a.heads_q;
@@ -953,7 +969,7 @@ int launch_train_extend_sm100(const TrainArgs &a, int dtype, int head_dim, cudaS
     return a.sink ? launch_mode<kExtendSink>(a, dtype, head_dim, stream) : launch_mode<kExtend>(a, dtype, head_dim, stream);
 }
 
-// A prefix: as against a cache.  `a` holds q, r, the keys (dense: one row of len_k; paged: a row of the page table), `parts` and
+// A prefix, behind a decode launch that lets it in early: as against a cache.  `a` holds q, r, the keys (dense: one row of len_k; paged: a row of the page table), `parts` and
 // n_parts; n_splits is the caller's (see prefix_splits), box_h and box_b follow from the heads.
 int launch_prefix_sm100(const TrainArgs &problem, int dtype, int head_dim, cudaStream_t stream) {
     TrainArgs a = problem;
