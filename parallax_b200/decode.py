@@ -9,6 +9,7 @@ keyword arguments.
 """
 from __future__ import annotations
 
+import gc
 import math
 from typing import Optional
 
@@ -477,8 +478,16 @@ class GraphedDecode:
                 call()
         torch.cuda.current_stream(self.q.device).wait_stream(side)
         self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
-            call()
+        # A graph that the garbage collector comes across while a stream is being captured is destroyed there and then, which CUDA
+        # does not permit and which ends the capture: what is garbage waits until this one is over.
+        collects = gc.isenabled()
+        gc.disable()
+        try:
+            with torch.cuda.graph(self.graph):
+                call()
+        finally:
+            if collects:
+                gc.enable()
 
     def replay(self) -> torch.Tensor:
         self.graph.replay()

@@ -5,7 +5,7 @@ import torch
 
 import parallax_b200 as plx
 from parallax_b200 import _cabi
-from tests.test_sinks_gpu import attend, close, randn
+from tests.test_sinks_gpu import attend, close, no_collection, randn
 
 pytestmark = pytest.mark.gpu
 BF, FP = torch.bfloat16, torch.float16
@@ -135,7 +135,7 @@ def test_captured_and_replayed_on_two_streams():
         plx.parallax_decode_shared_prefix(*args, seqused_k=lens)
         torch.cuda.synchronize()
         graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph):
+        with no_collection(), torch.cuda.graph(graph):
             out = plx.parallax_decode_shared_prefix(*args, seqused_k=lens)
         calls.append((graph, out, args, lens))
     for round_ in range(3):

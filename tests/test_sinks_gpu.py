@@ -3,6 +3,9 @@
 Tolerances (relative 2-norm), in halves of a step of the 16-bit type: one for the rounding of the result, one for that of the
 weights which multiply v (or k, q, r, dO), and for gradients one more for o and bar v, which the forward leaves in 16 bits.
 """
+import contextlib
+import gc
+
 import pytest
 import torch
 
@@ -10,6 +13,16 @@ import parallax_b200 as plx
 
 pytestmark = pytest.mark.gpu
 BF, FP = torch.bfloat16, torch.float16
+
+
+@contextlib.contextmanager
+def no_collection():
+    """No garbage collection inside: a graph that it destroys during a capture ends the capture."""
+    gc.disable()
+    try:
+        yield
+    finally:
+        gc.enable()
 
 
 def half_steps(dtype, n):
@@ -204,7 +217,7 @@ def test_captured_training_step():
         step()
     torch.cuda.current_stream().wait_stream(side)
     graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
+    with no_collection(), torch.cuda.graph(graph):
         out = step()
     with torch.no_grad():
         q.copy_(randn(*q.shape, seed=31))
@@ -338,6 +351,23 @@ def test_graphed_decode(hq, hkv):
         close(gd.replay().clone(), want, 2, "replay")
 
 
+def test_graphs_that_are_garbage_do_not_end_a_capture():
+    """A GraphedDecode made while the collector would run at every allocation and find an older one."""
+    def litter():
+        old = plx.GraphedDecode(1, 4, 64, 64)
+        old.itself = old
+
+    gc.collect()
+    before = gc.get_threshold()
+    litter()
+    try:
+        gc.set_threshold(1, 1, 1)
+        gd = plx.GraphedDecode(1, 8, 300, 64, window_size=50, sink_tokens=2)
+    finally:
+        gc.set_threshold(*before)
+    assert gc.isenabled() and torch.isfinite(gd.replay()).all()
+
+
 def test_two_captured_calls_do_not_share_a_workspace():
     b, h, t, d, window, sinks = 2, 8, 3000, 128, 1000, 4
     calls, streams = [], [torch.cuda.Stream(), torch.cuda.Stream()]
@@ -347,7 +377,7 @@ def test_two_captured_calls_do_not_share_a_workspace():
         plx.parallax_decode(q, r, k, v, window_size_left=window, sink_tokens=sinks)
         torch.cuda.synchronize()
         graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph):
+        with no_collection(), torch.cuda.graph(graph):
             out = plx.parallax_decode(q, r, k, v, window_size_left=window, sink_tokens=sinks)
         calls.append((graph, out, decode_reference(q, r, k, v, [t] * b, [0] * b, window, sinks), (q, r, k, v)))     # (the inputs stay alive)
     torch.cuda.synchronize()
