@@ -4,8 +4,8 @@
 // be captured; what a table holds beyond a row's active entries is not looked at, and page or row numbers out of range
 // are passed over.
 //
-// A call is two launches (copying: one).  The PLAN is one CTA: a bitmap of the live pages in shared memory (one bit a
-// page: 1.5 million pages; beyond that in global memory), filled from the active entries, counted once, from which ranks
+// A call is two launches (copying: one).  The PLAN is one CTA: a bitmap of the live pages in shared memory (up to 524288
+// pages; beyond that in global memory), filled from the active entries, counted once, from which ranks
 // of live and free pages follow by popcount.  The APPLICATION is spread over the chip: table entries, and pages cut into
 // pieces of 16 KB that CTAs take in turn, four 16-byte loads a thread in flight.
 #include <mutex>
@@ -20,7 +20,7 @@ namespace {
 constexpr int kPlanThreads = 1024;
 constexpr int kCopyThreads = 256, kCopyUnroll = 4;              // 16 KB of a page per CTA and step
 constexpr int kPieceChunks = kCopyThreads * kCopyUnroll;
-constexpr int kMaxBitmapWords = 48 * 1024;                      // 192 KB of shared memory: 1572864 pages
+constexpr int kMaxBitmapWords = 32 * 1024;                      // bitmap and ranks, 128 KB of shared memory: 524288 pages
 
 struct PoolArgs {
     void *k, *v;
@@ -81,19 +81,29 @@ __device__ __forceinline__ void clear(const Bitmap &m) {
 // The active entries of the table -> bits; len(b): the keys of row b.
 template <typename Len>
 __device__ __forceinline__ void mark(const Bitmap &m, const TableArgs &t, Len len) {
-    // a warp takes 128 entries of a row at a time
-    constexpr int kAhead = 4;
+    // a warp takes 128 entries of a row at a time, of two rows at once: bound by the round trips for lengths and entries
+    constexpr int kAhead = 4, kRows = 2;
     const int lane = threadIdx.x & 31, segments = (t.pages_per_seq + 32 * kAhead - 1) / (32 * kAhead), units = t.batch * segments;
-    for (int unit = threadIdx.x >> 5; unit < units; unit += kPlanThreads / 32) {
-        const int b = unit / segments, j0 = (unit - b * segments) * 32 * kAhead + lane;
-        const int active = static_cast<int>(min((static_cast<int64_t>(max(len(b), 0)) + t.mask) >> t.shift, static_cast<int64_t>(t.pages_per_seq)));
-        const int32_t *row = t.table + static_cast<int64_t>(b) * t.pages_per_seq;
-        int p[kAhead];
+    for (int unit0 = threadIdx.x >> 5; unit0 < units; unit0 += kRows * kPlanThreads / 32) {
+        int p[kRows][kAhead], active[kRows];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) p[u] = j0 + 32 * u < active ? row[j0 + 32 * u] : -1;
+        for (int i = 0; i < kRows; ++i) {
+            const int unit = unit0 + i * kPlanThreads / 32;
+            active[i] = unit < units ? static_cast<int>(min((static_cast<int64_t>(max(len(unit / segments), 0)) + t.mask) >> t.shift,
+                                                            static_cast<int64_t>(t.pages_per_seq))) : 0;
+        }
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u)
-            if (t.in_pool(p[u])) atomicOr(m.bits + (p[u] >> 5), 1u << (p[u] & 31));
+        for (int i = 0; i < kRows; ++i) {
+            const int unit = unit0 + i * kPlanThreads / 32, b = unit / segments, j0 = (unit - b * segments) * 32 * kAhead + lane;
+            const int32_t *row = t.table + static_cast<int64_t>(b) * t.pages_per_seq;
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) p[i][u] = j0 + 32 * u < active[i] ? row[j0 + 32 * u] : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+                if (t.in_pool(p[i][u])) atomicOr(m.bits + (p[i][u] >> 5), 1u << (p[i][u] & 31));
     }
     __syncthreads();
 }
@@ -174,20 +184,31 @@ __device__ __forceinline__ Bitmap bitmap_of(const Plan &plan, int n_pages) {
 // ------------------------------------------------------------------------- //
 // With n live pages, the i-th live page from n on goes to the i-th free page below n: as many of the one as of the
 // other, and no page is both a source and a target.
+constexpr int kHoles = 8192;              // targets that are passed on through shared memory; more, through the list of moves
 __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const TableArgs t, const Plan plan, int32_t *n_live) {
     __shared__ int s_warp[32];
+    __shared__ int s_holes[kHoles];
     grid_wait();
     const Bitmap m = bitmap_of(plan, t.n_pages);
     clear(m);
     mark(m, t, [&](int b) { return t.len(b); });
     const int n = rank(m, s_warp);
     const int front = n < t.n_pages ? m.live_before(n) : n;       // live pages that stay
+    const bool small = n - front <= kHoles;
     for (int p = threadIdx.x; p < n; p += kPlanThreads)
-        if (!m.live(p)) plan.moves[p - m.live_before(p)].dst = p;
-    for (int p = n + threadIdx.x; p < t.n_pages; p += kPlanThreads)
-        if (m.live(p)) plan.moves[m.live_before(p) - front].src = p;
+        if (!m.live(p)) {
+            const int i = p - m.live_before(p);
+            if (small) s_holes[i] = p;
+            else plan.moves[i].dst = p;
+        }
     __syncthreads();
-    for (int i = threadIdx.x; i < n - front; i += kPlanThreads) plan.map[plan.moves[i].src] = plan.moves[i].dst;
+    for (int p = n + threadIdx.x; p < t.n_pages; p += kPlanThreads)
+        if (m.live(p)) {
+            const int i = m.live_before(p) - front, to = small ? s_holes[i] : plan.moves[i].dst;
+            plan.moves[i].src = p;
+            plan.moves[i].dst = to;
+            plan.map[p] = to;
+        }
     if (threadIdx.x == 0) {
         *plan.n_moves = n - front;
         *n_live = n;
@@ -408,12 +429,14 @@ int make_table(const int32_t *table, const int32_t *lens, int batch, int pages_p
     return PLX_OK;
 }
 
-// CTAs of an application: what the pages and the entries at most ask for, up to the chip's fill
+// CTAs of an application: what the pages and the entries at most ask for, up to 32 an SM, four times what is resident.
+// (16384 pages of 16 keys, 8 heads of 128, 536 MB read and written: 8 an SM 107.6 us, 16 100.2, 32 97.1 with 4 loads a thread in flight; 98.0 to
+// 101.7 with 8 or 2, 117 with 1 or 16.)
 int apply_grid(const PoolArgs &pool, const TableArgs &t, int64_t moves) {
     const int sms = tma::sm_count();
     const int64_t units = 2 * moves * pieces_of(pool.page_size, pool.chunks_per_key);
     const int64_t entries = (static_cast<int64_t>(t.batch) * t.pages_per_seq + kCopyThreads - 1) / kCopyThreads;
-    const int64_t want = units > entries ? units : entries, most = 8ll * sms;
+    const int64_t want = units > entries ? units : entries, most = 32ll * sms;
     return static_cast<int>(want < most ? want : most);
 }
 

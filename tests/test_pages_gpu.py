@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import parallax_b200 as plx
+from tests.test_sinks_gpu import no_collection
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -175,7 +176,7 @@ def test_captured_calls_follow_the_tables():
         plx.parallax_free_pages(table, lens, rows, 64, 16)
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
+    with no_collection(), torch.cuda.graph(graph):
         forked, flens, missing = plx.parallax_fork_pages(k, v, table, lens, parents, children)
         packed, n_live = plx.parallax_compact_pages(k, v, forked, flens)
         left, free, n_free = plx.parallax_free_pages(packed, flens, rows, 64, 16)
