@@ -149,7 +149,7 @@ def _declare(lib):
     lib.plx_decode_step_sink.restype = C.c_int
     lib.plx_decode_step_sink.argtypes = [decode, i32] + [vp] * 9 + [vp, sz, vp]
     lib.plx_decode_prefix_splits.restype = C.c_int
-    lib.plx_decode_prefix_splits.argtypes = [i32, i32, i32, i32, i32]
+    lib.plx_decode_prefix_splits.argtypes = [i32, i32, i32, i32, i32, i32]
     lib.plx_decode_prefix_workspace_bytes.restype = C.c_int
     lib.plx_decode_prefix_workspace_bytes.argtypes = [decode, prefix, C.POINTER(sz)]
     lib.plx_decode_prefix.restype = C.c_int

@@ -163,6 +163,7 @@ struct Sweep {
     int min_len = 1;           // shorter lengths count as it
     int part_stride = 1;       // records between those of two (batch, head)
     int let_next_in = 0;       // the next launch may begin under this one
+    const plx_prefix *prefix = nullptr;   // keys in tensors of their own that every row begins with
 };
 
 static int run_decode(const plx_decode_problem *p, const void *q, const void *r, const void *k, const void *v, void *out,
@@ -184,6 +185,11 @@ static int run_decode(const plx_decode_problem *p, const void *q, const void *r,
     a.first_key = sweep.first_key;
     a.min_len = sweep.min_len;
     a.let_next_in = sweep.let_next_in;
+    if (sweep.prefix) {
+        a.k_prefix = sweep.prefix->k; a.v_prefix = sweep.prefix->v;
+        a.prefix_len = sweep.prefix->len;
+        a.prefix_st = sweep.prefix->stride_t; a.prefix_sh = sweep.prefix->stride_h;
+    }
     a.seqused = seqused_k;
     a.cache_start = cache_start;
     const size_t bh = static_cast<size_t>(p->batch) * p->heads_q;
@@ -230,11 +236,13 @@ static int run_decode(const plx_decode_problem *p, const void *q, const void *r,
 }
 
 static size_t prefix_part_bytes(const plx_decode_problem *p, const plx_prefix *x) {
+    if (x->n_splits == 0) return 0;
     return static_cast<size_t>(p->batch) * p->heads_q * (x->n_splits + 1) * PLX_DECODE_PART_FLOATS(p->head_dim) * sizeof(float);
 }
 
 static int check_prefix(const plx_decode_problem *p, const plx_prefix *x) {
-    if (!x || x->len <= 0 || x->n_splits < 1 || x->n_splits > PLX_PREFIX_MAX_SPLITS || p->window_left >= 0 || p->kv_offset != 0) return PLX_ERR_BAD_ARG;
+    if (!x || x->len <= 0 || x->n_splits < 0 || x->n_splits > PLX_PREFIX_MAX_SPLITS || p->window_left >= 0 || p->kv_offset != 0) return PLX_ERR_BAD_ARG;
+    if (x->n_splits > (static_cast<int64_t>(x->len) + 63) / 64) return PLX_ERR_BAD_ARG;      // a part holds a tile of 64 keys at least
     if (!x->k)        // in the pages of the cache
         return p->page_table && p->n_pages > 0 && !x->v && x->len % p->page_size == 0 && x->len <= p->cache_len ? PLX_OK : PLX_ERR_BAD_ARG;
     if (!x->v || misaligned16(x->k) || misaligned16(x->v)) return PLX_ERR_BAD_ARG;
@@ -572,26 +580,38 @@ int plx_decode_sink(const plx_decode_problem *p, int32_t sink_tokens, const void
                       nullptr, Sweep{sink_tokens});
 }
 
-int plx_decode_prefix_splits(int32_t batch, int32_t heads_q, int32_t heads_kv, int32_t len, int32_t sm_count) {
-    if (batch <= 0 || heads_kv <= 0 || heads_q % heads_kv != 0 || len <= 0 || sm_count <= 0) return 1;
-    // An item costs its key tiles and about four more for its start and its end; every SM takes the same number of items.
-    const int64_t units = static_cast<int64_t>(prefix_row_tiles(heads_q / heads_kv, batch)) * heads_kv, tiles = (len + 63) / 64;
+int plx_decode_prefix_splits(int32_t batch, int32_t heads_q, int32_t heads_kv, int32_t len, int32_t head_dim, int32_t sm_count) {
+    if (batch <= 0 || heads_kv <= 0 || heads_q % heads_kv != 0 || len <= 0 || head_dim <= 0 || sm_count <= 0) return 1;
+    // Shared: an item costs its tiles of 64 keys and about four more for its start and its end, the SMs take items in rounds, and
+    // the merge goes through 16 records at a time.
+    const int64_t units = static_cast<int64_t>(prefix_row_tiles(heads_q / heads_kv, batch)) * heads_kv, tiles = (static_cast<int64_t>(len) + 63) / 64;
     int best = 1;
-    int64_t best_cost = INT64_MAX;
+    int64_t best_cost = INT64_MAX, best_tiles = 0;
     for (int n = 1; n <= PLX_PREFIX_MAX_SPLITS && n <= tiles; ++n) {
-        const int64_t cost = ((units * n + sm_count - 1) / sm_count) * ((tiles + n - 1) / n + 4);
+        const int64_t rounds = (units * n + sm_count - 1) / sm_count, per_sm = rounds * ((tiles + n - 1) / n), cost = 16 * (per_sm + 4 * rounds) + n;
         if (cost < best_cost) {
             best_cost = cost;
+            best_tiles = per_sm;
             best = n;
         }
     }
-    return best;
+    // Against every row sweeping the prefix, which is one launch instead of three.  Measured at head_dim 128, device time of the whole
+    // call with 40 own keys, us, shared / every row: 8 : 8 heads, 4 rows, 500 keys 10.2 / 6.7, 2000 12.8 / 10.8, 4000 16.3 / 16.6, 16000 33.4 / 65.9; 8 rows,
+    // 500 10.2 / 8.5, 1000 11.2 / 15.6; 16 rows, 500 10.6 / 13.3; 32 : 8 heads, 2 rows, 4000 16.3 / 13.5, 16000 38.2 / 26.9; 4 rows, 4000 16.6 / 16.6; 16 rows, 1000
+    // 12.9 / 15.5, 4000 18.0 / 37.7; 8 : 1 heads, 8 rows, 16000 25.7 / 19.4, 16 rows 21.8 / 28.4.  In units of 10 ns: shared 10 us and 1.65 for a tile
+    // of the SM that has most; every row 4.5 us (64 (row, head) pairs at most, see plx_decode_choose_splits) or 9, and its bytes at 4.4 TB/s with one q
+    // head per kv head, 7 with grouped ones.
+    const int64_t kb = 4ll * batch * len * heads_kv * head_dim / 1000;
+    const bool grouped = heads_q > heads_kv;
+    const int64_t shared = 1000 + 165 * best_tiles, every_row = (!grouped && static_cast<int64_t>(batch) * heads_q <= PLX_DECODE_SPLIT_GROUP_MAX_BH ? 450 : 900) +
+                                                               kb / (grouped ? 70 : 44);
+    return every_row < shared ? 0 : best;
 }
 
 int plx_decode_prefix_workspace_bytes(const plx_decode_problem *p, const plx_prefix *x, size_t *bytes) {
     int st = check_decode(p);
     if (st != PLX_OK) return st;
-    if (!x || !bytes || x->n_splits < 1 || x->n_splits > PLX_PREFIX_MAX_SPLITS) return PLX_ERR_BAD_ARG;
+    if (!x || !bytes || x->n_splits < 0 || x->n_splits > PLX_PREFIX_MAX_SPLITS) return PLX_ERR_BAD_ARG;
     *bytes = prefix_part_bytes(p, x) + decode_ws_bytes(p);
     return PLX_OK;
 }
@@ -627,34 +647,25 @@ int plx_decode_prefix(const plx_decode_problem *p, const plx_prefix *x, const vo
         while ((1 << a.page_shift) < p->page_size) ++a.page_shift;
     }
     a.parts = parts;
-    const bool tensor_cores = train_extend_sm100_supported(a, p->head_dim);
-    // pages that the tensor-core kernel does not take: the prefix is swept with the rest of each row
-    if (!tensor_cores && in_cache) return run_decode(p, q, r, k, v, out, nullptr, seqused_k, nullptr, rest, rest_bytes, cs);
-    const int n_parts = tensor_cores ? x->n_splits + 1 : 2;
-    // Each row's own keys first: the items of the prefix, all alike, are handed out to the SMs as the sweep leaves them.
     Sweep own;
-    own.first_key = own.min_len = in_cache ? x->len : 0;
+    own.first_key = own.min_len = 0;
+    if (x->n_splits == 0 || !train_extend_sm100_supported(a, p->head_dim)) {
+        // every row sweeps the prefix in front of its own keys, in one launch
+        if (in_cache) own.min_len = x->len;
+        else own.prefix = x;
+        return run_decode(p, q, r, k, v, out, nullptr, seqused_k, nullptr, rest, rest_bytes, cs, nullptr, nullptr, own);
+    }
+    // Each row's own keys first: the items of the prefix, all alike, are handed out to the SMs as the sweep leaves them.
+    const int n_parts = x->n_splits + 1;
+    if (in_cache) own.first_key = own.min_len = x->len;
     own.part_stride = n_parts;
-    own.let_next_in = tensor_cores;
+    own.let_next_in = 1;
     st = run_decode(p, q, r, k, v, nullptr, parts + static_cast<size_t>(n_parts - 1) * PLX_DECODE_PART_FLOATS(p->head_dim), seqused_k, nullptr, rest, rest_bytes,
                     cs, nullptr, nullptr, own);
     if (st != PLX_OK) return st;
-    if (tensor_cores) {
-        a.n_splits = x->n_splits;
-        a.n_parts = n_parts;
-        st = launch_prefix_sm100(a, p->dtype, p->head_dim, cs);
-    } else {
-        // a scale or strides that it does not take either: every row sweeps the prefix
-        plx_decode_problem prefix = *p;
-        prefix.page_table = nullptr;
-        prefix.cache_len = x->len;
-        prefix.kv_offset = prefix.total_len = 0;
-        prefix.kv_stride_b = 0; prefix.kv_stride_t = x->stride_t; prefix.kv_stride_h = x->stride_h;
-        Sweep s;
-        s.part_stride = n_parts;
-        st = run_decode(&prefix, q, r, x->k, x->v, nullptr, parts, nullptr, nullptr, rest, rest_bytes, cs, nullptr, nullptr, s);
-    }
-    if (st != PLX_OK) return st;
+    a.n_splits = x->n_splits;
+    a.n_parts = n_parts;
+    if ((st = launch_prefix_sm100(a, p->dtype, p->head_dim, cs)) != PLX_OK) return st;
     return launch_prefix_merge(parts, n_parts, static_cast<int64_t>(p->batch) * p->heads_q, p->head_dim, p->dtype, out, cs);
 }
 

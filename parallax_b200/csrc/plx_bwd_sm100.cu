@@ -984,6 +984,7 @@ bwd_sm100_kernel(const TrainArgs a, int n_tok, const __grid_constant__ CUtensorM
 constexpr int kJoinThreads = 256;
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const TrainArgs a) {
+    grid_wait();           // for dq/dr, which waits for dk/dv at its end
     Seq s;
     int chunk;
     const int m0 = blockIdx.y * kBM;
@@ -1018,9 +1019,18 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const TrainArgs a) {
 // ------------------------------------------------------------------------- //
 template <typename T, int D>
 int launch_join(const TrainArgs &a, cudaStream_t stream) {
-    join_kernel<T, D><<<dim3(a.sink_slots, (a.sink + kBM - 1) / kBM, a.batch * a.heads_kv), kJoinThreads, 0, stream>>>(a);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.sink_slots, (a.sink + kBM - 1) / kBM, a.batch * a.heads_kv);
+    cfg.blockDim = dim3(kJoinThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t st = cudaLaunchKernelEx(&cfg, join_kernel<T, D>, a);
     count_launch();
-    return cudaGetLastError() == cudaSuccess ? PLX_OK : PLX_ERR_LAUNCH;
+    return st == cudaSuccess && cudaGetLastError() == cudaSuccess ? PLX_OK : PLX_ERR_LAUNCH;
 }
 
 template <typename T, int D, int MODE, bool SHORT, bool SINK>

@@ -277,32 +277,43 @@ __device__ __forceinline__ void row_range(const DecodeArgs &a, int b, int &lo, i
     hi = min(max(hi_g - a.kv_offset, 0), a.cache_len);
 }
 
-// Sinks: the first a.sink keys of a row, from its first valid one on, stay visible behind the window.  A row is swept as ONE
-// range of virtual keys: the sinks are moved up to right in front of the window, and keys below `border` lie `gap` further
-// down in the cache.  With ALIGN = 16 sinks and window each start on a multiple of 16, so that a tile of 16 keys has keys of one kind
-// (and lies in one page); what is then in between, [sink_end, border) and [border, window_lo), is not visible.
-struct SinkMap {
-    int border, gap, sink_end, window_lo;
+// FRONT: what a row sweeps in front of its own keys.  kSinks: the first a.sink ones, from its first valid one on, which stay
+// visible behind the window.  kShared: a prefix in tensors of its own.  Either way a row is swept as ONE range of virtual keys: those
+// below `border` are the ones in front, moved up to right before the others.  With ALIGN = 16 both kinds start on a multiple of 16,
+// so that a tile of 16 keys has keys of one kind (and lies in one page); what is then in between, [front_end, border) and
+// [border, own_lo), is not visible.  Where a key lies in its tensors: kSinks: `gap` further down in the cache if it is one in
+// front; kShared: at its own number, or `gap` further down in the cache if it is not.
+constexpr int kNone = 0, kSinks = 1, kShared = 2;
+struct Front {
+    int border, gap, front_end, own_lo;
 };
-template <int ALIGN>
-__device__ __forceinline__ SinkMap sink_range(const DecodeArgs &a, int b, int &lo, int &hi) {
+template <int FRONT, int ALIGN>
+__device__ __forceinline__ Front front_range(const DecodeArgs &a, int b, int &lo, int &hi) {
     row_range(a, b, lo, hi);
+    Front m{INT_MIN, 0, INT_MIN, lo};
+    if (FRONT == kShared) {
+        m.border = m.gap = (a.prefix_len + ALIGN - 1) / ALIGN * ALIGN;
+        m.front_end = a.prefix_len;
+        m.own_lo = m.border + lo;
+        lo = 0;
+        hi += m.border;
+        return m;
+    }
     const int start = min(a.cache_start ? max(a.cache_start[b], 0) : a.first_key, lo), n = min(a.sink, lo - start);
-    SinkMap m{INT_MIN, 0, INT_MIN, lo};
     if (n == lo - start) {           // nothing is hidden
-        lo = m.window_lo = start;
+        lo = m.own_lo = start;
         return m;
     }
     m.border = lo / ALIGN * ALIGN;
     lo = m.border - (n + ALIGN - 1) / ALIGN * ALIGN;
     m.gap = lo - start;
-    m.sink_end = lo + n;
+    m.front_end = lo + n;
     return m;
 }
 // the range that is cut into parts
-template <int G, bool SINK>
+template <int G, int FRONT>
 __device__ __forceinline__ void sweep_range(const DecodeArgs &a, int b, int &lo, int &hi) {
-    if constexpr (SINK) sink_range<G == 16 ? 16 : 1>(a, b, lo, hi);
+    if constexpr (FRONT != kNone) front_range<FRONT, G == 16 ? 16 : 1>(a, b, lo, hi);
     else row_range(a, b, lo, hi);
 }
 
@@ -321,10 +332,10 @@ __device__ __forceinline__ SplitPlan even_part(const DecodeArgs &a, int b, int p
     const int my_lo = min(lo + part * chunk, hi);
     return SplitPlan{b, part, a.n_splits, my_lo, min(my_lo + chunk, hi), static_cast<int64_t>(b) * a.n_splits * a.heads_q};
 }
-template <int G, bool SINK>
+template <int G, int FRONT>
 __device__ __forceinline__ SplitPlan plan_even(const DecodeArgs &a, int b, int part) {
     int lo, hi;
-    sweep_range<G, SINK>(a, b, lo, hi);
+    sweep_range<G, FRONT>(a, b, lo, hi);
     return even_part<G>(a, b, part, lo, hi);
 }
 
@@ -335,7 +346,7 @@ __device__ __forceinline__ SplitPlan plan_even(const DecodeArgs &a, int b, int p
 // ..: up to kBalancedRows rows.  `cap`: the most parts of a row that the merge takes.
 // Not so where the longest row is within a.balanced sixteenths of the mean (see balance_from): dealing out costs the
 // search and leaves parts and rows that no longer fall together with CTAs.
-template <int G, bool SINK>
+template <int G, int FRONT>
 __device__ __forceinline__ SplitPlan plan_slot(const DecodeArgs &a, int slot, int lane, int cap) {
     SplitPlan p{-1, 0, 1, 0, 0, 0};
     constexpr int kRows = kBalancedRows / 32;
@@ -345,7 +356,7 @@ __device__ __forceinline__ SplitPlan plan_slot(const DecodeArgs &a, int slot, in
         start[i] = n[i] = units[i] = 0;
         if (lane + 32 * i < a.batch) {
             int hi;
-            sweep_range<G, SINK>(a, lane + 32 * i, start[i], hi);
+            sweep_range<G, FRONT>(a, lane + 32 * i, start[i], hi);
             n[i] = max(hi - start[i], 0);
             units[i] = (n[i] + G - 1) / G;
         }
@@ -445,8 +456,8 @@ static cudaError_t launch_overlapped(void (*kern)(Params...), dim3 grid, int thr
 // DEAL: the slots may be dealt out by length (a.balanced > 0).  A kernel of its own: with the plan of either kind in one,
 // launches without lengths were 0.3 to 0.6 us longer (32 rows of 300 down to 100 keys, 8 : 8 heads, 12.4 -> 13.0).
 //
-// SINK: a kernel of its own too, with the keys of a.sink in front of the window's (see SinkMap).
-template <typename T, int D, int HG, int U, bool SG, bool DEAL, bool SINK = false>
+// FRONT: kernels of their own too.
+template <typename T, int D, int HG, int U, bool SG, bool DEAL, int FRONT = kNone>
 __global__ void __launch_bounds__(HG * 32, U > 4 ? 1 : 512 / (HG * 32)) decode_kernel(const DecodeArgs a) {
     grid_wait();
     if (a.let_next_in) launch_dependents();
@@ -462,12 +473,12 @@ __global__ void __launch_bounds__(HG * 32, U > 4 ? 1 : 512 / (HG * 32)) decode_k
     // the part of a batch row's keys that this warp sweeps
     SplitPlan plan;
     if constexpr (!DEAL) {
-        plan = plan_even<NS, SINK>(a, blockIdx.z, SG ? blockIdx.x * HG + warp : blockIdx.x);
+        plan = plan_even<NS, FRONT>(a, blockIdx.z, SG ? blockIdx.x * HG + warp : blockIdx.x);
     } else {
         // the warps of a CTA have one slot: one of them plans (all eight, they queued for the divisions)
         __shared__ SplitPlan s_plan;
         if (warp == 0) {
-            plan = plan_slot<NS, SINK>(a, blockIdx.z * a.n_splits + blockIdx.x, lane, a.n_groups ? 32 * a.n_groups : 32);
+            plan = plan_slot<NS, FRONT>(a, blockIdx.z * a.n_splits + blockIdx.x, lane, a.n_groups ? 32 * a.n_groups : 32);
             if (lane == 0) s_plan = plan;
         }
         __syncthreads();
@@ -476,10 +487,10 @@ __global__ void __launch_bounds__(HG * 32, U > 4 ? 1 : 512 / (HG * 32)) decode_k
     }
     const int b = plan.b, my_lo = plan.lo, my_hi = plan.hi;
     const int n_iter = (my_hi - my_lo + NS * U - 1) / (NS * U);
-    SinkMap sinks{INT_MIN, 0, 0, 0};
-    if constexpr (SINK) {
+    Front front{INT_MIN, 0, 0, 0};
+    if constexpr (FRONT != kNone) {
         int lo, hi;
-        sinks = sink_range<1>(a, b, lo, hi);
+        front = front_range<FRONT, 1>(a, b, lo, hi);
     }
 
     // this lane's 8 channels of q and r
@@ -499,6 +510,8 @@ __global__ void __launch_bounds__(HG * 32, U > 4 ? 1 : 512 / (HG * 32)) decode_k
     const int64_t row0 = (paged ? 0 : b * a.kv_sb) + hq * a.kv_sh + sl * 8;
     const T *kp = static_cast<const T *>(a.k) + row0;
     const T *vp = static_cast<const T *>(a.v) + row0;
+    const T *kp0 = FRONT == kShared ? static_cast<const T *>(a.k_prefix) + hq * a.prefix_sh + sl * 8 : nullptr;
+    const T *vp0 = FRONT == kShared ? static_cast<const T *>(a.v_prefix) + hq * a.prefix_sh + sl * 8 : nullptr;
 
     float m = -INFINITY, d1 = 0.f, d2 = 0.f, o1[8], o2[8];
 #pragma unroll
@@ -513,7 +526,14 @@ __global__ void __launch_bounds__(HG * 32, U > 4 ? 1 : 512 / (HG * 32)) decode_k
         for (int u = 0; u < U; ++u) {
             int kj = base + u * NS;
             if (kj < my_hi) {
-                if (SINK && kj < sinks.border) kj -= sinks.gap;
+                if (FRONT == kShared) {
+                    const bool shared = kj < front.border;
+                    const int64_t at = shared ? static_cast<int64_t>(kj) * a.prefix_st : static_cast<int64_t>(kj - front.gap) * a.kv_st;
+                    kr[u] = ld_stream16((shared ? kp0 : kp) + at);
+                    vr[u] = ld_stream16((shared ? vp0 : vp) + at);
+                    continue;
+                }
+                if (FRONT == kSinks && kj < front.border) kj -= front.gap;
                 const int64_t at = decltype(paged_tag)::value ? paged_key_offset(a, b, kj) : static_cast<int64_t>(kj) * a.kv_st;
                 const T *pk = kp + at, *pv = vp + at;
                 kr[u] = ld_stream16(pk);
@@ -995,8 +1015,8 @@ struct GqaSmem {
 // head_dim 128, where the other form fills 255); a movmatrix per 8 x 8 block turns P^T around.
 // B = 16, 1024 keys, 32 : 8 heads 16.7 -> 16.0 us, B = 8, 4000 keys, rows of different lengths 40.8 -> 34.0.
 //
-// SINK: see SinkMap; a tile holds sinks or keys of the window, and rows of it that are not visible are zeroed and masked.
-template <typename T, int D, bool PAGED, bool FEW, bool SINK = false>
+// FRONT: a tile holds keys of one kind, and rows of it that are not visible are zeroed and masked.
+template <typename T, int D, bool PAGED, bool FEW, int FRONT = kNone>
 __global__ void __launch_bounds__(kGqaWarps * 32, 1) decode_gqa_kernel(const DecodeArgs a, int n_hgroups) {
     grid_wait();
     if (a.let_next_in) launch_dependents();
@@ -1016,7 +1036,7 @@ __global__ void __launch_bounds__(kGqaWarps * 32, 1) decode_gqa_kernel(const Dec
     const int hunit = blockIdx.x % n_hunits, cta = blockIdx.x / n_hunits, slot = cta * kGqaWarps + warp;
     const int hk = hunit / n_hgroups, hgrp = hunit % n_hgroups;
     SplitPlan plan{-1, 0, 0, 0, 0, 0};
-    if (slot < n_slots) plan = a.balanced ? plan_slot<kGqaTile, SINK>(a, slot, lane, n_slots) : plan_even<kGqaTile, SINK>(a, slot / a.n_splits, slot % a.n_splits);
+    if (slot < n_slots) plan = a.balanced ? plan_slot<kGqaTile, FRONT>(a, slot, lane, n_slots) : plan_even<kGqaTile, FRONT>(a, slot / a.n_splits, slot % a.n_splits);
     const int b = max(plan.b, 0), my_lo = plan.lo, my_hi = plan.b < 0 ? plan.lo : plan.hi;
     const int n_tiles = (my_hi - my_lo + kGqaTile - 1) / kGqaTile;
     const int hq0 = hk * a.n_rep + hgrp * 16;       // first q head of this CTA's rows
@@ -1025,15 +1045,16 @@ __global__ void __launch_bounds__(kGqaWarps * 32, 1) decode_gqa_kernel(const Dec
     auto sK = [&](int st) -> uint32_t { return sbase + st * 2 * kTileBytes; };
     auto sV = [&](int st) -> uint32_t { return sbase + st * 2 * kTileBytes + kTileBytes; };
     if (lane == 0) s_row[warp] = plan.b;
-    SinkMap sinks{INT_MIN, 0, 0, 0};
-    if constexpr (SINK) {
+    constexpr bool kFront = FRONT != kNone;
+    Front front{INT_MIN, 0, 0, 0};
+    if constexpr (kFront) {
         int lo, hi;
-        sinks = sink_range<kGqaTile>(a, b, lo, hi);
+        front = front_range<FRONT, kGqaTile>(a, b, lo, hi);
     }
     // visible keys of a tile
-    auto first_of = [&](int tile0) { return SINK && tile0 >= sinks.border ? sinks.window_lo : INT_MIN; };
-    auto end_of = [&](int tile0) { return SINK && tile0 < sinks.border ? min(my_hi, sinks.sink_end) : my_hi; };
-    auto visible = [&](int key, int first, int end) { return key < end && (!SINK || key >= first); };
+    auto first_of = [&](int tile0) { return kFront && tile0 >= front.border ? front.own_lo : INT_MIN; };
+    auto end_of = [&](int tile0) { return kFront && tile0 < front.border ? min(my_hi, front.front_end) : my_hi; };
+    auto visible = [&](int key, int first, int end) { return key < end && (!kFront || key >= first); };
 
     // Tile i of this warp -> stage i % kGqaStages.  A lane copies the same 16-byte column of every
     // (32 / CPR)-th row, so its source and destination advance by constants; rows past my_hi (last tile
@@ -1042,15 +1063,17 @@ __global__ void __launch_bounds__(kGqaWarps * 32, 1) decode_gqa_kernel(const Dec
     // read ahead.
     constexpr int RPI = 32 / CPR;                                  // rows covered by one instruction of the warp
     const int my_row = lane / CPR, my_col = lane % CPR;
-    const bool page_per_tile = PAGED && a.page_mask + 1 >= kGqaTile && my_lo % kGqaTile == 0 && (!SINK || sinks.gap % kGqaTile == 0);
-    const T *kp = static_cast<const T *>(a.k) + (PAGED ? 0 : b * a.kv_sb) + hk * a.kv_sh + my_col * 8;
-    const T *vp = static_cast<const T *>(a.v) + (PAGED ? 0 : b * a.kv_sb) + hk * a.kv_sh + my_col * 8;
+    const bool page_per_tile = PAGED && a.page_mask + 1 >= kGqaTile && my_lo % kGqaTile == 0 && (!kFront || front.gap % kGqaTile == 0);
+    const T *kp_own = static_cast<const T *>(a.k) + (PAGED ? 0 : b * a.kv_sb) + hk * a.kv_sh + my_col * 8;
+    const T *vp_own = static_cast<const T *>(a.v) + (PAGED ? 0 : b * a.kv_sb) + hk * a.kv_sh + my_col * 8;
+    const T *kp_front = FRONT == kShared ? static_cast<const T *>(a.k_prefix) + hk * a.prefix_sh + my_col * 8 : nullptr;
+    const T *vp_front = FRONT == kShared ? static_cast<const T *>(a.v_prefix) + hk * a.prefix_sh + my_col * 8 : nullptr;
     const uint32_t my_dst = (my_row * LD + my_col * 8) * 2;
     // Pages of the next tiles to be loaded: as many as there are stages, so that no load waits for the page number of another;
     // two where registers are short (B = 64, 4096 keys, 16 : 1 heads, pages, 34.0 us, three 35.8).
     constexpr int kPages = FEW ? kGqaStages : 2;
     uint32_t next_page[kPages];
-    auto in_cache = [&](int key, int tile0) { return SINK && tile0 < sinks.border ? key - sinks.gap : key; };
+    auto in_cache = [&](int key, int tile0) { return kFront && (tile0 < front.border) == (FRONT == kSinks) ? key - front.gap : key; };
     auto page_of_tile = [&](int i) -> uint32_t {
         const int tile0 = my_lo + i * kGqaTile;
         return page_per_tile && i < n_tiles ? paged_key_page(a, b, in_cache(tile0, tile0)) : 0u;
@@ -1062,12 +1085,15 @@ __global__ void __launch_bounds__(kGqaWarps * 32, 1) decode_gqa_kernel(const Dec
         if (i < n_tiles) {
             const int st = i % kGqaStages, tile0 = my_lo + i * kGqaTile, key0 = tile0 + my_row, first = first_of(tile0), end = end_of(tile0);
             const uint32_t dk = sK(st) + my_dst, dv = sV(st) + my_dst;
-            const bool whole = tile0 + kGqaTile <= end && (!SINK || tile0 >= first);
+            const bool whole = tile0 + kGqaTile <= end && (!kFront || tile0 >= first);
             const int at0 = in_cache(key0, tile0);           // of the lane's first key
+            const bool shared = FRONT == kShared && tile0 < front.border;
+            const T *const kp = shared ? kp_front : kp_own, *const vp = shared ? vp_front : vp_own;
+            const int64_t kv_st = shared ? a.prefix_st : a.kv_st;
             if (!PAGED || page_per_tile) {
-                const int64_t step = static_cast<int64_t>(RPI) * a.kv_st;
+                const int64_t step = static_cast<int64_t>(RPI) * kv_st;
                 const int64_t at = page_per_tile ? static_cast<int64_t>(next_page[0]) * a.kv_sb + static_cast<int64_t>(at0 & a.page_mask) * a.kv_st
-                                                 : static_cast<int64_t>(at0) * a.kv_st;
+                                                 : static_cast<int64_t>(at0) * kv_st;
                 if (PAGED) {
 #pragma unroll
                     for (int n = 1; n < kPages; ++n) next_page[n - 1] = next_page[n];
@@ -1440,11 +1466,11 @@ __global__ void __launch_bounds__(kGqaWarps * 32, 1) decode_gqa_kernel(const Dec
     if (warp == w0 && lane == 0) a.ws_counters[bh_of(0)] = 0;   // ready for the next launch on this workspace
 }
 
-template <typename T, int D, bool PAGED, bool FEW, bool SINK>
+template <typename T, int D, bool PAGED, bool FEW, int FRONT>
 static int launch_decode_gqa(const DecodeArgs &a, cudaStream_t stream) {
     const int n_hgroups = (a.n_rep + 15) / 16;
     constexpr int kSmem = kGqaWarps * GqaSmem<D>::kPerWarp;
-    auto kern = decode_gqa_kernel<T, D, PAGED, FEW, SINK>;
+    auto kern = decode_gqa_kernel<T, D, PAGED, FEW, FRONT>;
     {   // the shared-memory opt-in is a per-device function attribute: set it once per device
         constexpr int kMaxDevices = 64;
         static std::mutex mu;
@@ -1471,9 +1497,10 @@ static int launch_decode_hg(const DecodeArgs &a, cudaStream_t stream) {
     constexpr int U = 4;  // key rows per stream and register buffer (two buffers: 8 rows of K and of V in flight)
     dim3 grid(a.n_splits, a.heads_q / HG, a.batch);
     // (with sinks the rows are as long as the window, most of them: never dealt out by length)
-    auto kern = a.sink       ? decode_kernel<T, D, HG, U, false, false, true>
-                : a.balanced ? decode_kernel<T, D, HG, U, false, true>
-                             : decode_kernel<T, D, HG, U, false, false>;
+    auto kern = a.sink         ? decode_kernel<T, D, HG, U, false, false, kSinks>
+                : a.prefix_len ? decode_kernel<T, D, HG, U, false, false, kShared>
+                : a.balanced   ? decode_kernel<T, D, HG, U, false, true>
+                               : decode_kernel<T, D, HG, U, false, false>;
     const cudaError_t st = launch_overlapped(kern, grid, HG * 32, 0, stream, a);
     count_launch();
     return st == cudaSuccess && cudaGetLastError() == cudaSuccess ? PLX_OK : PLX_ERR_LAUNCH;
@@ -1548,26 +1575,31 @@ static int launch_decode_sg(const DecodeArgs &a, cudaStream_t stream) {
         }
         roomy = roomy && units <= n;
     }
-    auto kern = a.sink  ? (roomy ? decode_kernel<T, D, 8, 8, true, false, true> : decode_kernel<T, D, 8, 4, true, false, true>)
-                : roomy ? decode_kernel<T, D, 8, 8, true, false>
-                        : decode_kernel<T, D, 8, 4, true, false>;
+    auto kern = a.sink         ? (roomy ? decode_kernel<T, D, 8, 8, true, false, kSinks> : decode_kernel<T, D, 8, 4, true, false, kSinks>)
+                : a.prefix_len ? (roomy ? decode_kernel<T, D, 8, 8, true, false, kShared> : decode_kernel<T, D, 8, 4, true, false, kShared>)
+                : roomy        ? decode_kernel<T, D, 8, 8, true, false>
+                               : decode_kernel<T, D, 8, 4, true, false>;
     cfg.numAttrs = cluster ? 2 : 1;
     cudaError_t st = cudaLaunchKernelEx(&cfg, kern, a);
     count_launch();
     return st == cudaSuccess && cudaGetLastError() == cudaSuccess ? PLX_OK : PLX_ERR_LAUNCH;
 }
 
-template <typename T, int D, bool SINK>
+template <typename T, int D, int FRONT>
 static int launch_decode_grouped(const DecodeArgs &a, cudaStream_t stream) {
-    if (a.n_rep > 8)
-        return a.page_table ? launch_decode_gqa<T, D, true, false, SINK>(a, stream) : launch_decode_gqa<T, D, false, false, SINK>(a, stream);
-    return a.page_table ? launch_decode_gqa<T, D, true, true, SINK>(a, stream) : launch_decode_gqa<T, D, false, true, SINK>(a, stream);
+    if constexpr (FRONT != kShared) {       // (a shared prefix in pages is part of the rows' tables)
+        if (a.page_table)
+            return a.n_rep > 8 ? launch_decode_gqa<T, D, true, false, FRONT>(a, stream) : launch_decode_gqa<T, D, true, true, FRONT>(a, stream);
+    }
+    return a.n_rep > 8 ? launch_decode_gqa<T, D, false, false, FRONT>(a, stream) : launch_decode_gqa<T, D, false, true, FRONT>(a, stream);
 }
 
 template <typename T, int D>
 static int launch_decode_t(const DecodeArgs &a, cudaStream_t stream) {
     if (a.n_rep >= 2)    // grouped heads: tensor-core kernel
-        return a.sink ? launch_decode_grouped<T, D, true>(a, stream) : launch_decode_grouped<T, D, false>(a, stream);
+        return a.sink         ? launch_decode_grouped<T, D, kSinks>(a, stream)
+               : a.prefix_len ? launch_decode_grouped<T, D, kShared>(a, stream)
+                              : launch_decode_grouped<T, D, kNone>(a, stream);
     if (decode_split_groups(a)) return launch_decode_sg<T, D>(a, stream);
     // adjacent q heads share a CTA (one warp each): the largest group that divides the head count
     if (a.heads_q % 8 == 0) return launch_decode_hg<T, D, 8>(a, stream);
@@ -1602,7 +1634,7 @@ static int balance_from(const DecodeArgs &a, int head_dim) {
         const bool rows_end_with_ctas = a.n_splits % kGqaWarps == 0 || kGqaWarps % a.n_splits == 0;
         return part < 384 * 128 && rows_end_with_ctas ? 32 : 17;
     }
-    if (part < 64 * 128 || a.sink) return 0;
+    if (part < 64 * 128 || a.sink || a.prefix_len) return 0;
     const bool one_wave = static_cast<int64_t>(a.batch) * a.heads_q * a.n_splits <= 16 * static_cast<int64_t>(tma_free_sm_count());
     return part < 100 * 128 || a.n_splits < 4 || !one_wave ? 32 : 17;
 }
@@ -1672,8 +1704,8 @@ int launch_decode_merge(const float *parts, int n_parts, int n_records, int head
 }
 
 // ========================================================================= //
-// A batch behind a shared prefix: the states of the prefix's splits and of the row's own keys, n_parts <= 32 records in a row for
-// each (batch, head), -> out.  One warp each; bound by one round trip to the L2.
+// A batch behind a shared prefix: the states of the prefix's splits and of the row's own keys, n_parts records in a row for
+// each (batch, head), -> out.  One warp each, 32 records at a time, 16 of them in flight; bound by the round trips to the L2.
 // ========================================================================= //
 template <typename T, int D>
 __global__ void __launch_bounds__(128) prefix_merge_kernel(const float *parts, int n_parts, int64_t n_rows, void *out) {
@@ -1683,7 +1715,22 @@ __global__ void __launch_bounds__(128) prefix_merge_kernel(const float *parts, i
     const int lane = threadIdx.x & 31;
     if (row >= n_rows) return;
     float big, D1, D2, O1[CH], O2[CH];
-    warp_merge<D, 8, true>(parts + row * n_parts * REC, n_parts, lane, big, D1, D2, O1, O2);
+    const float *recs = parts + row * n_parts * REC;
+    warp_merge<D, 16, true>(recs, min(n_parts, 32), lane, big, D1, D2, O1, O2);
+    for (int j = 32; j < n_parts; j += 32) {
+        float big2, E1, E2, P1[CH], P2[CH];
+        warp_merge<D, 16, true>(recs + static_cast<int64_t>(j) * REC, min(n_parts - j, 32), lane, big2, E1, E2, P1, P2);
+        const float top = fmaxf(big, big2), safe = top == -INFINITY ? 0.f : top;
+        const float wa = fast_exp2(big - safe), wb = fast_exp2(big2 - safe);
+        big = top;
+        D1 = wa * D1 + wb * E1;
+        D2 = wa * D2 + wb * E2;
+#pragma unroll
+        for (int e = 0; e < CH; ++e) {
+            O1[e] = wa * O1[e] + wb * P1[e];
+            O2[e] = wa * O2[e] + wb * P2[e];
+        }
+    }
     T *dst = static_cast<T *>(out) + row * D + lane * CH;
 #pragma unroll
     for (int e = 0; e < CH; e += 2)

@@ -32,6 +32,10 @@ struct DecodeArgs {
     int batch, heads_q, heads_kv, n_rep, cache_len, window, n_splits, kv_offset, total_len;
     int sink;          // keys in front that stay visible behind the window (0 without one)
     int first_key, min_len;   // keys before first_key are another launch's (0); lengths below min_len count as it (1)
+    // keys that all rows begin with, in tensors of their own (prefix_len 0: none), element strides as kv_st, kv_sh
+    const void *k_prefix, *v_prefix;
+    int prefix_len;
+    int64_t prefix_st, prefix_sh;
     int let_next_in;          // the next launch may begin under this one (it waits for its end by itself)
     float c2;  // qk_scale * log2(e)
     int64_t kv_sb, kv_st, kv_sh;   // paged: kv_sb is the stride between pages
@@ -52,7 +56,7 @@ struct DecodeArgs {
     // the most keys that a row sweeps
     int active_keys() const {
         const int64_t n = window >= 0 ? static_cast<int64_t>(window) + sink : cache_len;
-        return static_cast<int>((n < cache_len ? n : cache_len) - (window >= 0 ? 0 : first_key));
+        return static_cast<int>((n < cache_len ? n : cache_len) - (window >= 0 ? 0 : first_key)) + prefix_len;
     }
 };
 

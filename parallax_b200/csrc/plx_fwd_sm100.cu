@@ -760,13 +760,26 @@ fwd_sm100_kernel(const TrainArgs a, const __grid_constant__ CUtensorMap tm_q, co
                         tc_fence_before();
                         mbar_arrive(bar(L::kOFree));
                     }
+                    // 4 x 4 word transposes inside the quad, of even and of odd columns: a thread gets 8 columns in a row, a warp
+                    // store covers 128 contiguous bytes of 8 rows
 #pragma unroll
-                    for (int k = 0; k < 8; ++k)
+                    for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-                        for (int hh = 0; hh < 2; ++hh)
-                            if (rec[hh])
-                                __stcg(reinterpret_cast<float2 *>(rec[hh] + 4 + c + 8 * k + 2 * t),
-                                       make_float2(__uint_as_float(o[4 * k + 2 * hh]), __uint_as_float(o[4 * k + 2 * hh + 1])));
+                        for (int grp = 0; grp < 2; ++grp) {
+                            uint32_t even[4], odd[4];
+#pragma unroll
+                            for (int kk = 0; kk < 4; ++kk) {
+                                even[kk] = o[4 * (4 * grp + kk) + 2 * hh];
+                                odd[kk] = o[4 * (4 * grp + kk) + 2 * hh + 1];
+                            }
+                            quad_transpose(even, t);
+                            quad_transpose(odd, t);
+                            if (rec[hh]) {
+                                uint4 *dst = reinterpret_cast<uint4 *>(rec[hh] + 4 + c + 32 * grp + 8 * t);
+                                __stcg(dst, make_uint4(even[0], odd[0], even[1], odd[1]));
+                                __stcg(dst + 1, make_uint4(even[2], odd[2], even[3], odd[3]));
+                            }
+                        }
                 }
                 ++n_items_done;
                 continue;

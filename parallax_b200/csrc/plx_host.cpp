@@ -604,14 +604,16 @@ py::object decode_prefix(const py::object &q_, const py::object &r_, const py::o
     const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream();
     const int sms = at::cuda::getDeviceProperties(q.get_device())->multiProcessorCount;
     plx_decode_problem p = decode_problem(q, k, ceiling, table, scale, -1, 1);
-    p.n_splits = api.decode_choose_splits_gqa(p.batch, p.heads_q, p.heads_kv, static_cast<int32_t>(std::max<int64_t>(1, ceiling - least)), sms);
     x.len = static_cast<int32_t>(prefix_len);
-    x.n_splits = api.decode_prefix_splits(p.batch, p.heads_q, p.heads_kv, x.len, sms);
+    x.n_splits = api.decode_prefix_splits(p.batch, p.heads_q, p.heads_kv, x.len, p.head_dim, sms);
+    const int64_t n_keys = ceiling - least + (x.n_splits ? 0 : prefix_len);
+    if (n_keys > INT32_MAX) return py::none();
+    p.n_splits = api.decode_choose_splits_gqa(p.batch, p.heads_q, p.heads_kv, static_cast<int32_t>(std::max<int64_t>(1, n_keys)), sms);
     size_t need = 0;
     if (api.decode_prefix_workspace_bytes(&p, &x, &need) != PLX_OK) return py::none();
     const Tensor ws = workspaces().get(stream, q, p.n_splits, static_cast<int64_t>(need / sizeof(float)), x.n_splits);
     Tensor out = at::empty(q.sizes(), q.options());
-    LengthCheck check(lens, stream, true);
+    LengthCheck check(lens, stream, x.n_splits != 0 || decode_lasts(q, k, n_keys));
     if (api.decode_prefix(&p, &x, q.data_ptr(), r.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), int_ptr(lens), ws.data_ptr(), need,
                           stream.stream()) != PLX_OK ||
         !check.within(least, ceiling))

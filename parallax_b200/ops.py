@@ -288,9 +288,10 @@ def _prefix(k_prefix: Optional[Tensor], v_prefix: Optional[Tensor], prefix_len: 
     return x
 
 
-def choose_prefix_splits(batch: int, heads_q: int, heads_kv: int, prefix_len: int, device: torch.device) -> int:
+def choose_prefix_splits(batch: int, heads_q: int, heads_kv: int, prefix_len: int, head_dim: int, device: torch.device) -> int:
+    """Parts of a shared prefix; 0 where it is faster for every row to sweep the prefix itself."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
-    return int(_cabi.lib().plx_decode_prefix_splits(batch, heads_q, heads_kv, prefix_len, sm_count(idx)))
+    return int(_cabi.lib().plx_decode_prefix_splits(batch, heads_q, heads_kv, prefix_len, head_dim, sm_count(idx)))
 
 
 def decode_prefix_workspace_bytes(q: Tensor, k: Tensor, n_splits: int, prefix_splits: int, page_table: Optional[Tensor]) -> int:

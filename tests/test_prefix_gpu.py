@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import parallax_b200 as plx
-from parallax_b200 import _cabi
+from parallax_b200 import _cabi, ops
 from tests.test_sinks_gpu import attend, close, no_collection, randn
 
 pytestmark = pytest.mark.gpu
@@ -65,11 +65,38 @@ def test_dense(case):
     assert _cabi.device_error() == 0
 
 
+@pytest.mark.parametrize("splits", [0, 1, 2, 5, 16, 40, 127])
+@pytest.mark.parametrize("b,hq,hkv,d,dtype,p,t", [
+    (3, 8, 8, 128, BF, 8128, 20), (1, 4, 4, 64, FP, 130, 1), (9, 8, 2, 128, BF, 700, 130), (5, 3, 1, 64, BF, 321, 7), (140, 2, 2, 64, BF, 64, 3),
+    (4, 40, 2, 128, FP, 2600, 60), (2, 260, 2, 64, BF, 1000, 5), (33, 16, 4, 128, BF, 1, 40)])
+def test_every_way_to_split(b, hq, hkv, d, dtype, p, t, splits):
+    """0: every row sweeps the prefix in front of its own keys; else its parts, one for every 64 keys at most."""
+    q, r, kp, vp, k, v = make(b, hq, hkv, d, dtype, p, t)
+    n = [(i * 7) % (t + 1) for i in range(b)]
+    want = reference(q, r, [torch.cat((kp, k[i, :n[i]])) for i in range(b)], [torch.cat((vp, v[i, :n[i]])) for i in range(b)])
+    for i in range(b):
+        k[i, n[i]:] = v[i, n[i]:] = torch.nan
+    out = torch.empty_like(q)
+    for own in (1, 3, 8, 40):
+        if splits > -(-p // 64):
+            with pytest.raises(_cabi.PlxError):
+                ops.decode_prefix(q, r, kp, vp, p, k, v, out, torch.zeros(1 << 24, device="cuda"), d ** -0.5, own, splits, ints(n), None)
+            continue
+        ws = torch.zeros(max(ops.decode_prefix_workspace_bytes(q, k, own, splits, None) // 4, 4), device="cuda")
+        for _ in range(2):                                  # (a workspace is left as it was found)
+            ops.decode_prefix(q, r, kp, vp, p, k, v, out, ws, d ** -0.5, own, splits, ints(n), None)
+            close(out, want, 2, (splits, own))
+    assert _cabi.device_error() == 0
+
+
 @pytest.mark.parametrize("scale", [-0.2, 0.0, 0.4])
 def test_scales(scale):
     q, r, kp, vp, k, v = make(3, 8, 2, 64, BF, 300, 20)
     want = reference(q, r, [torch.cat((kp, k[i])) for i in range(3)], [torch.cat((vp, v[i])) for i in range(3)], scale)
     close(plx.parallax_decode_shared_prefix(q, r, kp, vp, k, v, scale), want, 2, "o")
+    out, ws = torch.empty_like(q), torch.zeros(1 << 20, device="cuda")
+    ops.decode_prefix(q, r, kp, vp, 300, k, v, out, ws, scale, 4, 3, None, None)      # shared where there is a kernel for it
+    close(out, want, 2, "o")
 
 
 def test_layouts():
