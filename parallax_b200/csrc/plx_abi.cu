@@ -87,7 +87,7 @@ static size_t train_ws_bytes(const plx_train_problem *p) {
 static void set_sinks(TrainArgs &a, int32_t sink_tokens) {
     if (sink_tokens <= 0 || a.window < 0 || a.window >= a.len_k) return;
     a.sink = sink_tokens < a.len_k ? sink_tokens : a.len_k;
-    a.sink_chunk = train_sink_chunk(a.window, a.len_q);
+    a.sink_chunk = train_sink_chunk(a.sink, a.window, a.len_q);
     const int64_t longest = a.len_q;          // of a pack: one sequence may hold all tokens
     if (longest > a.sink_chunk) a.sink_slots = static_cast<int>(a.cu ? 2 * longest / a.sink_chunk + 1 : (longest + a.sink_chunk - 1) / a.sink_chunk);
 }

@@ -979,35 +979,48 @@ bwd_sm100_kernel(const TrainArgs a, int n_tok, const __grid_constant__ CUtensorM
     if (DQR) grid_wait();
 }
 
-// dk, dv of the key tiles that were cut into chunks.  CTA (slot, key tile, (batch, kv head)); the CTAs of a sequence's slots share
-// its tile, 8 channels of a key per thread.  Bound by reading the parts: those of the first chunks whole, then the sinks' rows.
-constexpr int kJoinThreads = 256;
+// dk, dv of the key tiles that were cut into chunks.  CTA (a quarter of a slot, key tile, (batch, kv head)); the CTAs of a sequence's
+// slots share its tile, 8 channels of a key per thread.  Bound by the round trips for the parts (those of the first chunks whole,
+// then the sinks' rows), so those of eight chunks are on their way together: L = 8192, 16 heads 10.9 -> 4.9 us.
+constexpr int kJoinThreads = 256, kJoinCtas = 4;
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const TrainArgs a) {
     grid_wait();           // for dq/dr, which waits for dk/dv at its end
     Seq s;
     int chunk;
     const int m0 = blockIdx.y * kBM;
-    if (!locate_chunk(a, blockIdx.x, s, chunk) || m0 >= s.nk) return;
-    const int n_bh = gridDim.z, first = blockIdx.x - chunk, n_chunks = (s.nq + a.sink_chunk - 1) / a.sink_chunk;
+    const int slot = blockIdx.x / kJoinCtas;
+    if (!locate_chunk(a, slot, s, chunk) || m0 >= s.nk) return;
+    const int n_bh = gridDim.z, first = slot - chunk, n_chunks = (s.nq + a.sink_chunk - 1) / a.sink_chunk;
     const int b = blockIdx.z / a.heads_kv, hk = blockIdx.z % a.heads_kv;
     constexpr int kPerRow = D / 8;
-    for (int e = chunk * kJoinThreads + threadIdx.x; e < 2 * kBM * kPerRow; e += n_chunks * kJoinThreads) {
+    const int n_threads = n_chunks * kJoinCtas * kJoinThreads;
+    for (int e = (chunk * kJoinCtas + blockIdx.x % kJoinCtas) * kJoinThreads + threadIdx.x; e < 2 * kBM * kPerRow; e += n_threads) {
         const int which = e / (kBM * kPerRow), row = e / kPerRow % kBM, c = e % kPerRow * 8;
         if (m0 + row >= s.nk) continue;
         float x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = 0.f;
-#pragma unroll 4
-        for (int j = 0; j < n_chunks; ++j) {
-            int t_lo, n_t;
-            chunk_rows(a, s, m0, j, t_lo, n_t);
-            if (n_t == 0 || row >= chunk_keys(a, s, m0, t_lo)) continue;
-            const int64_t idx = (static_cast<int64_t>(blockIdx.y) * a.sink_slots + first + j) * n_bh + blockIdx.z;      // of the item, see get_item
-            const float4 *src = reinterpret_cast<const float4 *>(a.parts + (idx * 2 + which) * (kBM * D) + row * D + c);
-            const float4 u = __ldcg(src), v = __ldcg(src + 1);
-            x[0] += u.x; x[1] += u.y; x[2] += u.z; x[3] += u.w;
-            x[4] += v.x; x[5] += v.y; x[6] += v.z; x[7] += v.w;
+        constexpr int kAhead = 8;            // chunks whose parts are on their way together
+        for (int j0 = 0; j0 < n_chunks; j0 += kAhead) {
+            float4 u[kAhead], v[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                u[i] = v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                int t_lo = 0, n_t = 0;
+                if (j0 + i < n_chunks) chunk_rows(a, s, m0, j0 + i, t_lo, n_t);
+                if (n_t > 0 && row < chunk_keys(a, s, m0, t_lo)) {
+                    const int64_t idx = (static_cast<int64_t>(blockIdx.y) * a.sink_slots + first + j0 + i) * n_bh + blockIdx.z;      // of the item, see get_item
+                    const float4 *src = reinterpret_cast<const float4 *>(a.parts + (idx * 2 + which) * (kBM * D) + row * D + c);
+                    u[i] = __ldcg(src);
+                    v[i] = __ldcg(src + 1);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                x[0] += u[i].x; x[1] += u[i].y; x[2] += u[i].z; x[3] += u[i].w;
+                x[4] += v[i].x; x[5] += v[i].y; x[6] += v[i].z; x[7] += v[i].w;
+            }
         }
         T *dst = static_cast<T *>(which == 0 ? a.dk : a.dv) + b * a.kv_sb + hk * a.kv_sh + static_cast<int64_t>(s.bos + m0 + row) * a.kv_st + c;
         *reinterpret_cast<uint4 *>(dst) = make_uint4(Elem<T>::pack(x[0], x[1]), Elem<T>::pack(x[2], x[3]), Elem<T>::pack(x[4], x[5]), Elem<T>::pack(x[6], x[7]));
@@ -1020,7 +1033,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const TrainArgs a) {
 template <typename T, int D>
 int launch_join(const TrainArgs &a, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.sink_slots, (a.sink + kBM - 1) / kBM, a.batch * a.heads_kv);
+    cfg.gridDim = dim3(a.sink_slots * kJoinCtas, (a.sink + kBM - 1) / kBM, a.batch * a.heads_kv);
     cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -1056,7 +1069,7 @@ int launch_mode(const TrainArgs &a, int n_tok, const ErrSink &sink, bool overlap
     const int n_items = chunks + tiles * a.batch * (DQR ? a.heads_q : a.heads_kv), sms = tma::sm_count();
     if (sms <= 0) return PLX_ERR_LAUNCH;
     // with plenty of items a CTA takes them in neighbouring pairs (a heavy and a light tile)
-    const bool dynamic = items_by_hardware(n_items, sms, a.cu != nullptr || chunks > 0);
+    const bool dynamic = items_by_hardware(n_items, sms, a.cu != nullptr || (SINK && !DQR));
     const int chunk_shift = dynamic ? -1 : n_items >= 2 * sms ? 1 : 0;
     const int units = dynamic ? n_items : (n_items + (1 << chunk_shift) - 1) >> chunk_shift;
     const int group = !dynamic && n_items > sms ? 0 : dynamic && a.cu ? 1 : item_group(a.batch * (DQR ? a.heads_q : a.heads_kv), tiles, sms);
@@ -1126,8 +1139,11 @@ int launch_train_bwd_sm100(const TrainArgs &a, int dtype, int head_dim, int stag
 }
 
 // Rows of a chunk: about as much work as an item of other keys has, 512 at least (a chunk costs its sums in 32 bits), and some
-// 32 chunks in all at most, which bounds the workspace.
-int train_sink_chunk(int window, int len_q) {
+// 32 chunks in all at most, which bounds the workspace; none where there are many tiles of sinks, which are items enough.
+// dk/dv and the join against items as long as the sequence, us, 4 sinks, head_dim 128: L = 8192, window 1024, 16 (batch, head) 254 + 11 / 284,
+// 64 919 + 13 / 1259; window 256, 64 485 + 15 / 932.
+int train_sink_chunk(int sink, int window, int len_q) {
+    if (sink > 8 * kBM) return (len_q + kBN - 1) / kBN * kBN;
     const int64_t rows = std::max<int64_t>({512, static_cast<int64_t>(window) + kBM, len_q / 32});
     return static_cast<int>((rows + kBN - 1) / kBN * kBN);
 }

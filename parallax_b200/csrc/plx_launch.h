@@ -75,8 +75,9 @@ bool train_bwd_sm100_supported(const TrainArgs &a, int head_dim);
 // `overlap`: the kernel launched just before on this stream is the row statistics (dk/dv) or dk/dv (dq/dr) of the
 // same call, and this one may start under its end
 int launch_train_bwd_sm100(const TrainArgs &a, int dtype, int head_dim, int stage, bool overlap, cudaStream_t stream);
-// sinks: rows of a chunk of dk/dv, and the launch that adds the chunks up (behind dk/dv, where a.sink_slots > 0)
-int train_sink_chunk(int window, int len_q);
+// sinks: rows of a chunk of dk/dv (no fewer than there are: none), and the launch that adds the chunks up (behind dk/dv, where
+// a.sink_slots > 0)
+int train_sink_chunk(int sink, int window, int len_q);
 int launch_train_bwd_join(const TrainArgs &a, int dtype, int head_dim, cudaStream_t stream);
 
 constexpr int kDecodeGqaWarps = 8;   // warps (independent splits) per CTA of the grouped-query decode kernel

@@ -113,6 +113,8 @@ TRAIN = [
     (1, 2, 2, 1300, 2000, 128, BF, 30, 17),
     (1, 1, 1, 2200, 1500, 64, BF, 300, 4),
     (1, 2, 2, 2100, 2100, 128, BF, 1024, 6),
+    (9, 16, 16, 700, 700, 64, BF, 350, 4),        # many heads
+    (2, 2, 1, 1500, 1500, 64, FP, 20, 1100),      # tiles of sinks enough without chunks
 ]
 
 
