@@ -81,8 +81,8 @@ __device__ __forceinline__ void clear(const Bitmap &m) {
 // The active entries of the table -> bits; len(b): the keys of row b.
 template <typename Len>
 __device__ __forceinline__ void mark(const Bitmap &m, const TableArgs &t, Len len) {
-    // a warp takes 128 entries of a row at a time, of two rows at once: bound by the round trips for lengths and entries
-    constexpr int kAhead = 4, kRows = 2;
+    // a warp takes 128 entries of a row at a time, of four rows at once: bound by the round trips for lengths and entries
+    constexpr int kAhead = 4, kRows = 4;
     const int lane = threadIdx.x & 31, segments = (t.pages_per_seq + 32 * kAhead - 1) / (32 * kAhead), units = t.batch * segments;
     for (int unit0 = threadIdx.x >> 5; unit0 < units; unit0 += kRows * kPlanThreads / 32) {
         int p[kRows][kAhead], active[kRows];

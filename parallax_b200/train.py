@@ -94,36 +94,40 @@ def _unfold(x: torch.Tensor, rep: int) -> torch.Tensor:
     return x.contiguous().view(bh // rep, rep, n, d)
 
 
-def parallax_fwd(q, r, k, v, qk_scale, n_rep: int = 1, window_size_left: int = -1):
+def parallax_fwd(q, r, k, v, qk_scale, n_rep: int = 1, window_size_left: int = -1, sink_tokens: int = 0):
     """Raw forward with the saved statistics (reference: ``parallax_fwd``,
     parallax/triton/parallax_train.py:255-313).
 
     q, r: ``(B * H_q, L_q, D)``; k, v: ``(B * H_kv, L_kv, D)``.  Returns
     ``(o, barv, d1, bart, m)``: o, barv like q; d1, bart, m fp32
-    ``(B * H_q, L_q, 1)``.
+    ``(B * H_q, L_q, 1)``.  ``sink_tokens``: as in :func:`parallax_func`.
     """
     _check_dtype("parallax_fwd", q)
+    check_sinks("parallax_fwd", sink_tokens)
     assert q.shape[0] % n_rep == 0, f"q batch axis {q.shape[0]} must be divisible by n_rep={n_rep}"
     assert k.shape[0] == q.shape[0] // n_rep, "k batch axis must equal q batch axis // n_rep"
     _check_cuda("parallax_fwd", q, r, k, v)
     o, barv, d1, bart, m = ops.train_fwd(_unfold(q, n_rep), _unfold(r, n_rep), _unfold(k, 1), _unfold(v, 1),
-                                         float(qk_scale), int(window_size_left), ops.BHLD, None)
+                                         float(qk_scale), int(window_size_left), ops.BHLD, None, int(sink_tokens))
     flat = lambda x: x.reshape(q.shape[0], q.shape[1], -1)
     return flat(o), flat(barv), flat(d1), flat(bart), flat(m)
 
 
 def parallax_bwd(q, r, k, v, o, barv, d1, bart, m, grad_o, qk_scale, n_rep: int = 1,
-                 window_size_left: int = -1):
+                 window_size_left: int = -1, sink_tokens: int = 0):
     """Raw backward (reference: ``parallax_bwd``,
     parallax/triton/parallax_train.py:892-1006).  Returns
     ``(grad_q, grad_r, grad_k, grad_v)`` shaped like q, r, k, v; the kv-head
     gradients are already summed over the ``n_rep`` q heads of each group.
+    ``sink_tokens``: that of the forward.
     """
     _check_dtype("parallax_bwd", q)
+    check_sinks("parallax_bwd", sink_tokens)
     assert q.shape[0] % n_rep == 0 and k.shape[0] == q.shape[0] // n_rep
     _check_cuda("parallax_bwd", q, r, k, v, grad_o)
     st = lambda x: x.contiguous().view(q.shape[0] // n_rep, n_rep, q.shape[1])
     dq, dr, dk, dv = ops.train_bwd(_unfold(q, n_rep), _unfold(r, n_rep), _unfold(k, 1), _unfold(v, 1),
                                    _unfold(o, n_rep), _unfold(barv, n_rep), st(d1), st(bart), st(m),
-                                   _unfold(grad_o, n_rep), float(qk_scale), int(window_size_left), ops.BHLD, None)
+                                   _unfold(grad_o, n_rep), float(qk_scale), int(window_size_left), ops.BHLD, None,
+                                   int(sink_tokens))
     return dq.view_as(q), dr.view_as(r), dk.view_as(k), dv.view_as(v)

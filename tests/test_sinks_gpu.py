@@ -204,6 +204,17 @@ def test_gradients_against_differences():
     assert abs(got - want) <= bound, (got, want, bound)
 
 
+def test_raw_forward_and_backward():
+    """parallax_fwd / parallax_bwd: heads folded into the batch axis."""
+    window, sinks, n, d = 70, 4, 700, 64
+    q, r, k, v = inputs(1, 4, 2, n, n, d, BF)
+    go = randn(1, 4, n, d, seed=9)
+    flat = lambda x: x.reshape(-1, n, d)                                                                   # noqa: E731
+    saved = plx.parallax_fwd(flat(q), flat(r), flat(k), flat(v), d ** -0.5, 2, window, sinks)
+    grads = plx.parallax_bwd(flat(q), flat(r), flat(k), flat(v), *saved, flat(go), d ** -0.5, 2, window, sinks)
+    check([saved[0].view_as(q), *(g.view_as(x) for g, x in zip(grads, (q, r, k, v)))], reference(q, r, k, v, go, window, sinks))
+
+
 def test_captured_training_step():
     window, sinks, n = 40, 4, 800
     q, r, k, v = (x.requires_grad_() for x in inputs(1, 2, 2, n, n, 64, BF))
