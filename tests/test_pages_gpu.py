@@ -31,7 +31,7 @@ def make_pool(n_pages, page, h, d, dtype=torch.bfloat16, layout="token"):
 
 def make_table(rng, rows, m, page, n_pages, share=0):
     """Lengths and a table with garbage behind the active entries; the rows from 1 on begin with `share` pages of row 0."""
-    lens = [rng.choice([0, 1, page - 1, page, page + 1, rng.randint(0, m * page), m * page]) for _ in range(rows)]
+    lens = [min(rng.choice([0, 1, page - 1, page, page + 1, rng.randint(0, m * page), m * page]), m * page) for _ in range(rows)]
     order = list(range(n_pages))
     rng.shuffle(order)
     table, at = [], 0
