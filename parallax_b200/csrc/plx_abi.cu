@@ -170,9 +170,9 @@ static int run_decode(const plx_decode_problem *p, const void *q, const void *r,
                       float *part, const int32_t *seqused_k, const int32_t *cache_start, void *workspace,
                       size_t workspace_bytes, cudaStream_t stream, const plx_exchange *xch = nullptr,
                       const StepCopies *step = nullptr, const Sweep &sweep = Sweep()) {
+    if (sweep.sink < 0) return PLX_ERR_BAD_ARG;
     int st = check_decode_args(p, q, r, k, v, out, part);
     if (st != PLX_OK) return st;
-    if (sweep.sink < 0) return PLX_ERR_BAD_ARG;
     if (sweep.sink > 0 && (p->kv_offset != 0 || xch)) return PLX_ERR_UNSUPPORTED;   // sinks of a cache that is not key-sharded
     if (p->n_splits > 1 && (!workspace || workspace_bytes < decode_ws_bytes(p) || misaligned16(workspace)))
         return PLX_ERR_WORKSPACE;
@@ -548,7 +548,7 @@ int plx_decode_step(const plx_decode_problem *p, void *q, const void *q_src, voi
 int plx_decode_step_sink(const plx_decode_problem *p, int32_t sink_tokens, void *q, const void *q_src, void *r, const void *r_src, const void *k,
                          const void *v, void *out, int32_t *seqused_k, const int32_t *seqused_src, void *workspace, size_t workspace_bytes,
                          plx_stream_t stream) {
-    if (!p || !out || !q || !r || (seqused_src && !seqused_k) || misaligned16(q) || misaligned16(r)) return PLX_ERR_BAD_ARG;
+    if (!p || !out || !q || !r || (seqused_src && !seqused_k) || misaligned16(q) || misaligned16(r) || sink_tokens < 0) return PLX_ERR_BAD_ARG;
     if (p->batch > PLX_DECODE_STEP_ROWS) return PLX_ERR_UNSUPPORTED;
     const int st = check_decode(p);
     if (st != PLX_OK) return st;
@@ -618,8 +618,9 @@ int plx_decode_prefix_workspace_bytes(const plx_decode_problem *p, const plx_pre
 
 int plx_decode_prefix(const plx_decode_problem *p, const plx_prefix *x, const void *q, const void *r, const void *k, const void *v, void *out,
                       const int32_t *seqused_k, void *workspace, size_t workspace_bytes, plx_stream_t stream) {
-    int st = check_decode_args(p, q, r, k, v, out, nullptr);
+    int st = check_decode(p);
     if (st == PLX_OK) st = check_prefix(p, x);
+    if (st == PLX_OK) st = check_decode_args(p, q, r, k, v, out, nullptr);
     if (st != PLX_OK) return st;
     const size_t part_bytes = prefix_part_bytes(p, x);
     if (!workspace || misaligned16(workspace) || workspace_bytes < part_bytes + decode_ws_bytes(p)) return PLX_ERR_WORKSPACE;
