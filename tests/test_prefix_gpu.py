@@ -280,3 +280,57 @@ def test_the_life_of_a_paged_cache():
     assert n_live.item() == 200 - n_free.item() and table[live, :lens[0].item() // page].max() < n_live.item()
     k_pool[n_live.item():] = v_pool[n_live.item():] = torch.nan         # nothing behind the live pages is read
     agree(live)
+
+
+def test_pages_behind_two_to_the_31_elements():
+    """Pools of more than 2^31 elements: the last pages of one as a prefix, as sinks and windows, copied, forked and compacted."""
+    page, hq, hkv, d, n_pages = 64, 16, 8, 128, 33000
+    assert (n_pages - 20) * page * hkv * d > 2 ** 31
+    k_pool, v_pool = (torch.empty(n_pages, page, hkv, d, dtype=BF, device="cuda") for _ in range(2))
+    b, prefix, own = 2, 4 * page, 50
+    order = list(range(n_pages - 1, n_pages - 13, -2))             # pages n - 1, n - 3, ..
+    table = ints([order[:4] + [order[4]], order[:4] + [order[5]]])
+    for p in order:
+        k_pool[p], v_pool[p] = randn(page, hkv, d, seed=p), randn(page, hkv, d, seed=2 * p)
+    lens = ints([prefix + own, prefix + 3])
+    q, r = randn(b, 1, hq, d, seed=1), randn(b, 1, hq, d, scale=0.5, seed=2)
+
+    def rows():
+        return [[pool[table[i].long()].flatten(0, 1)[:lens[i].item()].clone() for i in range(b)] for pool in (k_pool, v_pool)]
+
+    keys, values = rows()
+    want = reference(q, r, keys, values)
+    ws = torch.zeros(1 << 22, device="cuda")
+    for splits in (0, 1, 3):
+        out = torch.empty_like(q)
+        ops.decode_prefix(q, r, None, None, prefix, k_pool, v_pool, out, ws, d ** -0.5, 2, splits, lens, table)
+        close(out, want, 2, splits)
+    hidden = [torch.cat([torch.arange(5), torch.arange(n - 90, n)]).cuda() for n in lens.tolist()]
+    sinks = reference(q, r, [x[at] for x, at in zip(keys, hidden)], [x[at] for x, at in zip(values, hidden)])
+    close(plx.parallax_attn_with_kvcache(q, r, k_pool, v_pool, page_table=table, seqused_k=lens, window_size=90, sink_tokens=5), sinks, 2, "sinks")
+    several = plx.parallax_attn_with_kvcache(q.expand(-1, 2, -1, -1).contiguous(), r.expand(-1, 2, -1, -1).contiguous(), k_pool, v_pool, page_table=table,
+                                             seqused_k=lens, window_size=90, sink_tokens=5)
+    close(several[:, 1:], sinks, 2, "sinks, two tokens")
+    plx.parallax_copy_pages(k_pool, v_pool, ints([order[0], order[5]]), ints([7, n_pages - 2]))
+    assert torch.equal(k_pool[7], k_pool[order[0]]) and torch.equal(v_pool[n_pages - 2], v_pool[order[5]])
+    forked, flens, missing = plx.parallax_fork_pages(k_pool, v_pool, table, lens, ints([0]), ints([1]))
+    assert missing.item() == 0 and forked[1].tolist() == order[:4] + [0] and torch.equal(k_pool[0, :own], k_pool[order[4], :own])
+    table, n_live = plx.parallax_compact_pages(k_pool, v_pool, table, lens)
+    assert n_live.item() == 6 and sorted(set(table.flatten().tolist())) == list(range(6))
+    again = rows()
+    assert all(torch.equal(x, y) for new, old in zip(again, (keys, values)) for x, y in zip(new, old))
+
+
+def test_dense_prefix_behind_two_to_the_31_elements():
+    """A prefix of more than 2^31 elements, of which all but the last keys weigh nothing."""
+    hkv, d, p = 8, 128, 2 ** 21 + 1000
+    assert p * hkv * d > 2 ** 31
+    kp, vp = (torch.zeros(p, hkv, d, dtype=BF, device="cuda") for _ in range(2))
+    q, r = randn(3, 1, 16, d, seed=1), randn(3, 1, 16, d, scale=0.5, seed=2)
+    k, v = randn(3, 5, hkv, d, seed=3), randn(3, 5, hkv, d, seed=4)
+    kp[-200:], vp[-200:] = randn(200, hkv, d, scale=12.0, seed=5), randn(200, hkv, d, seed=6)      # logits far above those of the zeros
+    want = reference(q, r, [torch.cat((kp[-4000:], k[i])) for i in range(3)], [torch.cat((vp[-4000:], v[i])) for i in range(3)])
+    close(plx.parallax_decode_shared_prefix(q, r, kp, vp, k, v), want, 2, "shared")
+    out, ws = torch.empty_like(q), torch.zeros(1 << 22, device="cuda")
+    ops.decode_prefix(q, r, kp, vp, p, k, v, out, ws, d ** -0.5, 16, 0, None, None)
+    close(out, want, 2, "every row")
