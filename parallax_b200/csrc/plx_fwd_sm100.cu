@@ -347,7 +347,11 @@ fwd_sm100_kernel(const TrainArgs a, const __grid_constant__ CUtensorMap tm_q, co
                     // A tile that reaches past the row's active length inside the cache: what lies there must not
                     // be seen (0 * NaN), so its rows are zeroed once the copy has landed, before the tile is handed
                     // over.  (Past the end of a tensor map the copy itself fills zeros.)
-                    const bool tail = EXT && key0 + kBN > it.nk && (a.page_table || it.nk < a.len_k);
+                    // With sinks so do values between the sinks and the window of the item's first row (pages of them may have gone to
+                    // another sequence); the scores of such keys are masked.
+                    const int hidden_lo = MODE == kExtendSink ? max(a.sink, key0) : 0;
+                    const int hidden_hi = MODE == kExtendSink && !is_k ? min(it.r0 + it.off - a.window + 1, key0 + kBN) : 0;
+                    const bool past = EXT && key0 + kBN > it.nk && (a.page_table || it.nk < a.len_k), tail = past || hidden_hi > hidden_lo;
                     const uint32_t full = bar(tail ? L::kTail + (is_k ? 0 : 1) : full0 + s);
                     if (EXT && a.page_table) {
                         const int n_boxes = min(kBN >> box_shift, (it.nk - key0 + (1 << box_shift) - 1) >> box_shift);
@@ -368,11 +372,15 @@ fwd_sm100_kernel(const TrainArgs a, const __grid_constant__ CUtensorMap tm_q, co
                         ok = mbar_wait(full, n_tails & 1, err, is_k ? 17 : 18);
                         if (!ok) break;
                         ++n_tails;
-                        for (int row = it.nk - key0; row < kBN; ++row)
-                            for (int pn = 0; pn < L::kPanels; ++pn)
+                        auto zero = [&](int row, int end) {
+                            for (; row < end; ++row)
+                                for (int pn = 0; pn < L::kPanels; ++pn)
 #pragma unroll
-                                for (int c = 0; c < 8; ++c)
-                                    asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};\n" ::"r"(dst + pn * kKVPanel + row * 128 + c * 16), "r"(0u) : "memory");
+                                    for (int c = 0; c < 8; ++c)
+                                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};\n" ::"r"(dst + pn * kKVPanel + row * 128 + c * 16), "r"(0u) : "memory");
+                        };
+                        if (past) zero(it.nk - key0, kBN);
+                        if (MODE == kExtendSink) zero(hidden_lo - key0, hidden_hi - key0);
                         fence_proxy_async();
                         mbar_arrive(bar(full0 + s));
                     }
@@ -592,7 +600,10 @@ fwd_sm100_kernel(const TrainArgs a, const __grid_constant__ CUtensorMap tm_q, co
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
                                 const int c = c0 + 8 * k + 2 * t + e;
-                                if (c > last || (c < first && !(SINK && c < a.sink))) s1[4 * k + 2 * hh + e] = 0xff800000u;  // -inf
+                                if (c > last || (c < first && !(SINK && c < a.sink))) {
+                                    s1[4 * k + 2 * hh + e] = 0xff800000u;  // -inf
+                                    if (MODE == kExtendSink) s2[4 * k + 2 * hh + e] = 0u;
+                                }
                             }
                     }
                 }

@@ -336,18 +336,31 @@ def test_decode_behind_padding(hq, hkv, window, sinks):
 
 @pytest.mark.parametrize("hq,hkv,d,page,t,lq,window,sinks", [
     (4, 4, 128, 0, 500, 17, 60, 4), (8, 2, 64, 0, 900, 200, 0, 3), (8, 2, 128, 16, 640, 64, 100, 70), (4, 1, 64, 64, 700, 130, 33, 5),
-    (4, 2, 128, 4, 300, 9, 20, 2), (2, 2, 64, 128, 1500, 3, 128, 130)])
+    (2, 2, 64, 128, 1500, 3, 128, 130), (8, 8, 128, 32, 2048, 300, 256, 4)])
 def test_extend(hq, hkv, d, page, t, lq, window, sinks):
     lens = [t, max(lq, t // 2 + 1), lq]
     b = len(lens)
     q, r = randn(b, lq, hq, d, seed=1), randn(b, lq, hq, d, scale=0.5, seed=2)
     k, v = randn(b, t, hkv, d, seed=3), randn(b, t, hkv, d, seed=4)
     want = decode_reference(q, r, k, v, lens, [0] * b, window, sinks)
+    k, v = hide(k, lens, [0] * b, window, sinks, lq), hide(v, lens, [0] * b, window, sinks, lq)
     seqused = torch.tensor(lens, dtype=torch.int32, device="cuda")
     table = None
     if page:
         k, v, table = paged(k, v, page)
     got = plx.parallax_attn_with_kvcache(q, r, k, v, page_table=table, seqused_k=seqused, window_size=window, sink_tokens=sinks)
+    close(got, want, 2, "o")
+
+
+def test_extend_over_pages_that_are_too_small_for_a_tile():
+    """Pages of fewer than 8 keys: gathered row by row, and run as a dense problem of the training forward."""
+    t, lq, window, sinks, lens = 300, 9, 20, 2, [300, 151, 9]
+    q, r = randn(3, lq, 4, 128, seed=1), randn(3, lq, 4, 128, scale=0.5, seed=2)
+    k, v = randn(3, t, 2, 128, seed=3), randn(3, t, 2, 128, seed=4)
+    want = decode_reference(q, r, k, v, lens, [0] * 3, window, sinks)
+    k, v, table = paged(k, v, 4)
+    got = plx.parallax_attn_with_kvcache(q, r, k, v, page_table=table, seqused_k=torch.tensor(lens, dtype=torch.int32, device="cuda"), window_size=window,
+                                         sink_tokens=sinks)
     close(got, want, 2, "o")
 
 
