@@ -158,6 +158,34 @@ def test_lengths_and_pages_out_of_range_are_passed_over():
     assert lens.tolist() == [10, 0] and missing.tolist() == [0] and new[0].tolist() == [2 ** 31 - 1, 15, 0]
 
 
+@pytest.mark.parametrize("rows,n", [(5000, 4000), (300, 2500), (4096, 1024), (4097, 1025)])
+def test_fork_of_many_rows(rows, n):
+    """More rows than shared memory has room for, more pairs than a CTA has threads."""
+    rng = random.Random(6)
+    page, m = 4, 3
+    n_pages = rows * m + n
+    k, v = make_pool(n_pages, page, 1, 8)
+    lens = [rng.randint(0, m * page) for _ in range(rows)]
+    order = rng.sample(range(n_pages), rows * m)
+    table = torch.tensor(order, dtype=torch.int32).view(rows, m)
+    parents, children = [rng.randrange(rows) for _ in range(n)], [rng.randrange(rows) for _ in range(n)]
+    want_k, want_table, want_lens = k.clone(), table.clone(), list(lens)
+    live = {int(table[b, j]) for b in range(rows) for j in range(-(-lens[b] // page))}
+    free = iter(p for p in range(n_pages) if p not in live)
+    final = dict(zip(children, range(n)))
+    for i, (p, c) in enumerate(zip(parents, children)):
+        if final[c] != i:
+            continue
+        want_table[c], want_lens[c] = table[p], lens[p]
+        if lens[p] % page and p != c:
+            new, slot = next(free), lens[p] // page
+            want_k[new, :lens[p] % page] = k[int(table[p, slot]), :lens[p] % page]
+            want_table[c, slot] = new
+    got, got_lens, missing = plx.parallax_fork_pages(k, v, table.cuda(), ints(lens), ints(parents), ints(children))
+    assert missing.item() == 0 and got_lens.tolist() == want_lens and torch.equal(got.cpu(), want_table)
+    assert torch.equal(k.view(torch.int16), want_k.view(torch.int16))
+
+
 def test_fork_without_a_free_page():
     k, v = make_pool(4, 16, 1, 64)
     table, lens = ints([0, 1, 2, 3]).view(2, 2), ints([20, 30])
