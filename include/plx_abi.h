@@ -272,7 +272,7 @@ int plx_decode_step_sink(const plx_decode_problem *p, int32_t sink_tokens, void 
  * cache of `p` itself: every row's page table begins with the same pages, len is a multiple of the page size, and lengths count
  * the prefix too (shorter ones count as len).  Only the first row's entries of it are read.  No sliding window, no kv_offset.
  * The q heads of a kv head of all rows are the M dimension of tensor-core products over the prefix, whose keys are cut into
- * n_splits parts (plx_decode_prefix_splits; at most one for every 64 keys); each row's own keys are a plx_decode_partial, and a third launch merges.  n_splits 0, where
+ * n_splits parts (at most one for every 64 keys); each row's own keys are a plx_decode_partial that runs beside that, and a third launch merges.  n_splits 0, where
  * that is slower: one launch, in which every row sweeps the prefix in front of its own keys (p->n_splits is then for all of them).
  * Workspace: plx_decode_prefix_workspace_bytes(), ZERO-FILLED ONCE like that of plx_decode.  (No counterpart in the reference.) */
 #define PLX_PREFIX_MAX_SPLITS 127
@@ -282,8 +282,9 @@ typedef struct plx_prefix {
     int32_t len;
     int32_t n_splits;
 } plx_prefix;
-int plx_decode_prefix_splits(int32_t batch, int32_t heads_q, int32_t heads_kv, int32_t len, int32_t head_dim,
-                             int32_t sm_count);
+/* n_splits of plx_prefix and of the problem, for own keys of up to own_len a row.  Pure host arithmetic. */
+int plx_decode_prefix_plan(int32_t batch, int32_t heads_q, int32_t heads_kv, int32_t len, int32_t own_len, int32_t head_dim,
+                           int32_t sm_count, int32_t *prefix_splits, int32_t *own_splits);
 int plx_decode_prefix_workspace_bytes(const plx_decode_problem *p, const plx_prefix *x, size_t *bytes);
 int plx_decode_prefix(const plx_decode_problem *p, const plx_prefix *x, const void *q, const void *r, const void *k,
                       const void *v, void *out, const int32_t *seqused_k, void *workspace, size_t workspace_bytes,

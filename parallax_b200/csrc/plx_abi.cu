@@ -1,5 +1,6 @@
 // extern "C" surface of libplx_sm100.so (declared in include/plx_abi.h):
 // argument validation, kernel selection, launch accounting.
+#include <algorithm>
 #include <atomic>
 
 #include "plx_common.cuh"
@@ -162,7 +163,7 @@ struct Sweep {
     int first_key = 0;         // keys before it are not looked at
     int min_len = 1;           // shorter lengths count as it
     int part_stride = 1;       // records between those of two (batch, head)
-    int let_next_in = 0;       // the next launch may begin under this one
+    int under = 0;             // runs under the launch before it, which has waited for what came before both
     const plx_prefix *prefix = nullptr;   // keys in tensors of their own that every row begins with
 };
 
@@ -184,7 +185,7 @@ static int run_decode(const plx_decode_problem *p, const void *q, const void *r,
     a.sink = p->window_left >= 0 && p->window_left < p->cache_len ? (sweep.sink < p->cache_len ? sweep.sink : p->cache_len) : 0;
     a.first_key = sweep.first_key;
     a.min_len = sweep.min_len;
-    a.let_next_in = sweep.let_next_in;
+    a.under = sweep.under;
     if (sweep.prefix) {
         a.k_prefix = sweep.prefix->k; a.v_prefix = sweep.prefix->v;
         a.prefix_len = sweep.prefix->len;
@@ -580,32 +581,60 @@ int plx_decode_sink(const plx_decode_problem *p, int32_t sink_tokens, const void
                       nullptr, Sweep{sink_tokens});
 }
 
-int plx_decode_prefix_splits(int32_t batch, int32_t heads_q, int32_t heads_kv, int32_t len, int32_t head_dim, int32_t sm_count) {
-    if (batch <= 0 || heads_kv <= 0 || heads_q % heads_kv != 0 || len <= 0 || head_dim <= 0 || sm_count <= 0) return 1;
-    // Shared: an item costs its tiles of 64 keys and about four more for its start and its end, the SMs take items in rounds, and
-    // the merge goes through 16 records at a time.
+int plx_decode_prefix_plan(int32_t batch, int32_t heads_q, int32_t heads_kv, int32_t len, int32_t own_len, int32_t head_dim, int32_t sm_count,
+                           int32_t *prefix_splits, int32_t *own_splits) {
+    if (batch <= 0 || heads_kv <= 0 || heads_q < heads_kv || heads_q % heads_kv != 0 || len <= 0 || own_len < 0 || head_dim <= 0 || sm_count <= 0 ||
+        !prefix_splits || !own_splits)
+        return PLX_ERR_BAD_ARG;
+    // A model of a call in units of 10 ns, its constants fitted at head_dim 128 to the times of 25 shapes at up to 90 pairs of splits each (4 to 200
+    // rows, prefixes of 1000 to 32768 keys, 30 to 8000 own ones of uneven lengths): what it chooses is within 7% of the best pair for each of them.
+    const bool grouped = heads_q > heads_kv;
+    const int64_t rows = static_cast<int64_t>(batch) * heads_kv * (grouped ? (heads_q / heads_kv + 15) / 16 : 1);   // sweeps of own keys
+    // Shared.  The prefix: rounds of items over the SMs, 1.07 us a tile of 64 keys and about four tiles for start and end.  The own keys run beside
+    // it, `k` times 16 of them in a CTA: one CTA on an SM of the prefix, which slows that one down, eight on an SM that the prefix leaves free; the
+    // longest row's CTA may take longest.  So the best prefix may leave SMs free.  Then the merge.  (The two one after the other, each over all SMs: 32
+    // rows, 32 : 8 heads, 8192 keys and 512 own ones 34.7 us against 29.2; 128 rows, 32768 keys 172 against 153.)
+    const int64_t beside = grouped ? 80 : 460, free_start = grouped ? 300 : 380, free_step = grouped ? 140 : 240, tail_start = grouped ? 350 : 600,
+                  tail_step = grouped ? 100 : 200;
     const int64_t units = static_cast<int64_t>(prefix_row_tiles(heads_q / heads_kv, batch)) * heads_kv, tiles = (static_cast<int64_t>(len) + 63) / 64;
-    int best = 1;
-    int64_t best_cost = INT64_MAX, best_tiles = 0;
+    int best = 1, best_own = 1;
+    int64_t shared = INT64_MAX;
     for (int n = 1; n <= PLX_PREFIX_MAX_SPLITS && n <= tiles; ++n) {
-        const int64_t rounds = (units * n + sm_count - 1) / sm_count, per_sm = rounds * ((tiles + n - 1) / n), cost = 16 * (per_sm + 4 * rounds) + n;
-        if (cost < best_cost) {
-            best_cost = cost;
-            best_tiles = per_sm;
-            best = n;
+        const int64_t rounds = (units * n + sm_count - 1) / sm_count, used = units * n / rounds, free = sm_count > used ? sm_count - used : 0;
+        const int64_t prefix = 400 + rounds * (107 * ((tiles + n - 1) / n) + 400);
+        const int64_t merge = 200 + static_cast<int64_t>(batch) * heads_q * (n + 1) * PLX_DECODE_PART_FLOATS(head_dim) * 4 / 40000;
+        for (int own = 1; own <= 32 && (own == 1 || 16 * own <= own_len); own *= 2) {
+            const int64_t k = (static_cast<int64_t>(own_len) + 16 * own - 1) / (16 * own);
+            const int64_t ctas = grouped || heads_q % 2 ? rows * own : rows * own / 2;
+            int64_t cost = prefix;
+            if (k > 0) {
+                const double rate_beside = static_cast<double>(used) / (beside * k), rate = rate_beside + 8.0 * free / (free_start + free_step * k);
+                const int64_t all = static_cast<int64_t>(ctas / rate), tail = tail_start + tail_step * k;
+                cost += static_cast<int64_t>(0.75 * std::min(all, prefix) * rate_beside / rate);
+                cost = std::max(cost, std::max(500 + all, tail) + std::min(all, tail) / 8);
+            }
+            cost += merge;
+            if (cost < shared) {
+                shared = cost;
+                best = n;
+                best_own = own;
+            }
         }
     }
-    // Against every row sweeping the prefix, which is one launch instead of three.  Measured at head_dim 128, device time of the whole
-    // call with 40 own keys, us, shared / every row: 8 : 8 heads, 4 rows, 500 keys 10.2 / 6.7, 2000 12.8 / 10.8, 4000 16.3 / 16.6, 16000 33.4 / 65.9; 8 rows,
-    // 500 10.2 / 8.5, 1000 11.2 / 15.6; 16 rows, 500 10.6 / 13.3; 32 : 8 heads, 2 rows, 4000 16.3 / 13.5, 16000 38.2 / 26.9; 4 rows, 4000 16.6 / 16.6; 16 rows, 1000
-    // 12.9 / 15.5, 4000 18.0 / 37.7; 8 : 1 heads, 8 rows, 16000 25.7 / 19.4, 16 rows 21.8 / 28.4.  In units of 10 ns: shared 10 us and 1.65 for a tile
-    // of the SM that has most; every row 4.5 us (64 (row, head) pairs at most, see plx_decode_choose_splits) or 9, and its bytes at 4.4 TB/s with one q
-    // head per kv head, 7 with grouped ones.
-    const int64_t kb = 4ll * batch * len * heads_kv * head_dim / 1000;
-    const bool grouped = heads_q > heads_kv;
-    const int64_t shared = 1000 + 165 * best_tiles, every_row = (!grouped && static_cast<int64_t>(batch) * heads_q <= PLX_DECODE_SPLIT_GROUP_MAX_BH ? 450 : 900) +
-                                                               kb / (grouped ? 70 : 44);
-    return every_row < shared ? 0 : best;
+    // Against every row sweeping the prefix in front of its own keys, one launch instead of three, its bytes at 4.4 TB/s with one q head per kv head and, the
+    // rows meeting in L2, 9 with grouped ones.  Measured, device time of the call with 40 own keys, us, shared / every row: 8 : 8 heads, 4 rows, 500 keys
+    // 11.4 / 7.2, 2000 12.6 / 11.4, 4000 14.7 / 17.4, 16000 25.0 / 66.1; 8 rows, 500 11.2 / 9.2, 1000 11.7 / 15.8; 16 rows, 500 11.3 / 14.3; 32 : 8 heads, 2 rows, 4000
+    // 15.0 / 13.7, 16000 24.8 / 26.8; 4 rows, 4000 14.8 / 17.4; 16 rows, 500 12.8 / 12.0, 1000 13.3 / 16.3, 4000 16.4 / 38.8; 8 : 1 heads, 8 rows, 16000 19.8 / 20.0, 16 rows 21.0 / 28.2.
+    const int64_t keys = static_cast<int64_t>(len) + own_len, kb = 4ll * batch * keys * heads_kv * head_dim / 1000;
+    const int64_t every_row = grouped ? 1050 + kb / 90 : (static_cast<int64_t>(batch) * heads_q <= PLX_DECODE_SPLIT_GROUP_MAX_BH ? 450 : 900) + kb / 44;
+    if (every_row < shared * 15 / 16) {      // (the model is that much above the times, where there are few own keys)
+        *prefix_splits = 0;
+        *own_splits = plx_decode_choose_splits_gqa(batch, heads_q, heads_kv, static_cast<int32_t>(keys < INT32_MAX ? keys : INT32_MAX), sm_count);
+        return PLX_OK;
+    }
+    *prefix_splits = best;
+    *own_splits = best_own;
+    return PLX_OK;
 }
 
 int plx_decode_prefix_workspace_bytes(const plx_decode_problem *p, const plx_prefix *x, size_t *bytes) {
@@ -650,23 +679,24 @@ int plx_decode_prefix(const plx_decode_problem *p, const plx_prefix *x, const vo
     a.parts = parts;
     Sweep own;
     own.first_key = own.min_len = 0;
-    if (x->n_splits == 0 || !train_extend_sm100_supported(a, p->head_dim)) {
+    if (x->n_splits == 0 || p->batch == 65535 || !train_extend_sm100_supported(a, p->head_dim)) {      // (65535: no room for the sweep's one more)
         // every row sweeps the prefix in front of its own keys, in one launch
         if (in_cache) own.min_len = x->len;
         else own.prefix = x;
         return run_decode(p, q, r, k, v, out, nullptr, seqused_k, nullptr, rest, rest_bytes, cs, nullptr, nullptr, own);
     }
-    // Each row's own keys first: the items of the prefix, all alike, are handed out to the SMs as the sweep leaves them.
+    // The prefix, bound by the tensor pipe's tile period, takes a CTA per SM and lets the sweep of the rows' own keys in, bound by
+    // memory, whose CTAs of a warp or two fit beside it.
     const int n_parts = x->n_splits + 1;
-    if (in_cache) own.first_key = own.min_len = x->len;
-    own.part_stride = n_parts;
-    own.let_next_in = 1;
-    st = run_decode(p, q, r, k, v, nullptr, parts + static_cast<size_t>(n_parts - 1) * PLX_DECODE_PART_FLOATS(p->head_dim), seqused_k, nullptr, rest, rest_bytes,
-                    cs, nullptr, nullptr, own);
-    if (st != PLX_OK) return st;
     a.n_splits = x->n_splits;
     a.n_parts = n_parts;
     if ((st = launch_prefix_sm100(a, p->dtype, p->head_dim, cs)) != PLX_OK) return st;
+    if (in_cache) own.first_key = own.min_len = x->len;
+    own.part_stride = n_parts;
+    own.under = 1;
+    st = run_decode(p, q, r, k, v, nullptr, parts + static_cast<size_t>(n_parts - 1) * PLX_DECODE_PART_FLOATS(p->head_dim), seqused_k, nullptr, rest, rest_bytes,
+                    cs, nullptr, nullptr, own);
+    if (st != PLX_OK) return st;
     return launch_prefix_merge(parts, n_parts, static_cast<int64_t>(p->batch) * p->heads_q, p->head_dim, p->dtype, out, cs);
 }
 

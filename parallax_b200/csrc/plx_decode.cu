@@ -459,8 +459,11 @@ static cudaError_t launch_overlapped(void (*kern)(Params...), dim3 grid, int thr
 // FRONT: kernels of their own too.
 template <typename T, int D, int HG, int U, bool SG, bool DEAL, int FRONT = kNone>
 __global__ void __launch_bounds__(HG * 32, U > 4 ? 1 : 512 / (HG * 32)) decode_kernel(const DecodeArgs a) {
-    grid_wait();
-    if (a.let_next_in) launch_dependents();
+    if (!a.under) grid_wait();
+    else if (blockIdx.z == a.batch) {      // one CTA ends behind the kernel above, so that whatever follows this one follows both
+        if (blockIdx.x == 0 && blockIdx.y == 0) grid_wait();
+        return;
+    }
     constexpr int LPK = D / 8;      // lanes per key row
     constexpr int NS = 32 / LPK;    // streams per warp
     constexpr int REC = 2 * D + 4;  // floats per partial record
@@ -1016,10 +1019,15 @@ struct GqaSmem {
 // B = 16, 1024 keys, 32 : 8 heads 16.7 -> 16.0 us, B = 8, 4000 keys, rows of different lengths 40.8 -> 34.0.
 //
 // FRONT: a tile holds keys of one kind, and rows of it that are not visible are zeroed and masked.
-template <typename T, int D, bool PAGED, bool FEW, int FRONT = kNone>
-__global__ void __launch_bounds__(kGqaWarps * 32, 1) decode_gqa_kernel(const DecodeArgs a, int n_hgroups) {
-    grid_wait();
-    if (a.let_next_in) launch_dependents();
+//
+// WARPS per CTA: eight, or one beside the CTAs of another kernel (a.under).
+template <typename T, int D, bool PAGED, bool FEW, int FRONT = kNone, int WARPS = kGqaWarps>
+__global__ void __launch_bounds__(WARPS * 32, 1) decode_gqa_kernel(const DecodeArgs a, int n_hgroups) {
+    if (!a.under) grid_wait();
+    else if (blockIdx.x == gridDim.x - 1) {      // see decode_kernel
+        grid_wait();
+        return;
+    }
     constexpr int LD = D + 8;                       // padded row: ldmatrix without bank conflicts
     constexpr int REC = 2 * D + 4, CH = D / 32;
     constexpr int KS = D / 16;                      // k-steps of the score products
@@ -1027,13 +1035,13 @@ __global__ void __launch_bounds__(kGqaWarps * 32, 1) decode_gqa_kernel(const Dec
     constexpr int CPR = D / 8;                      // 16-byte chunks per row
     static_assert(16 * REC * 4 <= GqaSmem<D>::kPerWarp, "a warp's records fit where its tiles were");
     extern __shared__ __align__(16) unsigned char gqa_smem[];
-    __shared__ int s_row[kGqaWarps], s_arrived[kGqaWarps];   // batch row of each warp (-1: none); arrival order of its segment
+    __shared__ int s_row[WARPS], s_arrived[WARPS];   // batch row of each warp (-1: none); arrival order of its segment
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     // A CTA is eight adjacent slots of one (kv head, head group); heads are fastest over the grid, so CTAs that run
     // together read neighbouring memory.
     const int n_hunits = a.heads_kv * n_hgroups, n_slots = a.batch * a.n_splits;
-    const int hunit = blockIdx.x % n_hunits, cta = blockIdx.x / n_hunits, slot = cta * kGqaWarps + warp;
+    const int hunit = blockIdx.x % n_hunits, cta = blockIdx.x / n_hunits, slot = cta * WARPS + warp;
     const int hk = hunit / n_hgroups, hgrp = hunit % n_hgroups;
     SplitPlan plan{-1, 0, 0, 0, 0, 0};
     if (slot < n_slots) plan = a.balanced ? plan_slot<kGqaTile, FRONT>(a, slot, lane, n_slots) : plan_even<kGqaTile, FRONT>(a, slot / a.n_splits, slot % a.n_splits);
@@ -1373,9 +1381,9 @@ __global__ void __launch_bounds__(kGqaWarps * 32, 1) decode_gqa_kernel(const Dec
     __syncthreads();
     int w0 = warp, n_seg = 0;
     while (w0 > 0 && s_row[w0 - 1] == plan.b) --w0;
-    while (w0 + n_seg < kGqaWarps && s_row[w0 + n_seg] == plan.b) ++n_seg;
-    const int head_slot = slot - plan.part, first_cta = head_slot / kGqaWarps;
-    const int n_ctas = plan.b < 0 ? 0 : (head_slot + plan.n_parts - 1) / kGqaWarps - first_cta + 1;
+    while (w0 + n_seg < WARPS && s_row[w0 + n_seg] == plan.b) ++n_seg;
+    const int head_slot = slot - plan.part, first_cta = head_slot / WARPS;
+    const int n_ctas = plan.b < 0 ? 0 : (head_slot + plan.n_parts - 1) / WARPS - first_cta + 1;
     const bool alone = n_ctas == 1;
     auto bh_of = [&](int row) -> int64_t { return static_cast<int64_t>(b) * a.heads_q + hq0 + row; };
     auto recs_of = [&](int row) -> float * { return a.ws_parts + (plan.first + static_cast<int64_t>(hq0 + row) * plan.n_parts) * REC; };
@@ -1466,11 +1474,11 @@ __global__ void __launch_bounds__(kGqaWarps * 32, 1) decode_gqa_kernel(const Dec
     if (warp == w0 && lane == 0) a.ws_counters[bh_of(0)] = 0;   // ready for the next launch on this workspace
 }
 
-template <typename T, int D, bool PAGED, bool FEW, int FRONT>
+template <typename T, int D, bool PAGED, bool FEW, int FRONT, int WARPS = kGqaWarps>
 static int launch_decode_gqa(const DecodeArgs &a, cudaStream_t stream) {
     const int n_hgroups = (a.n_rep + 15) / 16;
-    constexpr int kSmem = kGqaWarps * GqaSmem<D>::kPerWarp;
-    auto kern = decode_gqa_kernel<T, D, PAGED, FEW, FRONT>;
+    constexpr int kSmem = WARPS * GqaSmem<D>::kPerWarp;
+    auto kern = decode_gqa_kernel<T, D, PAGED, FEW, FRONT, WARPS>;
     {   // the shared-memory opt-in is a per-device function attribute: set it once per device
         constexpr int kMaxDevices = 64;
         static std::mutex mu;
@@ -1486,8 +1494,8 @@ static int launch_decode_gqa(const DecodeArgs &a, cudaStream_t stream) {
             done[dev] = true;
         }
     }
-    const int64_t ctas = (static_cast<int64_t>(a.batch) * a.n_splits + kGqaWarps - 1) / kGqaWarps * a.heads_kv * n_hgroups;
-    const cudaError_t st = launch_overlapped(kern, dim3(static_cast<unsigned>(ctas)), kGqaWarps * 32, kSmem, stream, a, n_hgroups);
+    const int64_t ctas = (static_cast<int64_t>(a.batch) * a.n_splits + WARPS - 1) / WARPS * a.heads_kv * n_hgroups + (a.under ? 1 : 0);
+    const cudaError_t st = launch_overlapped(kern, dim3(static_cast<unsigned>(ctas)), WARPS * 32, kSmem, stream, a, n_hgroups);
     count_launch();
     return st == cudaSuccess && cudaGetLastError() == cudaSuccess ? PLX_OK : PLX_ERR_LAUNCH;
 }
@@ -1495,7 +1503,7 @@ static int launch_decode_gqa(const DecodeArgs &a, cudaStream_t stream) {
 template <typename T, int D, int HG>
 static int launch_decode_hg(const DecodeArgs &a, cudaStream_t stream) {
     constexpr int U = 4;  // key rows per stream and register buffer (two buffers: 8 rows of K and of V in flight)
-    dim3 grid(a.n_splits, a.heads_q / HG, a.batch);
+    dim3 grid(a.n_splits, a.heads_q / HG, a.batch + (a.under ? 1 : 0));
     // (with sinks the rows are as long as the window, most of them: never dealt out by length)
     auto kern = a.sink         ? decode_kernel<T, D, HG, U, false, false, kSinks>
                 : a.prefix_len ? decode_kernel<T, D, HG, U, false, false, kShared>
@@ -1594,8 +1602,18 @@ static int launch_decode_grouped(const DecodeArgs &a, cudaStream_t stream) {
     return a.n_rep > 8 ? launch_decode_gqa<T, D, false, false, FRONT>(a, stream) : launch_decode_gqa<T, D, false, true, FRONT>(a, stream);
 }
 
+// Beside a kernel that takes a CTA with most of the shared memory and registers of every SM: CTAs of a warp or two.
+template <typename T, int D>
+static int launch_decode_under(const DecodeArgs &a, cudaStream_t stream) {
+    if (a.n_rep == 1) return a.heads_q % 2 == 0 ? launch_decode_hg<T, D, 2>(a, stream) : launch_decode_hg<T, D, 1>(a, stream);
+    if (a.n_rep > 8)
+        return a.page_table ? launch_decode_gqa<T, D, true, false, kNone, 1>(a, stream) : launch_decode_gqa<T, D, false, false, kNone, 1>(a, stream);
+    return a.page_table ? launch_decode_gqa<T, D, true, true, kNone, 1>(a, stream) : launch_decode_gqa<T, D, false, true, kNone, 1>(a, stream);
+}
+
 template <typename T, int D>
 static int launch_decode_t(const DecodeArgs &a, cudaStream_t stream) {
+    if (a.under) return launch_decode_under<T, D>(a, stream);
     if (a.n_rep >= 2)    // grouped heads: tensor-core kernel
         return a.sink         ? launch_decode_grouped<T, D, kSinks>(a, stream)
                : a.prefix_len ? launch_decode_grouped<T, D, kShared>(a, stream)
@@ -1710,7 +1728,6 @@ int launch_decode_merge(const float *parts, int n_parts, int n_records, int head
 template <typename T, int D>
 __global__ void __launch_bounds__(128) prefix_merge_kernel(const float *parts, int n_parts, int64_t n_rows, void *out) {
     constexpr int REC = 2 * D + 4, CH = D / 32;
-    grid_wait();
     const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     if (row >= n_rows) return;
@@ -1739,9 +1756,10 @@ __global__ void __launch_bounds__(128) prefix_merge_kernel(const float *parts, i
 
 template <typename T, int D>
 static int launch_prefix_merge_t(const float *parts, int n_parts, int64_t n_rows, void *out, cudaStream_t stream) {
-    const cudaError_t st = launch_overlapped(prefix_merge_kernel<T, D>, dim3(static_cast<unsigned>((n_rows + 3) / 4)), 128, 0, stream, parts, n_parts, n_rows, out);
+    // (in the ordinary order of the stream: behind the prefix and behind the sweep that ran under it)
+    prefix_merge_kernel<T, D><<<static_cast<unsigned>((n_rows + 3) / 4), 128, 0, stream>>>(parts, n_parts, n_rows, out);
     count_launch();
-    return st == cudaSuccess && cudaGetLastError() == cudaSuccess ? PLX_OK : PLX_ERR_LAUNCH;
+    return cudaGetLastError() == cudaSuccess ? PLX_OK : PLX_ERR_LAUNCH;
 }
 
 int launch_prefix_merge(const float *parts, int n_parts, int64_t n_rows, int head_dim, int dtype, void *out, cudaStream_t stream) {

@@ -36,7 +36,7 @@ struct DecodeArgs {
     const void *k_prefix, *v_prefix;
     int prefix_len;
     int64_t prefix_st, prefix_sh;
-    int let_next_in;          // the next launch may begin under this one (it waits for its end by itself)
+    int under;                // runs under the launch before it, which has waited for what came before both
     float c2;  // qk_scale * log2(e)
     int64_t kv_sb, kv_st, kv_sh;   // paged: kv_sb is the stride between pages
     // paged cache (page_table != nullptr): key j of batch row b lives in page

@@ -243,6 +243,13 @@ fwd_sm100_kernel(const TrainArgs a, const __grid_constant__ CUtensorMap tm_q, co
     auto tP1 = [&](int pb) -> uint32_t { return kInPlace ? tS1(pb) : tmem_base + 384 + 64 * pb; };
     auto tP2 = [&](int pb) -> uint32_t { return kInPlace ? tS2(pb) : tmem_base + 384 + 64 * pb + 32; };
 
+    // A prefix sets itself up under the end of what came before it, and then lets in the sweep of the rows' own keys, which does not
+    // wait by itself: what it reads is complete now.
+    if (PART) {
+        grid_wait();
+        launch_dependents();
+    }
+
     // Items (`valid` = 0: no more).  DYN: the producer finds them ...
     const ItemRing ring{base + L::kItems, bar(L::kItemFull), bar(L::kItemEmpty)};
     struct Source {
@@ -625,7 +632,9 @@ fwd_sm100_kernel(const TrainArgs a, const __grid_constant__ CUtensorMap tm_q, co
                 for (int hh = 0; hh < 2; ++hh) {
                     const float m_tile = mx[hh] * a.c2;               // c2 > 0 (checked on the host)
                     m_true[hh] = fmaxf(m_true[hh], m_tile);
-                    grow[hh] = m_tile > m_ref[hh] + kRescaleThreshold;
+                    // (A prefix: rows behind the box hold what was in shared memory.  Nothing reads them, and left to grow their maxima
+                    // cost the warp a rescale a tile: 2 rows, 32 : 8 heads, 32000 keys 60.8 us.)
+                    grow[hh] = m_tile > m_ref[hh] + kRescaleThreshold && (!PART || rl0 + 8 * hh < a.box_h * a.box_b);
                 }
                 if (__any_sync(0xffffffffu, grow[0] || grow[1])) {
                     float alpha[2];
@@ -839,9 +848,6 @@ fwd_sm100_kernel(const TrainArgs a, const __grid_constant__ CUtensorMap tm_q, co
     tc_fence_before();
     __syncthreads();
     if (warp == 1) tmem_dealloc(tmem_base, kTmemCols);
-    // A prefix is launched under the end of the sweep of the rows' own keys.  What it reads was complete before that let it in; it
-    // ends behind it, so that whatever follows on the stream follows both.
-    if (PART) grid_wait();
 }
 
 // ------------------------------------------------------------------------- //
@@ -920,14 +926,11 @@ int launch_t(const TrainArgs &a, cudaStream_t stream) {
     if constexpr (PART) {
         static std::mutex mu;
         static bool done[tma::kMaxDevices] = {};
-        // A CTA per item: they take the SMs as the sweep before leaves them.  (Handed on from item to item a CTA asks for the next
-        // one when it begins one, and with about an item per SM the first SMs to be free keep two: 32 rows, 32 : 8 heads, 8192 keys
-        // 40 us against 24.)
         auto kern = fwd_sm100_kernel<T, D, NS, MODE, false>;
         if (!tma::opt_in_smem(kern, static_cast<int>(L::kBytes), done, mu)) return PLX_ERR_LAUNCH;
         const int n_rt = prefix_row_tiles(a.n_rep, a.batch), n = n_rt * a.heads_kv * a.n_splits;
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(n);
+        cfg.gridDim = dim3(n < sms ? n : sms);
         cfg.blockDim = dim3(352);
         cfg.dynamicSmemBytes = L::kBytes;
         cfg.stream = stream;
@@ -993,7 +996,7 @@ int launch_train_extend_sm100(const TrainArgs &a, int dtype, int head_dim, cudaS
     return a.sink ? launch_mode<kExtendSink>(a, dtype, head_dim, stream) : launch_mode<kExtend>(a, dtype, head_dim, stream);
 }
 
-// A prefix, behind a decode launch that lets it in early: as against a cache.  `a` holds q, r, the keys (dense: one row of len_k; paged: a row of the page table), `parts` and
+// A prefix, in front of a decode launch that runs under it: as against a cache.  `a` holds q, r, the keys (dense: one row of len_k; paged: a row of the page table), `parts` and
 // n_parts; n_splits is the caller's (see prefix_splits), box_h and box_b follow from the heads.
 int launch_prefix_sm100(const TrainArgs &problem, int dtype, int head_dim, cudaStream_t stream) {
     TrainArgs a = problem;

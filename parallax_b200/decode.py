@@ -310,9 +310,7 @@ def _prefix_core(q, r, k_prefix, v_prefix, prefix_len: int, k, v, scale, *, sequ
     k, v = _kv_pair(k, v)
     if k_prefix is not None:
         k_prefix, v_prefix = (x[0] for x in _kv_pair(k_prefix.unsqueeze(0), v_prefix.unsqueeze(0)))
-    prefix_splits = ops.choose_prefix_splits(bsz, hq, k.shape[2], prefix_len, d, q.device)
-    own_keys = ceiling - least
-    n_splits = split_count(q, k, -1, max(1, own_keys if prefix_splits else own_keys + prefix_len))
+    prefix_splits, n_splits = ops.plan_prefix(bsz, hq, k.shape[2], prefix_len, ceiling - least, d, q.device)
     ops.decode_prefix(q, r, k_prefix, v_prefix, prefix_len, k, v, out, _prefix_workspace(q, k, n_splits, prefix_splits, page_table),
                       float(1.0 / math.sqrt(d) if scale is None else scale), n_splits, prefix_splits, seqused_k, page_table)
     return out

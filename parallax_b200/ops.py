@@ -288,10 +288,15 @@ def _prefix(k_prefix: Optional[Tensor], v_prefix: Optional[Tensor], prefix_len: 
     return x
 
 
-def choose_prefix_splits(batch: int, heads_q: int, heads_kv: int, prefix_len: int, head_dim: int, device: torch.device) -> int:
-    """Parts of a shared prefix; 0 where it is faster for every row to sweep the prefix itself."""
+def plan_prefix(batch: int, heads_q: int, heads_kv: int, prefix_len: int, own_len: int, head_dim: int, device: torch.device) -> Tuple[int, int]:
+    """Parts of a shared prefix (0 where it is faster for every row to sweep it itself) and of a row's own keys
+    (``PLX_DECODE_SPLITS`` overrides the latter)."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
-    return int(_cabi.lib().plx_decode_prefix_splits(batch, heads_q, heads_kv, prefix_len, head_dim, sm_count(idx)))
+    splits, own = C.c_int32(0), C.c_int32(0)
+    _cabi.check(_cabi.lib().plx_decode_prefix_plan(batch, heads_q, heads_kv, prefix_len, own_len, head_dim, sm_count(idx), C.byref(splits),
+                                                   C.byref(own)), "plx_decode_prefix_plan")
+    env = os.environ.get("PLX_DECODE_SPLITS")
+    return splits.value, max(1, int(env)) if env else own.value
 
 
 def decode_prefix_workspace_bytes(q: Tensor, k: Tensor, n_splits: int, prefix_splits: int, page_table: Optional[Tensor]) -> int:

@@ -127,10 +127,21 @@ def test_decode_with_sinks_and_prefixes_at_the_abi():
 
 
 def test_how_a_prefix_is_split():
-    splits = lambda *a: _cabi.lib().plx_decode_prefix_splits(*a)                     # noqa: E731  batch, heads_q, heads_kv, len, head_dim, SMs
-    assert splits(4, 8, 8, 500, 128, 148) == 0 and splits(4, 8, 8, 2000, 128, 148) == 0       # every row by itself, in one launch
-    assert splits(16, 8, 8, 500, 128, 148) == 8 and splits(8, 8, 8, 1000, 128, 148) == 16     # at most one for 64 keys
-    assert splits(2, 32, 8, 16000, 128, 148) == 0 and splits(32, 32, 8, 8192, 128, 148) >= 8
-    assert 1 <= splits(128, 32, 8, 32768, 128, 148) <= 16
-    for b, hq, hkv, n in ((1, 1, 1, 1), (300, 64, 8, 100000), (64, 8, 1, 64), (64, 128, 1, 65), (10 ** 4, 32, 8, 10 ** 6)):
-        assert 0 <= splits(b, hq, hkv, n, 128, 148) <= min(127, -(-n // 64))
+    def plan(*a):                                                          # batch, heads_q, heads_kv, prefix, own keys, head_dim, SMs
+        x, y = C.c_int32(-1), C.c_int32(-1)
+        assert _cabi.lib().plx_decode_prefix_plan(*a, C.byref(x), C.byref(y)) == 0
+        return x.value, y.value
+
+    assert plan(4, 8, 8, 500, 40, 128, 148)[0] == 0 and plan(4, 8, 8, 1000, 40, 128, 148)[0] == 0      # every row by itself, in one launch
+    assert plan(1, 32, 8, 4000, 40, 128, 148)[0] == 0
+    assert 1 <= plan(16, 8, 8, 500, 40, 128, 148)[0] <= 8                  # at most one part for 64 keys
+    wide, own = plan(32, 32, 8, 8192, 512, 128, 148)
+    assert 8 <= wide <= 12 and own >= 1                                    # leaves SMs to the rows' own keys
+    assert 16 <= plan(32, 32, 8, 32768, 0, 128, 148)[0] <= 18              # where there are some
+    assert plan(128, 32, 8, 32768, 512, 128, 148)[0] == 4                  # one round of the SMs
+    for b, hq, hkv, n, t in ((1, 1, 1, 1, 0), (300, 64, 8, 100000, 10), (64, 8, 1, 64, 3), (64, 128, 1, 65, 70), (10 ** 4, 32, 8, 10 ** 6, 10 ** 6)):
+        parts, own = plan(b, hq, hkv, n, t, 128, 148)
+        assert 0 <= parts <= min(127, -(-n // 64)) and 1 <= own <= 256
+    one = C.c_int32(0)
+    for bad in ((0, 8, 8, 9, 0, 128, 148), (1, 4, 8, 9, 0, 128, 148), (1, 9, 2, 9, 0, 128, 148), (1, 8, 8, 0, 0, 128, 148), (1, 8, 8, 9, -1, 128, 148)):
+        assert _cabi.lib().plx_decode_prefix_plan(*bad, C.byref(one), C.byref(one)) == -1
