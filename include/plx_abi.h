@@ -272,8 +272,8 @@ int plx_decode_step_sink(const plx_decode_problem *p, int32_t sink_tokens, void 
  * cache of `p` itself: every row's page table begins with the same pages, len is a multiple of the page size, and lengths count
  * the prefix too (shorter ones count as len).  Only the first row's entries of it are read.  No sliding window, no kv_offset.
  * The q heads of a kv head of all rows are the M dimension of tensor-core products over the prefix, whose keys are cut into
- * n_splits parts (at most one for every 64 keys); each row's own keys are a plx_decode_partial that runs beside that, and a third launch merges.  n_splits 0, where
- * that is slower: one launch, in which every row sweeps the prefix in front of its own keys (p->n_splits is then for all of them).
+ * n_splits parts (at most one for every 64 keys); each row's own keys are a plx_decode_partial that runs beside that, and a
+ * third launch merges.  n_splits 0, where that is slower: one launch, in which every row sweeps the prefix in front of its own keys (p->n_splits is then for all of them).
  * Workspace: plx_decode_prefix_workspace_bytes(), ZERO-FILLED ONCE like that of plx_decode.  (No counterpart in the reference.) */
 #define PLX_PREFIX_MAX_SPLITS 127
 typedef struct plx_prefix {

@@ -997,7 +997,7 @@ int launch_train_extend_sm100(const TrainArgs &a, int dtype, int head_dim, cudaS
 }
 
 // A prefix, in front of a decode launch that runs under it: as against a cache.  `a` holds q, r, the keys (dense: one row of len_k; paged: a row of the page table), `parts` and
-// n_parts; n_splits is the caller's (see prefix_splits), box_h and box_b follow from the heads.
+// n_parts; n_splits is the caller's, box_h and box_b follow from the heads.
 int launch_prefix_sm100(const TrainArgs &problem, int dtype, int head_dim, cudaStream_t stream) {
     TrainArgs a = problem;
     prefix_boxes(a.n_rep, a.batch, a.box_h, a.box_b);
