@@ -367,6 +367,18 @@ def _extend_fused(q, r, k, v, scale, window_size_left, seqused_k, page_table, re
     return True
 
 
+def _without_hidden(k, v, lq, window_size_left, sink_tokens, ours):
+    """Keys and values (B, n, H_kv, D) for the last `lq` positions, with zeros between the sinks and the first window: what lies there
+    (pages of it may have gone to another sequence) must not be seen, not even as 0 * NaN.  `ours`: a copy that may be written."""
+    end = k.shape[1] - lq - window_size_left + 1
+    if sink_tokens == 0 or window_size_left < 0 or end <= sink_tokens:
+        return k, v
+    k, v = (k, v) if ours else (k.clone(), v.clone())
+    k[:, sink_tokens:end] = 0
+    v[:, sink_tokens:end] = 0
+    return k, v
+
+
 def _extend_core(q, r, k_cache, v_cache, *, page_table, seqused_k, window_size_left, scale, out, sink_tokens=0):
     """L_q > 1 queries against a cache through the training forward kernel: one launch for all rows
     (:func:`_extend_fused`).  Where that does not apply, rows that share an active length of a dense cache
@@ -409,7 +421,8 @@ def _extend_core(q, r, k_cache, v_cache, *, page_table, seqused_k, window_size_l
     if _extend_fused(q, r, ks, vs, scale, window_size_left, None if uniform else seqused_k, page_table, res, sink_tokens):
         return res
     if uniform:
-        o = _extend_dense(q, r, k_cache[:, :lens[0]], v_cache[:, :lens[0]], scale, window_size_left, sink_tokens)
+        kb, vb = _without_hidden(k_cache[:, :lens[0]], v_cache[:, :lens[0]], lq, window_size_left, sink_tokens, False)
+        o = _extend_dense(q, r, kb, vb, scale, window_size_left, sink_tokens)
         if out is None:
             return o
         out.copy_(o)
@@ -421,6 +434,7 @@ def _extend_core(q, r, k_cache, v_cache, *, page_table, seqused_k, window_size_l
             vb = v_cache.index_select(0, pages).reshape(1, -1, k_cache.shape[2], d)[:, :n]
         else:
             kb, vb = k_cache[b:b + 1, :n], v_cache[b:b + 1, :n]
+        kb, vb = _without_hidden(kb, vb, lq, window_size_left, sink_tokens, paged)
         res[b:b + 1].copy_(_extend_dense(q[b:b + 1], r[b:b + 1], kb, vb, scale, window_size_left, sink_tokens))
     return res
 

@@ -364,6 +364,27 @@ def test_extend_over_pages_that_are_too_small_for_a_tile():
     close(got, want, 2, "o")
 
 
+@pytest.mark.parametrize("lens", [[300, 151, 9], [300, 300, 300]])
+@pytest.mark.parametrize("page", [0, 1, 2, 4])
+def test_extend_without_its_own_kernel_sees_nothing_hidden(page, lens):
+    """Pages of fewer than 8 keys, and dense rows whose channels are not next to one another."""
+    t, lq, window, sinks = 300, 9, 20, 2
+    q, r = randn(3, lq, 4, 128, seed=1), randn(3, lq, 4, 128, scale=0.5, seed=2)
+    k, v = randn(3, t, 2, 128, seed=3), randn(3, t, 2, 128, seed=4)
+    want = decode_reference(q, r, k, v, lens, [0] * 3, window, sinks)
+    k, v = hide(k, lens, [0] * 3, window, sinks, lq), hide(v, lens, [0] * 3, window, sinks, lq)
+    table = None
+    if page:
+        k, v, table = paged(k, v, page)
+    else:
+        k, v = (x.transpose(2, 3).contiguous().transpose(2, 3) for x in (k, v))
+    before = k.clone(), v.clone()
+    got = plx.parallax_attn_with_kvcache(q, r, k, v, page_table=table, seqused_k=torch.tensor(lens, dtype=torch.int32, device="cuda"), window_size=window,
+                                         sink_tokens=sinks)
+    close(got, want, 2, "o")
+    assert all(torch.equal(x.view(torch.int16), y.view(torch.int16)) for x, y in zip((k, v), before))      # (bits: there are NaN)
+
+
 @pytest.mark.parametrize("hq,hkv", [(8, 8), (16, 4)])
 def test_graphed_decode(hq, hkv):
     b, t, d, window, sinks = 3, 700, 128, 90, 4
