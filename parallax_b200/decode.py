@@ -217,8 +217,7 @@ def parallax_attn_with_kvcache(q: torch.Tensor, r: torch.Tensor, k_cache: torch.
     And two the reference does not name:
 
     * ``sink_tokens = S`` -- the first S keys of a row stay visible behind ``window_size`` (without one it changes nothing).  What lies
-      between them and the window of a row's first query does not reach the output, so its pages may have gone to another sequence (with
-      ``L_q > 1`` where all rows are one launch: pages of at least 8 keys, no gradients).
+      between them and the window of a row's first query does not reach the output, so its pages may have gone to another sequence.
     * ``shared_prefix = P`` -- the caller's word that all rows of a paged cache begin with the same P keys in the same pages, as
       after :func:`parallax_fork_pages`: every row of ``page_table`` starts with the same ``P // page_size`` entries and holds at least
       those keys.  Single-token calls without a window then read the whole pages of the prefix once for all rows
