@@ -179,6 +179,37 @@ def test_captured_and_replayed_on_two_streams():
             close(out, reference(q, r, [torch.cat((kp, k[i, :n[i]])) for i in range(6)], [torch.cat((vp, v[i, :n[i]])) for i in range(6)]), 2, "o")
 
 
+@pytest.mark.parametrize("hq,hkv", [(8, 8), (3, 3), (16, 4), (32, 2)])
+@pytest.mark.parametrize("p,t,prefix_splits,n_splits", [(30000, 1, 2, 1), (30000, 40, 18, 2), (130, 6000, 1, 1), (4000, 3000, 9, 8)])
+def test_whichever_ends_first(hq, hkv, p, t, prefix_splits, n_splits):
+    """Own keys are swept beside the prefix: the merge, and what follows it, come behind both, captured too.  Inputs that change between
+    the calls show a merge of records of the call before."""
+    b, d = 4, 128
+    sets = [make(b, hq, hkv, d, BF, p, t, seed=7 * i) for i in range(2)]
+    ins = [x.clone() for x in sets[0]]
+    q, r, kp, vp, k, v = ins
+    out, after = torch.empty_like(q), torch.empty_like(q)
+    ws = torch.zeros(ops.decode_prefix_workspace_bytes(q, k, n_splits, prefix_splits, None) // 4, device="cuda")
+
+    def call():
+        ops.decode_prefix(q, r, kp, vp, p, k, v, out, ws, d ** -0.5, n_splits, prefix_splits, None, None)
+        after.copy_(out)
+        out.zero_()
+
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with no_collection(), torch.cuda.graph(graph):
+        call()
+    want = [reference(x[0], x[1], [torch.cat((x[2], x[4][i])) for i in range(b)], [torch.cat((x[3], x[5][i])) for i in range(b)]) for x in sets]
+    for run in (call, graph.replay):
+        for i in range(6):
+            for x, y in zip(ins, sets[i % 2]):
+                x.copy_(y)
+            run()
+            close(after, want[i % 2], 2, "o")
+
+
 def test_two_threads_on_two_streams():
     """Eager calls of one shape at once: a workspace for each stream."""
     import threading
