@@ -268,7 +268,7 @@ int plx_decode_step_sink(const plx_decode_problem *p, int32_t sink_tokens, void 
 
 /* plx_decode for a batch whose rows all begin with the same `len` keys, which are read once for all of them.  The prefix
  * is either keys of its own, (len, heads_kv, head_dim) by the element strides (token, head) of k / v -- `p` then describes what
- * follows it, and lengths (seqused_k, 0 to cache_len, NULL: cache_len) count that -- or, with k and v NULL, the first len keys of the paged
+ * follows it, a dense cache (a paged one: PLX_ERR_UNSUPPORTED), and lengths (seqused_k, 0 to cache_len, NULL: cache_len) count that -- or, with k and v NULL, the first len keys of the paged
  * cache of `p` itself: every row's page table begins with the same pages, len is a multiple of the page size, and lengths count
  * the prefix too (shorter ones count as len).  Only the first row's entries of it are read.  No sliding window, no kv_offset.
  * The q heads of a kv head of all rows are the M dimension of tensor-core products over the prefix, whose keys are cut into

@@ -247,6 +247,7 @@ static int check_prefix(const plx_decode_problem *p, const plx_prefix *x) {
     if (!x->k)        // in the pages of the cache
         return p->page_table && p->n_pages > 0 && !x->v && x->len % p->page_size == 0 && x->len <= p->cache_len ? PLX_OK : PLX_ERR_BAD_ARG;
     if (!x->v || misaligned16(x->k) || misaligned16(x->v)) return PLX_ERR_BAD_ARG;
+    if (p->page_table) return PLX_ERR_UNSUPPORTED;      // the kernels of kShared have no page table behind the prefix
     return x->stride_t >= 0 && x->stride_h >= 0 && (x->stride_t & 7) == 0 && (x->stride_h & 7) == 0 ? PLX_OK : PLX_ERR_BAD_ARG;
 }
 
