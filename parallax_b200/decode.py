@@ -366,6 +366,15 @@ def _extend_fused(q, r, k, v, scale, window_size_left, seqused_k, page_table, re
     return True
 
 
+def _gathered(pool, pages):
+    """The keys of `pages` (int32) one after the other, (1, n, H_kv, D), in a copy that may be written.  What is not a page of the pool
+    reads as zeros, as in the launch for all rows: entries that no query sees may hold anything, and an index out of range would end the
+    context."""
+    inside = (pages >= 0) & (pages < pool.shape[0])
+    keys = pool.index_select(0, torch.where(inside, pages, 0)).masked_fill_(~inside[:, None, None, None], 0)
+    return keys.reshape(1, -1, *pool.shape[2:])
+
+
 def _without_hidden(k, v, lq, window_size_left, sink_tokens, ours):
     """Keys and values (B, n, H_kv, D) for the last `lq` positions, with zeros between the sinks and the first window: what lies there
     (pages of it may have gone to another sequence) must not be seen, not even as 0 * NaN.  `ours`: a copy that may be written."""
@@ -428,9 +437,8 @@ def _extend_core(q, r, k_cache, v_cache, *, page_table, seqused_k, window_size_l
         return out
     for b, n in enumerate(lens):
         if paged:
-            pages = page_table[b, :(n + page - 1) // page].long()
-            kb = k_cache.index_select(0, pages).reshape(1, -1, k_cache.shape[2], d)[:, :n]
-            vb = v_cache.index_select(0, pages).reshape(1, -1, k_cache.shape[2], d)[:, :n]
+            pages = page_table[b, :(n + page - 1) // page]
+            kb, vb = _gathered(k_cache, pages)[:, :n], _gathered(v_cache, pages)[:, :n]
         else:
             kb, vb = k_cache[b:b + 1, :n], v_cache[b:b + 1, :n]
         kb, vb = _without_hidden(kb, vb, lq, window_size_left, sink_tokens, paged)

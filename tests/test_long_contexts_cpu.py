@@ -18,3 +18,18 @@ def test_a_prefix_of_its_own_in_front_of_pages_is_refused(splits, scale):
     one = C.c_void_p(1 << 20)
     call = lambda p: _cabi.lib().plx_decode_prefix(C.byref(p), C.byref(prefix(n_splits=splits)), *[one] * 6, one, 1 << 30, None)    # noqa: E731
     assert call(decode_problem(qk_scale=scale, **PAGED)) == _cabi.PLX_ERR_UNSUPPORTED
+
+
+def test_gathered_pages_outside_the_pool_read_as_zeros():
+    """-1 is what forking writes where there was no page, and an entry that no query sees may hold any number."""
+    from parallax_b200.decode import _gathered
+
+    pool = torch.randn(5, 2, 3, 8, requires_grad=True)
+    pages = torch.tensor([4, -1, 0, 5, 2 ** 31 - 1, -2 ** 31, 3], dtype=torch.int32)
+    got = _gathered(pool, pages)
+    assert got.shape == (1, 14, 3, 8)
+    for i, page in enumerate(pages.tolist()):
+        want = pool[page] if 0 <= page < 5 else torch.zeros(2, 3, 8)
+        assert torch.equal(got[0, 2 * i:2 * i + 2], want)
+    got.sum().backward()
+    assert torch.equal(pool.grad, torch.tensor([1., 0., 0., 1., 1.])[:, None, None, None].expand_as(pool))
