@@ -23,7 +23,7 @@ def _check_cuda(name: str, *tensors: torch.Tensor) -> None:
 
 
 def check_sinks(name: str, sink_tokens: int) -> None:
-    if sink_tokens < 0 or sink_tokens > 2 ** 31 - 1:
+    if not 0 <= sink_tokens <= 2 ** 31 - 1 or sink_tokens != int(sink_tokens):
         raise ValueError(f"{name}: sink_tokens must be a number of tokens, got {sink_tokens}")
 
 

@@ -33,3 +33,18 @@ def test_gathered_pages_outside_the_pool_read_as_zeros():
         assert torch.equal(got[0, 2 * i:2 * i + 2], want)
     got.sum().backward()
     assert torch.equal(pool.grad, torch.tensor([1., 0., 0., 1., 1.])[:, None, None, None].expand_as(pool))
+
+
+@pytest.mark.parametrize("call", [
+    lambda n: plx.parallax_func(z(1, 2, 8, 64), z(1, 2, 8, 64), z(1, 2, 8, 64), z(1, 2, 8, 64), window_size_left=4, sink_tokens=n),
+    lambda n: plx.parallax_varlen_func(z(1, 8, 2, 64), z(1, 8, 2, 64), z(1, 8, 2, 64), z(1, 8, 2, 64), window_size_left=4, sink_tokens=n),
+    lambda n: plx.parallax_fwd(z(2, 8, 64), z(2, 8, 64), z(2, 8, 64), z(2, 8, 64), 0.1, sink_tokens=n),
+    lambda n: plx.parallax_bwd(*[z(2, 8, 64)] * 6, *[z(2, 8, 1)] * 3, z(2, 8, 64), 0.1, sink_tokens=n),
+    lambda n: plx.parallax_decode(z(2, 1, 4, 64), z(2, 1, 4, 64), z(2, 8, 2, 64), z(2, 8, 2, 64), window_size_left=4, sink_tokens=n),
+    lambda n: plx.parallax_attn_with_kvcache(z(2, 1, 4, 64), z(2, 1, 4, 64), z(2, 8, 2, 64), z(2, 8, 2, 64), window_size=4, sink_tokens=n),
+    lambda n: plx.GraphedDecode(2, 4, 8, 64, window_size=4, sink_tokens=n),
+], ids=["func", "varlen", "fwd", "bwd", "decode", "attn", "graphed"])
+@pytest.mark.parametrize("sinks", [4.5, 0.5, float("nan"), float("inf"), -1, 2 ** 31])
+def test_sinks_that_are_no_number_of_tokens(call, sinks):
+    with pytest.raises(ValueError, match="sink_tokens must be a number of tokens"):
+        call(sinks)
