@@ -48,3 +48,21 @@ def test_gathered_pages_outside_the_pool_read_as_zeros():
 def test_sinks_that_are_no_number_of_tokens(call, sinks):
     with pytest.raises(ValueError, match="sink_tokens must be a number of tokens"):
         call(sinks)
+
+
+def plan(*a):                                                              # batch, heads_q, heads_kv, prefix, room for own keys, head_dim, SMs
+    x, y = C.c_int32(-1), C.c_int32(-1)
+    assert _cabi.lib().plx_decode_prefix_plan(*a, C.byref(x), C.byref(y)) == 0
+    return x.value, y.value
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("b,hq,hkv,p", [(128, 32, 8, 32768), (32, 32, 8, 8192), (16, 8, 1, 16000), (16, 32, 8, 32768), (100, 28, 4, 5000), (64, 16, 2, 16000),
+                                        (8, 8, 8, 4000), (12, 16, 16, 6000)])
+def test_room_behind_a_prefix_is_not_taken_for_keys(b, hq, hkv, p, d):
+    """A page table or a buffer is as wide as the longest row may grow: the prefix stays shared, in about as many parts as without room."""
+    tight = plan(b, hq, hkv, p, 512, d, 148)[0]
+    assert tight > 0
+    for room in (1024, 2048, 8192, 65536, 131072 - p, 2 ** 31 - 1 - p):
+        parts, own = plan(b, hq, hkv, p, room, d, 148)
+        assert tight / 2 <= parts <= 2 * tight and 1 <= own <= 32, room

@@ -4,6 +4,7 @@ import torch
 
 import parallax_b200 as plx
 from parallax_b200 import _cabi
+from tests.test_prefix_gpu import make, pages_of, reference
 from tests.test_sinks_gpu import close, decode_reference, hide, paged, randn
 
 pytestmark = pytest.mark.gpu
@@ -35,3 +36,26 @@ def test_extend_over_a_table_without_its_hidden_pages(page, recorded, scale, now
         dq, = torch.autograd.grad(got, q, torch.ones_like(got))
         assert torch.isfinite(dq).all() and dq.abs().max() > 0
     assert _cabi.device_error() == 0
+
+
+@pytest.mark.parametrize("hq,hkv,d,p,room,page", [(32, 8, 128, 2048, 20000, 0), (32, 8, 128, 2048, 20000, 16), (8, 8, 64, 3000, 9000, 0), (8, 1, 128, 4096, 6000, 64),
+                                                  (8, 8, 128, 2048, 3000, 2), (16, 4, 64, 640, 1500, 1)])
+def test_a_prefix_in_front_of_rows_with_room(hq, hkv, d, p, room, page):
+    """Buffers and tables many times as wide as what the rows hold, of which all but that is NaN or no page."""
+    lens = [300, 0, 1, 77, 2, 900, 64, 65]
+    b = len(lens)
+    q, r, kp, vp, k, v = make(b, hq, hkv, d, BF, p, max(lens))
+    want = reference(q, r, [torch.cat((kp, k[i, :n])) for i, n in enumerate(lens)], [torch.cat((vp, v[i, :n])) for i, n in enumerate(lens)])
+    if page:
+        pools_k, pools_v, table = pages_of(kp, vp, k, v, lens, page)
+        table = torch.nn.functional.pad(table, (0, room // page), value=-1)
+        call = lambda: plx.parallax_attn_with_kvcache(q, r, pools_k, pools_v, page_table=table, seqused_k=ints([p + n for n in lens]), shared_prefix=p)  # noqa: E731
+    else:
+        wide = [torch.full((b, room, hkv, d), torch.nan, dtype=BF, device="cuda") for _ in range(2)]
+        for x, y in zip(wide, (k, v)):
+            for i, n in enumerate(lens):
+                x[i, :n] = y[i, :n]
+        call = lambda: plx.parallax_decode_shared_prefix(q, r, kp, vp, *wide, seqused_k=ints(lens))        # noqa: E731
+    got = call()
+    close(got, want, 2, "o")
+    assert torch.equal(call(), got) and _cabi.device_error() == 0
