@@ -285,6 +285,9 @@ typedef struct plx_prefix {
 /* n_splits of plx_prefix and of the problem, for own keys of up to own_len a row.  Pure host arithmetic. */
 int plx_decode_prefix_plan(int32_t batch, int32_t heads_q, int32_t heads_kv, int32_t len, int32_t own_len, int32_t head_dim,
                            int32_t sm_count, int32_t *prefix_splits, int32_t *own_splits);
+/* The same for the call that `p` and `x` describe (their n_splits are not looked at): 0 and the splits of all keys where no shared
+ * kernel takes it (pages of fewer than 8 keys, scales <= 0, strides of 0, 65535 rows). */
+int plx_decode_prefix_plan_call(const plx_decode_problem *p, const plx_prefix *x, int32_t sm_count, int32_t *prefix_splits, int32_t *own_splits);
 int plx_decode_prefix_workspace_bytes(const plx_decode_problem *p, const plx_prefix *x, size_t *bytes);
 int plx_decode_prefix(const plx_decode_problem *p, const plx_prefix *x, const void *q, const void *r, const void *k,
                       const void *v, void *out, const int32_t *seqused_k, void *workspace, size_t workspace_bytes,

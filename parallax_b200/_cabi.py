@@ -26,7 +26,7 @@ SYMBOLS = (
     "plx_decode_choose_splits", "plx_decode_choose_splits_gqa", "plx_decode_workspace_bytes", "plx_decode_stage", "plx_decode_step", "plx_decode", "plx_decode_static", "plx_decode_partial",
     "plx_decode_merge", "plx_decode_exchange_bytes", "plx_decode_exchange_merge", "plx_decode_partial_exchange",
     "plx_train_workspace_bytes_sink", "plx_train_fwd_sink", "plx_train_extend_sink", "plx_train_bwd_sink",
-    "plx_decode_sink", "plx_decode_step_sink", "plx_decode_prefix_plan", "plx_decode_prefix_workspace_bytes", "plx_decode_prefix",
+    "plx_decode_sink", "plx_decode_step_sink", "plx_decode_prefix_plan", "plx_decode_prefix_plan_call", "plx_decode_prefix_workspace_bytes", "plx_decode_prefix",
     "plx_pages_copy", "plx_pages_workspace_bytes", "plx_pages_fork", "plx_pages_compact", "plx_pages_free",
 )
 EXCHANGE_MAX_RANKS = 16
@@ -150,6 +150,8 @@ def _declare(lib):
     lib.plx_decode_step_sink.argtypes = [decode, i32] + [vp] * 9 + [vp, sz, vp]
     lib.plx_decode_prefix_plan.restype = C.c_int
     lib.plx_decode_prefix_plan.argtypes = [i32] * 7 + [C.POINTER(i32), C.POINTER(i32)]
+    lib.plx_decode_prefix_plan_call.restype = C.c_int
+    lib.plx_decode_prefix_plan_call.argtypes = [decode, prefix, i32, C.POINTER(i32), C.POINTER(i32)]
     lib.plx_decode_prefix_workspace_bytes.restype = C.c_int
     lib.plx_decode_prefix_workspace_bytes.argtypes = [decode, prefix, C.POINTER(sz)]
     lib.plx_decode_prefix.restype = C.c_int

@@ -252,6 +252,29 @@ static int check_prefix(const plx_decode_problem *p, const plx_prefix *x) {
     return x->stride_t >= 0 && x->stride_h >= 0 && (x->stride_t & 7) == 0 && (x->stride_h & 7) == 0 ? PLX_OK : PLX_ERR_BAD_ARG;
 }
 
+constexpr int kMostRows = 65535;      // rows of a shared launch are fewer: the sweep of own keys has one more CTA than they need
+
+// a batch's rows against their prefix, but for pointers to q, r and keys
+static TrainArgs make_prefix_args(const plx_decode_problem *p, const plx_prefix *x) {
+    const bool in_cache = !x->k;                       // the rows' own page tables begin with the prefix
+    TrainArgs a{};
+    a.batch = p->batch; a.heads_q = p->heads_q; a.heads_kv = p->heads_kv; a.n_rep = p->heads_q / p->heads_kv;
+    a.len_q = 1; a.len_k = x->len;
+    a.window = -1;
+    a.scale = p->qk_scale;
+    a.c2 = p->qk_scale * kLog2e;
+    a.q_st = p->head_dim; a.q_sh = static_cast<int64_t>(a.n_rep) * p->head_dim; a.q_sb = static_cast<int64_t>(p->heads_q) * p->head_dim;
+    a.kv_sb = in_cache ? p->kv_stride_b : x->stride_t; a.kv_st = in_cache ? p->kv_stride_t : x->stride_t; a.kv_sh = in_cache ? p->kv_stride_h : x->stride_h;
+    if (in_cache) {
+        a.page_table = p->page_table;
+        a.pages_per_seq = p->pages_per_seq;
+        a.n_pages = p->n_pages;
+        a.page_mask = p->page_size - 1;
+        while ((1 << a.page_shift) < p->page_size) ++a.page_shift;
+    }
+    return a;
+}
+
 // the backward: the chosen stages (all of them with sinks)
 static int run_train_bwd(const plx_train_problem *p, int32_t sink_tokens, int32_t stages, const void *q, const void *r, const void *k, const void *v,
                          const void *o, const void *barv, const float *d1, const float *bart, const float *m, const void *grad_o, void *dq, void *dr,
@@ -659,6 +682,23 @@ int plx_decode_prefix_plan(int32_t batch, int32_t heads_q, int32_t heads_kv, int
     return PLX_OK;
 }
 
+int plx_decode_prefix_plan_call(const plx_decode_problem *p, const plx_prefix *x, int32_t sm_count, int32_t *prefix_splits, int32_t *own_splits) {
+    if (!p || !x || sm_count <= 0 || !prefix_splits || !own_splits) return PLX_ERR_BAD_ARG;
+    plx_decode_problem problem = *p;
+    plx_prefix prefix = *x;
+    problem.n_splits = 1;
+    prefix.n_splits = 0;
+    int st = check_decode(&problem);
+    if (st == PLX_OK) st = check_prefix(&problem, &prefix);
+    if (st != PLX_OK) return st;
+    const int64_t keys = x->k ? static_cast<int64_t>(x->len) + p->cache_len : p->cache_len;
+    if (p->batch < kMostRows && train_extend_sm100_fits(make_prefix_args(p, x), p->head_dim))
+        return plx_decode_prefix_plan(p->batch, p->heads_q, p->heads_kv, x->len, static_cast<int32_t>(keys - x->len), p->head_dim, sm_count, prefix_splits, own_splits);
+    *prefix_splits = 0;
+    *own_splits = plx_decode_choose_splits_gqa(p->batch, p->heads_q, p->heads_kv, static_cast<int32_t>(keys < INT32_MAX ? keys : INT32_MAX), sm_count);
+    return PLX_OK;
+}
+
 int plx_decode_prefix_workspace_bytes(const plx_decode_problem *p, const plx_prefix *x, size_t *bytes) {
     int st = check_decode(p);
     if (st != PLX_OK) return st;
@@ -679,29 +719,15 @@ int plx_decode_prefix(const plx_decode_problem *p, const plx_prefix *x, const vo
     float *parts = static_cast<float *>(workspace);
     unsigned char *rest = static_cast<unsigned char *>(workspace) + part_bytes;
     const size_t rest_bytes = workspace_bytes - part_bytes;
-    const bool in_cache = !x->k;                       // the rows' own page tables begin with the prefix
-    TrainArgs a{};
+    const bool in_cache = !x->k;
+    TrainArgs a = make_prefix_args(p, x);
     a.q = q; a.r = r;
     a.k = in_cache ? k : x->k;
     a.v = in_cache ? v : x->v;
-    a.batch = p->batch; a.heads_q = p->heads_q; a.heads_kv = p->heads_kv; a.n_rep = p->heads_q / p->heads_kv;
-    a.len_q = 1; a.len_k = x->len;
-    a.window = -1;
-    a.scale = p->qk_scale;
-    a.c2 = p->qk_scale * kLog2e;
-    a.q_st = p->head_dim; a.q_sh = static_cast<int64_t>(a.n_rep) * p->head_dim; a.q_sb = static_cast<int64_t>(p->heads_q) * p->head_dim;
-    a.kv_sb = in_cache ? p->kv_stride_b : x->stride_t; a.kv_st = in_cache ? p->kv_stride_t : x->stride_t; a.kv_sh = in_cache ? p->kv_stride_h : x->stride_h;
-    if (in_cache) {
-        a.page_table = p->page_table;
-        a.pages_per_seq = p->pages_per_seq;
-        a.n_pages = p->n_pages;
-        a.page_mask = p->page_size - 1;
-        while ((1 << a.page_shift) < p->page_size) ++a.page_shift;
-    }
     a.parts = parts;
     Sweep own;
     own.first_key = own.min_len = 0;
-    if (x->n_splits == 0 || p->batch == 65535 || !train_extend_sm100_supported(a, p->head_dim)) {      // (65535: no room for the sweep's one more)
+    if (x->n_splits == 0 || p->batch == kMostRows || !train_extend_sm100_supported(a, p->head_dim)) {
         // every row sweeps the prefix in front of its own keys, in one launch
         if (in_cache) own.min_len = x->len;
         else own.prefix = x;

@@ -966,13 +966,14 @@ int launch_t(const TrainArgs &a, cudaStream_t stream) {
 
 }  // namespace
 
-bool train_fwd_sm100_supported(const TrainArgs &a, int head_dim) {
+static bool train_fwd_sm100_fits(const TrainArgs &a, int head_dim) {
     if ((head_dim != 64 && head_dim != 128) || (a.window == 0 && a.sink == 0) || !(a.c2 > 0.f)) return false;
     // TMA needs 16-byte aligned strides; the ABI already guarantees multiples of 8 elements
     const char *env = std::getenv("PLX_FWD_KERNEL");
-    if (env && env[0] == 'm') return false;  // "mma": force the warp-level kernels
-    return tma::encode_fn() != nullptr;
+    return !env || env[0] != 'm';            // "mma": force the warp-level kernels
 }
+
+bool train_fwd_sm100_supported(const TrainArgs &a, int head_dim) { return train_fwd_sm100_fits(a, head_dim) && tma::encode_fn() != nullptr; }
 
 template <int MODE>
 static int launch_mode(const TrainArgs &a, int dtype, int head_dim, cudaStream_t stream) {
@@ -987,10 +988,12 @@ int launch_train_fwd_sm100(const TrainArgs &a, int dtype, int head_dim, cudaStre
 
 // Against a cache: any key range the forward takes; pages from 8 keys on (below that a box would not start on
 // the 1024-byte swizzle period of its tile), and strides a tensor map can express (no broadcast axes).
-bool train_extend_sm100_supported(const TrainArgs &a, int head_dim) {
+bool train_extend_sm100_fits(const TrainArgs &a, int head_dim) {
     if (a.kv_sb <= 0 || a.kv_sh <= 0 || a.kv_st <= 0 || (a.page_table && a.page_mask + 1 < kMinPage)) return false;
-    return train_fwd_sm100_supported(a, head_dim);
+    return train_fwd_sm100_fits(a, head_dim);
 }
+
+bool train_extend_sm100_supported(const TrainArgs &a, int head_dim) { return train_extend_sm100_fits(a, head_dim) && tma::encode_fn() != nullptr; }
 
 int launch_train_extend_sm100(const TrainArgs &a, int dtype, int head_dim, cudaStream_t stream) {
     return a.sink ? launch_mode<kExtendSink>(a, dtype, head_dim, stream) : launch_mode<kExtend>(a, dtype, head_dim, stream);

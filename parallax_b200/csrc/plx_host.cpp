@@ -52,7 +52,7 @@ struct Api {
     decltype(&plx_decode_choose_splits_gqa) decode_choose_splits_gqa;
     decltype(&plx_decode_workspace_bytes) decode_workspace_bytes;
     decltype(&plx_decode_sink) decode;
-    decltype(&plx_decode_prefix_plan) decode_prefix_plan;
+    decltype(&plx_decode_prefix_plan_call) decode_prefix_plan;
     decltype(&plx_decode_prefix_workspace_bytes) decode_prefix_workspace_bytes;
     decltype(&plx_decode_prefix) decode_prefix;
     decltype(&plx_pages_workspace_bytes) pages_workspace_bytes;
@@ -78,7 +78,7 @@ void bind(const py::dict &addresses) {
     bind_one(api.decode_choose_splits_gqa, addresses, "plx_decode_choose_splits_gqa");
     bind_one(api.decode_workspace_bytes, addresses, "plx_decode_workspace_bytes");
     bind_one(api.decode, addresses, "plx_decode_sink");
-    bind_one(api.decode_prefix_plan, addresses, "plx_decode_prefix_plan");
+    bind_one(api.decode_prefix_plan, addresses, "plx_decode_prefix_plan_call");
     bind_one(api.decode_prefix_workspace_bytes, addresses, "plx_decode_prefix_workspace_bytes");
     bind_one(api.decode_prefix, addresses, "plx_decode_prefix");
     bind_one(api.pages_workspace_bytes, addresses, "plx_pages_workspace_bytes");
@@ -605,8 +605,7 @@ py::object decode_prefix(const py::object &q_, const py::object &r_, const py::o
     const int sms = at::cuda::getDeviceProperties(q.get_device())->multiProcessorCount;
     plx_decode_problem p = decode_problem(q, k, ceiling, table, scale, -1, 1);
     x.len = static_cast<int32_t>(prefix_len);
-    if (api.decode_prefix_plan(p.batch, p.heads_q, p.heads_kv, x.len, static_cast<int32_t>(ceiling - least), p.head_dim, sms, &x.n_splits, &p.n_splits) != PLX_OK)
-        return py::none();
+    if (api.decode_prefix_plan(&p, &x, sms, &x.n_splits, &p.n_splits) != PLX_OK) return py::none();
     size_t need = 0;
     if (api.decode_prefix_workspace_bytes(&p, &x, &need) != PLX_OK) return py::none();
     const Tensor ws = workspaces().get(stream, q, p.n_splits, static_cast<int64_t>(need / sizeof(float)), x.n_splits);

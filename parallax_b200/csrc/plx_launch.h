@@ -49,6 +49,7 @@ bool train_fwd_sm100_supported(const TrainArgs &a, int head_dim);
 int launch_train_fwd_sm100(const TrainArgs &a, int dtype, int head_dim, cudaStream_t stream);
 // the same kernel for several query rows per sequence against a dense or paged KV cache (writes `o` only)
 bool train_extend_sm100_supported(const TrainArgs &a, int head_dim);
+bool train_extend_sm100_fits(const TrainArgs &a, int head_dim);      // without asking for the driver
 int launch_train_extend_sm100(const TrainArgs &a, int dtype, int head_dim, cudaStream_t stream);
 // Rows of a tile of the prefix kernel: box_h q heads of a kv head by box_b batch rows, 128 at most.
 inline void prefix_boxes(int n_rep, int batch, int &box_h, int &box_b) {

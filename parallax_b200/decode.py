@@ -309,9 +309,10 @@ def _prefix_core(q, r, k_prefix, v_prefix, prefix_len: int, k, v, scale, *, sequ
     k, v = _kv_pair(k, v)
     if k_prefix is not None:
         k_prefix, v_prefix = (x[0] for x in _kv_pair(k_prefix.unsqueeze(0), v_prefix.unsqueeze(0)))
-    prefix_splits, n_splits = ops.plan_prefix(bsz, hq, k.shape[2], prefix_len, ceiling - least, d, q.device)
+    scale = float(1.0 / math.sqrt(d) if scale is None else scale)
+    prefix_splits, n_splits = ops.plan_prefix(q, k, k_prefix, v_prefix, prefix_len, scale, page_table)
     ops.decode_prefix(q, r, k_prefix, v_prefix, prefix_len, k, v, out, _prefix_workspace(q, k, n_splits, prefix_splits, page_table),
-                      float(1.0 / math.sqrt(d) if scale is None else scale), n_splits, prefix_splits, seqused_k, page_table)
+                      scale, n_splits, prefix_splits, seqused_k, page_table)
     return out
 
 

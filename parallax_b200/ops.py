@@ -288,13 +288,15 @@ def _prefix(k_prefix: Optional[Tensor], v_prefix: Optional[Tensor], prefix_len: 
     return x
 
 
-def plan_prefix(batch: int, heads_q: int, heads_kv: int, prefix_len: int, own_len: int, head_dim: int, device: torch.device) -> Tuple[int, int]:
-    """Parts of a shared prefix (0 where it is faster for every row to sweep it itself) and of a row's own keys
-    (``PLX_DECODE_SPLITS`` overrides the latter)."""
-    idx = device.index if device.index is not None else torch.cuda.current_device()
+def plan_prefix(q: Tensor, k: Tensor, k_prefix: Optional[Tensor], v_prefix: Optional[Tensor], prefix_len: int, qk_scale: float,
+                page_table: Optional[Tensor]) -> Tuple[int, int]:
+    """Parts of a shared prefix (0 where it is faster for every row to sweep it itself, or there is no shared kernel) and of a row's own
+    keys (``PLX_DECODE_SPLITS`` overrides the latter)."""
+    p, x = _decode_problem(q, k, qk_scale, -1, 1, 0, 0, page_table), _prefix(k_prefix, v_prefix, prefix_len, 0)
+    idx = q.device.index if q.device.index is not None else torch.cuda.current_device()
     splits, own = C.c_int32(0), C.c_int32(0)
-    _cabi.check(_cabi.lib().plx_decode_prefix_plan(batch, heads_q, heads_kv, prefix_len, own_len, head_dim, sm_count(idx), C.byref(splits),
-                                                   C.byref(own)), "plx_decode_prefix_plan")
+    _cabi.check(_cabi.lib().plx_decode_prefix_plan_call(C.byref(p), C.byref(x), sm_count(idx), C.byref(splits), C.byref(own)),
+                "plx_decode_prefix_plan_call")
     env = os.environ.get("PLX_DECODE_SPLITS")
     return splits.value, max(1, int(env)) if env else own.value
 

@@ -66,3 +66,39 @@ def test_room_behind_a_prefix_is_not_taken_for_keys(b, hq, hkv, p, d):
     for room in (1024, 2048, 8192, 65536, 131072 - p, 2 ** 31 - 1 - p):
         parts, own = plan(b, hq, hkv, p, room, d, 148)
         assert tight / 2 <= parts <= 2 * tight and 1 <= own <= 32, room
+
+
+@pytest.mark.parametrize("b,hq,hkv,n", [(16, 32, 8, 32768), (4, 8, 8, 32768), (128, 32, 8, 32768), (2, 8, 1, 4096)])
+def test_splits_where_there_is_no_shared_kernel(b, hq, hkv, n):
+    """Every row sweeps the prefix itself there: its splits are those of a call of all keys, not those of its own ones beside a prefix."""
+    room = 512
+
+    def call(x, **kw):
+        parts, own = C.c_int32(-1), C.c_int32(-1)
+        p = decode_problem(batch=b, heads_q=hq, heads_kv=hkv, kv_stride_t=hkv * 128, **kw)
+        assert _cabi.lib().plx_decode_prefix_plan_call(C.byref(p), C.byref(x), 148, C.byref(parts), C.byref(own)) == 0
+        return parts.value, own.value
+
+    def paged(page):
+        return dict(page_table=1 << 20, page_size=page, pages_per_seq=(n + room) // page, n_pages=100, cache_len=n + room, kv_stride_b=page * hkv * 128)
+
+    every = (0, _cabi.lib().plx_decode_choose_splits_gqa(b, hq, hkv, n + room, 148))
+    shared = plan(b, hq, hkv, n, room, 128, 148)
+    in_pages, own_tensors = prefix(k=None, v=None, len=n), prefix(len=n, stride_t=hkv * 128)
+    for page in (1, 2, 4, 8, 64):
+        assert call(in_pages, **paged(page)) == (every if page < 8 else shared)
+    dense = dict(cache_len=room, kv_stride_b=room * hkv * 128)
+    assert call(own_tensors, **dense) == shared
+    for scale in (0.0, -0.1):
+        assert call(own_tensors, qk_scale=scale, **dense) == call(in_pages, qk_scale=scale, **paged(64)) == every
+    assert call(prefix(len=n, stride_t=0), **dense) == call(prefix(len=n, stride_t=hkv * 128, stride_h=0), **dense) == every
+
+
+def test_plans_of_calls_that_are_refused():
+    x, one = prefix(), C.c_int32(0)
+    ask = lambda p, x, sms=148: _cabi.lib().plx_decode_prefix_plan_call(p, x, sms, C.byref(one), C.byref(one))         # noqa: E731
+    assert ask(None, C.byref(x)) == ask(C.byref(decode_problem()), None) == ask(C.byref(decode_problem()), C.byref(x), 0) == -1
+    assert ask(C.byref(decode_problem(window_left=4)), C.byref(x)) == -1 and ask(C.byref(decode_problem()), C.byref(prefix(len=0))) == -1
+    assert ask(C.byref(decode_problem(**PAGED)), C.byref(x)) == ask(C.byref(decode_problem(head_dim=96)), C.byref(x)) == _cabi.PLX_ERR_UNSUPPORTED
+    p = decode_problem(batch=65535)
+    assert ask(C.byref(p), C.byref(x)) == 0 and one.value >= 1
