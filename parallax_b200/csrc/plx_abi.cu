@@ -1,6 +1,7 @@
 // extern "C" surface of libplx_sm100.so (declared in include/plx_abi.h):
 // argument validation, kernel selection, launch accounting.
 #include <algorithm>
+#include <array>
 #include <atomic>
 #include <cmath>
 
@@ -317,6 +318,79 @@ static int run_train_bwd(const plx_train_problem *p, int32_t sink_tokens, int32_
     return PLX_OK;
 }
 
+// n_splits of plx_prefix and of the problem
+static void plan_prefix(int32_t batch, int32_t heads_q, int32_t heads_kv, int32_t len, int32_t own_len, int32_t head_dim, int32_t sm_count,
+                        int32_t *prefix_splits, int32_t *own_splits) {
+    // A model of a call in units of 10 ns, its constants fitted at head_dim 128 to the times of 25 shapes at up to 90 pairs of splits each (4 to 200
+    // rows, prefixes of 1000 to 32768 keys, 30 to 8000 own ones of uneven lengths): what it chooses is within 7% of the best pair for each of them.
+    const bool grouped = heads_q > heads_kv;
+    const int64_t rows = static_cast<int64_t>(batch) * heads_kv * (grouped ? (heads_q / heads_kv + 15) / 16 : 1);   // sweeps of own keys
+    // own_len is the room that rows have; what they hold of it is on the device.  Up to 512 keys the plan is that for full rows; with more room
+    // it has the least product of its times at 512 keys and at the room, counted up to 8192.  Measured over 19 shapes with rooms of 4096 and 65536 keys,
+    // rows of 40 to 16384 in use, against the best way for each: 17% more time in the mean, the worst 1.9 times; the plan for full rows 62% and 10.8 times,
+    // the one for 512 keys 46% and 12.1 times.  Device time with 512 keys in room for 512 / 8192 / 98304, us: 32 rows, 32 : 8 heads, 8192 keys in front
+    // 29.9 / 31.6 / 31.4; 128 rows, 32768 keys 155 / 174 / 173; 16 rows, 8 : 1 heads, 16000 keys 24.2 / 30.8 / 29.7.
+    const int64_t lens[2] = {std::min<int64_t>(own_len, 512), std::min<int64_t>(own_len, 8192)};
+    const int n_lens = lens[1] > lens[0] ? 2 : 1;
+    const int dim = n_lens > 1 ? 128 : head_dim;      // (64 takes 0.6 to 0.8 of the time, either way: its own figures in half the model are 29% off, those of 128 21%)
+    // Shared.  The prefix: rounds of items over the SMs, 1.07 us a tile of 64 keys and about four tiles for start and end.  The own keys run beside
+    // it, `k` times 16 of them in a CTA: one CTA on an SM of the prefix, which slows that one down, eight on an SM that the prefix leaves free; the
+    // longest row's CTA may take longest.  So the best prefix may leave SMs free.  Then the merge.  (The two one after the other, each over all SMs: 32
+    // rows, 32 : 8 heads, 8192 keys and 512 own ones 34.7 us against 29.2; 128 rows, 32768 keys 172 against 153.)
+    const int64_t beside = grouped ? 80 : 460, free_start = grouped ? 300 : 380, free_step = grouped ? 140 : 240, tail_start = grouped ? 350 : 600,
+                  tail_step = grouped ? 100 : 200;
+    const int64_t units = static_cast<int64_t>(prefix_row_tiles(heads_q / heads_kv, batch)) * heads_kv, tiles = (static_cast<int64_t>(len) + 63) / 64;
+    auto shared_time = [&](int n, int own, int64_t own_keys) {
+        const int64_t rounds = (units * n + sm_count - 1) / sm_count, used = units * n / rounds, free = sm_count > used ? sm_count - used : 0;
+        const int64_t prefix = 400 + rounds * (107 * ((tiles + n - 1) / n) + 400);
+        const int64_t merge = 200 + static_cast<int64_t>(batch) * heads_q * (n + 1) * PLX_DECODE_PART_FLOATS(dim) * 4 / 40000;
+        const int64_t k = (own_keys + 16 * own - 1) / (16 * own);
+        const int64_t ctas = grouped || heads_q % 2 ? rows * own : rows * own / 2;
+        int64_t cost = prefix;
+        if (k > 0) {
+            const double rate_beside = static_cast<double>(used) / (beside * k), rate = rate_beside + 8.0 * free / (free_start + free_step * k);
+            const int64_t all = static_cast<int64_t>(ctas / rate), tail = tail_start + tail_step * k;
+            cost += static_cast<int64_t>(0.75 * std::min(all, prefix) * rate_beside / rate);
+            cost = std::max(cost, std::max(500 + all, tail) + std::min(all, tail) / 8);
+        }
+        return cost + merge;
+    };
+    // Every row sweeping the prefix in front of its own keys, one launch instead of three, its bytes at 4.4 TB/s with one q head per kv head and, the
+    // rows meeting in L2, 9 with grouped ones.  Measured, device time of the call with 40 own keys, us, shared / every row: 8 : 8 heads, 4 rows, 500 keys
+    // 11.4 / 7.2, 2000 12.6 / 11.4, 4000 14.7 / 17.4, 16000 25.0 / 66.1; 8 rows, 500 11.2 / 9.2, 1000 11.7 / 15.8; 16 rows, 500 11.3 / 14.3; 32 : 8 heads, 2 rows, 4000
+    // 15.0 / 13.7, 16000 24.8 / 26.8; 4 rows, 4000 14.8 / 17.4; 16 rows, 500 12.8 / 12.0, 1000 13.3 / 16.3, 4000 16.4 / 38.8; 8 : 1 heads, 8 rows, 16000 19.8 / 20.0, 16 rows 21.0 / 28.2.
+    auto every_row_time = [&](int64_t own_keys) {
+        const int64_t kb = 4ll * batch * (len + own_keys) * heads_kv * dim / 1000;
+        return grouped ? 1050 + kb / 90 : (static_cast<int64_t>(batch) * heads_q <= PLX_DECODE_SPLIT_GROUP_MAX_BH ? 450 : 900) + kb / 44;
+    };
+    int best = 1, best_own = 1;
+    double shared = INFINITY, limit = 0, every_row = 1;      // (the model is 1/15 above the times of shared ones, where there are few own keys)
+    for (int i = 0; i < n_lens; ++i) every_row *= static_cast<double>(every_row_time(lens[i]));
+    for (int n = 1; n <= PLX_PREFIX_MAX_SPLITS && n <= tiles; ++n)
+        for (int own = 1; own <= 32 && (own == 1 || 16 * own <= own_len); own *= 2) {
+            double cost = 1, less = 1;
+            for (int i = 0; i < n_lens; ++i) {
+                const int64_t t = shared_time(n, own, lens[i]);
+                cost *= static_cast<double>(t);
+                less *= static_cast<double>(t * 15 / 16);
+            }
+            if (cost < shared) {
+                shared = cost;
+                limit = less;
+                best = n;
+                best_own = own;
+            }
+        }
+    if (every_row < limit) {
+        const int64_t keys = static_cast<int64_t>(len) + own_len;
+        *prefix_splits = 0;
+        *own_splits = plx_decode_choose_splits_gqa(batch, heads_q, heads_kv, static_cast<int32_t>(keys < INT32_MAX ? keys : INT32_MAX), sm_count);
+        return;
+    }
+    *prefix_splits = best;
+    *own_splits = best_own;
+}
+
 }  // namespace plx
 
 using namespace plx;
@@ -611,74 +685,23 @@ int plx_decode_prefix_plan(int32_t batch, int32_t heads_q, int32_t heads_kv, int
     if (batch <= 0 || heads_kv <= 0 || heads_q < heads_kv || heads_q % heads_kv != 0 || len <= 0 || own_len < 0 || head_dim <= 0 || sm_count <= 0 ||
         !prefix_splits || !own_splits)
         return PLX_ERR_BAD_ARG;
-    // A model of a call in units of 10 ns, its constants fitted at head_dim 128 to the times of 25 shapes at up to 90 pairs of splits each (4 to 200
-    // rows, prefixes of 1000 to 32768 keys, 30 to 8000 own ones of uneven lengths): what it chooses is within 7% of the best pair for each of them.
-    const bool grouped = heads_q > heads_kv;
-    const int64_t rows = static_cast<int64_t>(batch) * heads_kv * (grouped ? (heads_q / heads_kv + 15) / 16 : 1);   // sweeps of own keys
-    // own_len is the room that rows have; what they hold of it is on the device.  Up to 512 keys the plan is that for full rows; with more room
-    // it has the least product of its times at 512 keys and at the room, counted up to 8192.  Measured over 19 shapes with rooms of 4096 and 65536 keys,
-    // rows of 40 to 16384 in use, against the best way for each: 17% more time in the mean, the worst 1.9 times; the plan for full rows 62% and 10.8 times,
-    // the one for 512 keys 46% and 12.1 times.  Device time with 512 keys in room for 512 / 8192 / 98304, us: 32 rows, 32 : 8 heads, 8192 keys in front
-    // 29.9 / 31.6 / 31.4; 128 rows, 32768 keys 155 / 174 / 173; 16 rows, 8 : 1 heads, 16000 keys 24.2 / 30.8 / 29.7.
-    const int64_t lens[2] = {std::min<int64_t>(own_len, 512), std::min<int64_t>(own_len, 8192)};
-    const int n_lens = lens[1] > lens[0] ? 2 : 1;
-    const int dim = n_lens > 1 ? 128 : head_dim;      // (64 takes 0.6 to 0.8 of the time, either way: its own figures in half the model are 29% off, those of 128 21%)
-    // Shared.  The prefix: rounds of items over the SMs, 1.07 us a tile of 64 keys and about four tiles for start and end.  The own keys run beside
-    // it, `k` times 16 of them in a CTA: one CTA on an SM of the prefix, which slows that one down, eight on an SM that the prefix leaves free; the
-    // longest row's CTA may take longest.  So the best prefix may leave SMs free.  Then the merge.  (The two one after the other, each over all SMs: 32
-    // rows, 32 : 8 heads, 8192 keys and 512 own ones 34.7 us against 29.2; 128 rows, 32768 keys 172 against 153.)
-    const int64_t beside = grouped ? 80 : 460, free_start = grouped ? 300 : 380, free_step = grouped ? 140 : 240, tail_start = grouped ? 350 : 600,
-                  tail_step = grouped ? 100 : 200;
-    const int64_t units = static_cast<int64_t>(prefix_row_tiles(heads_q / heads_kv, batch)) * heads_kv, tiles = (static_cast<int64_t>(len) + 63) / 64;
-    auto shared_time = [&](int n, int own, int64_t own_keys) {
-        const int64_t rounds = (units * n + sm_count - 1) / sm_count, used = units * n / rounds, free = sm_count > used ? sm_count - used : 0;
-        const int64_t prefix = 400 + rounds * (107 * ((tiles + n - 1) / n) + 400);
-        const int64_t merge = 200 + static_cast<int64_t>(batch) * heads_q * (n + 1) * PLX_DECODE_PART_FLOATS(dim) * 4 / 40000;
-        const int64_t k = (own_keys + 16 * own - 1) / (16 * own);
-        const int64_t ctas = grouped || heads_q % 2 ? rows * own : rows * own / 2;
-        int64_t cost = prefix;
-        if (k > 0) {
-            const double rate_beside = static_cast<double>(used) / (beside * k), rate = rate_beside + 8.0 * free / (free_start + free_step * k);
-            const int64_t all = static_cast<int64_t>(ctas / rate), tail = tail_start + tail_step * k;
-            cost += static_cast<int64_t>(0.75 * std::min(all, prefix) * rate_beside / rate);
-            cost = std::max(cost, std::max(500 + all, tail) + std::min(all, tail) / 8);
-        }
-        return cost + merge;
+    // Host arithmetic on these seven numbers, for up to 762 pairs, 20 to 50 us of a host core.  A decode loop asks the same for every
+    // layer and step, so a thread keeps its last plans.
+    struct Plan {
+        std::array<int32_t, 7> key;
+        int32_t prefix_splits, own_splits;
     };
-    // Every row sweeping the prefix in front of its own keys, one launch instead of three, its bytes at 4.4 TB/s with one q head per kv head and, the
-    // rows meeting in L2, 9 with grouped ones.  Measured, device time of the call with 40 own keys, us, shared / every row: 8 : 8 heads, 4 rows, 500 keys
-    // 11.4 / 7.2, 2000 12.6 / 11.4, 4000 14.7 / 17.4, 16000 25.0 / 66.1; 8 rows, 500 11.2 / 9.2, 1000 11.7 / 15.8; 16 rows, 500 11.3 / 14.3; 32 : 8 heads, 2 rows, 4000
-    // 15.0 / 13.7, 16000 24.8 / 26.8; 4 rows, 4000 14.8 / 17.4; 16 rows, 500 12.8 / 12.0, 1000 13.3 / 16.3, 4000 16.4 / 38.8; 8 : 1 heads, 8 rows, 16000 19.8 / 20.0, 16 rows 21.0 / 28.2.
-    auto every_row_time = [&](int64_t own_keys) {
-        const int64_t kb = 4ll * batch * (len + own_keys) * heads_kv * dim / 1000;
-        return grouped ? 1050 + kb / 90 : (static_cast<int64_t>(batch) * heads_q <= PLX_DECODE_SPLIT_GROUP_MAX_BH ? 450 : 900) + kb / 44;
-    };
-    int best = 1, best_own = 1;
-    double shared = INFINITY, limit = 0, every_row = 1;      // (the model is 1/15 above the times of shared ones, where there are few own keys)
-    for (int i = 0; i < n_lens; ++i) every_row *= static_cast<double>(every_row_time(lens[i]));
-    for (int n = 1; n <= PLX_PREFIX_MAX_SPLITS && n <= tiles; ++n)
-        for (int own = 1; own <= 32 && (own == 1 || 16 * own <= own_len); own *= 2) {
-            double cost = 1, less = 1;
-            for (int i = 0; i < n_lens; ++i) {
-                const int64_t t = shared_time(n, own, lens[i]);
-                cost *= static_cast<double>(t);
-                less *= static_cast<double>(t * 15 / 16);
-            }
-            if (cost < shared) {
-                shared = cost;
-                limit = less;
-                best = n;
-                best_own = own;
-            }
-        }
-    if (every_row < limit) {
-        const int64_t keys = static_cast<int64_t>(len) + own_len;
-        *prefix_splits = 0;
-        *own_splits = plx_decode_choose_splits_gqa(batch, heads_q, heads_kv, static_cast<int32_t>(keys < INT32_MAX ? keys : INT32_MAX), sm_count);
-        return PLX_OK;
+    thread_local Plan plans[16] = {};                   // (a key of zeros is not valid)
+    const std::array<int32_t, 7> key = {batch, heads_q, heads_kv, len, own_len, head_dim, sm_count};
+    uint32_t h = 0;
+    for (int32_t x : key) h = (h ^ static_cast<uint32_t>(x)) * 0x9E3779B1u;
+    Plan &plan = plans[h >> 28];
+    if (plan.key != key) {
+        plan_prefix(batch, heads_q, heads_kv, len, own_len, head_dim, sm_count, &plan.prefix_splits, &plan.own_splits);
+        plan.key = key;
     }
-    *prefix_splits = best;
-    *own_splits = best_own;
+    *prefix_splits = plan.prefix_splits;
+    *own_splits = plan.own_splits;
     return PLX_OK;
 }
 

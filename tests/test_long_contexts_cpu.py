@@ -102,3 +102,16 @@ def test_plans_of_calls_that_are_refused():
     assert ask(C.byref(decode_problem(**PAGED)), C.byref(x)) == ask(C.byref(decode_problem(head_dim=96)), C.byref(x)) == _cabi.PLX_ERR_UNSUPPORTED
     p = decode_problem(batch=65535)
     assert ask(C.byref(p), C.byref(x)) == 0 and one.value >= 1
+
+
+def test_plans_that_are_kept():
+    """A thread keeps its last plans: asked again, in any order and by any thread, each shape has its own."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    shapes = [(b, hq, 8, p, room, d, sms) for b in (4, 32, 128) for hq in (8, 32) for p in (500, 8192) for room in (40, 512, 8192) for d in (64, 128) for sms in (74, 148)]
+    first = [plan(*x) for x in shapes]
+    assert len(set(first)) > 20
+    assert [plan(*x) for x in reversed(shapes) for _ in range(2)][::2] == first[::-1]
+    with ThreadPoolExecutor(4) as pool:
+        for got in pool.map(lambda i: [plan(*x) for x in shapes[i:] + shapes[:i]], range(0, len(shapes), 9)):
+            assert sorted(got) == sorted(first)
