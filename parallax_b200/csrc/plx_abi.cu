@@ -819,9 +819,7 @@ int plx_pages_copy(const plx_page_pool *p, const int32_t *src, const int32_t *ds
 }
 
 int plx_pages_workspace_bytes(int32_t n_pages, int32_t batch, int32_t n_forks, size_t *bytes) {
-    if (n_pages <= 0 || batch <= 0 || n_forks < 0 || !bytes) return PLX_ERR_BAD_ARG;
-    *bytes = pages_workspace_bytes(n_pages, batch, n_forks);
-    return PLX_OK;
+    return pages_workspace_bytes(n_pages, batch, n_forks, bytes);
 }
 
 int plx_pages_fork(const plx_page_pool *p, const int32_t *page_table, const int32_t *lens, int32_t batch, int32_t pages_per_seq,

@@ -20,6 +20,7 @@ namespace {
 constexpr int kPlanThreads = 1024;
 constexpr int kCopyThreads = 256, kCopyUnroll = 4;              // 16 KB of a page per CTA and step
 constexpr int kPieceChunks = kCopyThreads * kCopyUnroll;
+constexpr int kMost = 1 << 30;                                  // pages, table entries, items of a list: strides of a CTA stay inside 32 bits
 constexpr int kMaxBitmapWords = 32 * 1024;                      // bitmap and ranks, 128 KB of shared memory: 524288 pages
 
 struct PoolArgs {
@@ -406,7 +407,7 @@ int make_pool(const plx_page_pool *p, PoolArgs &a, bool &flat) {
         if (s < 0 || (s & 7) != 0) return PLX_ERR_BAD_ARG;
     if (p->n_pages > 1 && (p->k_stride_p == 0 || p->v_stride_p == 0)) return PLX_ERR_BAD_ARG;      // pages on top of each other
     const int64_t row = p->head_dim, key = row * p->heads_kv;
-    if (key / 8 * p->page_size > INT32_MAX / 2) return PLX_ERR_UNSUPPORTED;
+    if (key / 8 * p->page_size > INT32_MAX / 2 || p->n_pages > kMost) return PLX_ERR_UNSUPPORTED;
     a = PoolArgs{};
     a.k = p->k; a.v = p->v;
     a.n_pages = p->n_pages; a.page_size = p->page_size;
@@ -421,7 +422,7 @@ int make_pool(const plx_page_pool *p, PoolArgs &a, bool &flat) {
 
 int make_table(const int32_t *table, const int32_t *lens, int batch, int pages_per_seq, int n_pages, int page_size, TableArgs &t) {
     if (!table || !lens || batch <= 0 || pages_per_seq <= 0 || n_pages <= 0 || page_size <= 0 || (page_size & (page_size - 1)) != 0) return PLX_ERR_BAD_ARG;
-    if (static_cast<int64_t>(batch) * pages_per_seq > INT32_MAX) return PLX_ERR_UNSUPPORTED;
+    if (static_cast<int64_t>(batch) * pages_per_seq > kMost || n_pages > kMost) return PLX_ERR_UNSUPPORTED;
     t = TableArgs{};
     t.table = table; t.lens = lens;
     t.batch = batch; t.pages_per_seq = pages_per_seq; t.n_pages = n_pages;
@@ -448,6 +449,7 @@ int launch_pages_copy(const plx_page_pool *p, const int32_t *src, const int32_t 
     int st = make_pool(p, pool, flat);
     if (st != PLX_OK) return st;
     if (n < 0 || (n > 0 && (!src || !dst))) return PLX_ERR_BAD_ARG;
+    if (n > kMost) return PLX_ERR_UNSUPPORTED;
     if ((st = check_device()) != PLX_OK) return st;
     const int pieces = pieces_of(pool.page_size, pool.chunks_per_key);
     for (int at = 0; at < n && st == PLX_OK; at += 65535) {          // the grid's third axis
@@ -458,7 +460,12 @@ int launch_pages_copy(const plx_page_pool *p, const int32_t *src, const int32_t 
     return st;
 }
 
-size_t pages_workspace_bytes(int n_pages, int batch, int n_forks) { return lay_out(nullptr, n_pages, batch, n_forks, nullptr); }
+int pages_workspace_bytes(int n_pages, int batch, int n_forks, size_t *bytes) {
+    if (n_pages <= 0 || batch <= 0 || n_forks < 0 || !bytes) return PLX_ERR_BAD_ARG;
+    if (n_pages > kMost || batch > kMost || n_forks > kMost) return PLX_ERR_UNSUPPORTED;
+    *bytes = lay_out(nullptr, n_pages, batch, n_forks, nullptr);
+    return PLX_OK;
+}
 
 int launch_pages_compact(const plx_page_pool *p, const int32_t *table, const int32_t *lens, int batch, int pages_per_seq, int32_t *new_table, int32_t *n_live,
                          void *ws, size_t ws_bytes, cudaStream_t stream) {
@@ -491,6 +498,7 @@ int launch_pages_fork(const plx_page_pool *p, const int32_t *table, const int32_
     if (st == PLX_OK) st = make_table(table, lens, batch, pages_per_seq, p->n_pages, p->page_size, t);
     if (st != PLX_OK) return st;
     if (n <= 0 || !parents || !children || !new_table || !new_lens || !missing) return PLX_ERR_BAD_ARG;
+    if (n > kMost) return PLX_ERR_UNSUPPORTED;
     Plan plan;
     if (!ws || (reinterpret_cast<uintptr_t>(ws) & 15u) != 0 || lay_out(static_cast<unsigned char *>(ws), p->n_pages, batch, n, &plan) > ws_bytes) return PLX_ERR_WORKSPACE;
     t.new_table = new_table;
@@ -510,6 +518,7 @@ int launch_pages_free(const int32_t *table, const int32_t *lens, int batch, int 
     int st = make_table(table, lens, batch, pages_per_seq, n_pages, page_size, t);
     if (st != PLX_OK) return st;
     if (n_rows < 0 || (n_rows > 0 && !rows) || !new_lens || !free_list || !n_free) return PLX_ERR_BAD_ARG;
+    if (n_rows > kMost) return PLX_ERR_UNSUPPORTED;
     Plan plan;
     if (!ws || (reinterpret_cast<uintptr_t>(ws) & 15u) != 0 || lay_out(static_cast<unsigned char *>(ws), n_pages, batch, 0, &plan) > ws_bytes) return PLX_ERR_WORKSPACE;
     t.new_lens = new_lens;

@@ -115,3 +115,23 @@ def test_plans_that_are_kept():
     with ThreadPoolExecutor(4) as pool:
         for got in pool.map(lambda i: [plan(*x) for x in shapes[i:] + shapes[:i]], range(0, len(shapes), 9)):
             assert sorted(got) == sorted(first)
+
+
+def test_lists_of_pages_that_are_too_long_for_their_indices():
+    """Threads step through pages, entries and lists by the thousand in 32 bits: near 2^31 that would wrap around and read before the list."""
+    from tests.test_pages_cpu import c_pool
+
+    lib, one, most, n = _cabi.lib(), C.c_void_p(1 << 20), 1 << 30, C.c_size_t(0)
+    refused, ws = _cabi.PLX_ERR_UNSUPPORTED, 1 << 60
+    pool, big = C.byref(c_pool()), C.byref(c_pool(n_pages=most + 1))
+    assert lib.plx_pages_copy(pool, one, one, most + 1, None) == lib.plx_pages_copy(big, one, one, 1, None) == refused
+    for size in (most + 1, 2 ** 31 - 1):
+        assert lib.plx_pages_fork(pool, one, one, 2, 4, one, one, size, one, one, one, one, ws, None) == refused
+        assert lib.plx_pages_free(one, one, 2, 4, one, size, 8, 16, one, one, one, one, ws, None) == refused          # rows
+        assert lib.plx_pages_free(one, one, 2, 4, one, 1, size, 16, one, one, one, one, ws, None) == refused          # pages
+        assert lib.plx_pages_free(one, one, 1, size, one, 1, 8, 16, one, one, one, one, ws, None) == refused          # entries
+        for sizes in ((size, 2, 0), (8, size, 0), (8, 2, size)):
+            assert lib.plx_pages_workspace_bytes(*sizes, C.byref(n)) == refused
+    assert lib.plx_pages_fork(big, one, one, 2, 4, one, one, 1, one, one, one, one, ws, None) == refused
+    assert lib.plx_pages_compact(big, one, one, 2, 4, one, one, one, ws, None) == refused
+    assert lib.plx_pages_workspace_bytes(most, 2, 0, C.byref(n)) == 0 and n.value > 16 * most
