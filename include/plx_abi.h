@@ -402,8 +402,10 @@ typedef struct plx_page_pool {
  * target (what such a page holds afterwards is not defined). */
 int plx_pages_copy(const plx_page_pool *p, const int32_t *src, const int32_t *dst, int32_t n, plx_stream_t stream);
 
-/* n_forks: the n of plx_pages_fork; 0 for the other two */
+/* n_forks: the n of plx_pages_fork; 0 for plx_pages_compact */
 int plx_pages_workspace_bytes(int32_t n_pages, int32_t batch, int32_t n_forks, size_t *bytes);
+/* of plx_pages_free; 0 (and no workspace) for pools of up to 524288 pages */
+int plx_pages_free_workspace_bytes(int32_t n_pages, size_t *bytes);
 
 /* Row children[i] becomes row parents[i] (as it was before the call), i < n; of a row mentioned twice among the
  * children the last one counts.  Whole pages are shared; the keys of a last page that is not full are copied to a page of

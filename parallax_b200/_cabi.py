@@ -27,7 +27,7 @@ SYMBOLS = (
     "plx_decode_merge", "plx_decode_exchange_bytes", "plx_decode_exchange_merge", "plx_decode_partial_exchange",
     "plx_train_workspace_bytes_sink", "plx_train_fwd_sink", "plx_train_extend_sink", "plx_train_bwd_sink",
     "plx_decode_sink", "plx_decode_step_sink", "plx_decode_prefix_plan", "plx_decode_prefix_plan_call", "plx_decode_prefix_workspace_bytes", "plx_decode_prefix",
-    "plx_pages_copy", "plx_pages_workspace_bytes", "plx_pages_fork", "plx_pages_compact", "plx_pages_free",
+    "plx_pages_copy", "plx_pages_workspace_bytes", "plx_pages_free_workspace_bytes", "plx_pages_fork", "plx_pages_compact", "plx_pages_free",
 )
 EXCHANGE_MAX_RANKS = 16
 
@@ -160,6 +160,8 @@ def _declare(lib):
     lib.plx_pages_copy.argtypes = [pool, vp, vp, i32, vp]
     lib.plx_pages_workspace_bytes.restype = C.c_int
     lib.plx_pages_workspace_bytes.argtypes = [i32, i32, i32, C.POINTER(sz)]
+    lib.plx_pages_free_workspace_bytes.restype = C.c_int
+    lib.plx_pages_free_workspace_bytes.argtypes = [i32, C.POINTER(sz)]
     lib.plx_pages_fork.restype = C.c_int
     lib.plx_pages_fork.argtypes = [pool, vp, vp, i32, i32, vp, vp, i32, vp, vp, vp, vp, sz, vp]
     lib.plx_pages_compact.restype = C.c_int

@@ -822,6 +822,8 @@ int plx_pages_workspace_bytes(int32_t n_pages, int32_t batch, int32_t n_forks, s
     return pages_workspace_bytes(n_pages, batch, n_forks, bytes);
 }
 
+int plx_pages_free_workspace_bytes(int32_t n_pages, size_t *bytes) { return pages_free_workspace_bytes(n_pages, bytes); }
+
 int plx_pages_fork(const plx_page_pool *p, const int32_t *page_table, const int32_t *lens, int32_t batch, int32_t pages_per_seq,
                    const int32_t *parents, const int32_t *children, int32_t n, int32_t *new_page_table, int32_t *new_lens,
                    int32_t *missing, void *workspace, size_t workspace_bytes, plx_stream_t stream) {

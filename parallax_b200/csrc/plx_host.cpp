@@ -56,6 +56,7 @@ struct Api {
     decltype(&plx_decode_prefix_workspace_bytes) decode_prefix_workspace_bytes;
     decltype(&plx_decode_prefix) decode_prefix;
     decltype(&plx_pages_workspace_bytes) pages_workspace_bytes;
+    decltype(&plx_pages_free_workspace_bytes) pages_free_workspace_bytes;
     decltype(&plx_pages_copy) pages_copy;
     decltype(&plx_pages_fork) pages_fork;
     decltype(&plx_pages_compact) pages_compact;
@@ -82,6 +83,7 @@ void bind(const py::dict &addresses) {
     bind_one(api.decode_prefix_workspace_bytes, addresses, "plx_decode_prefix_workspace_bytes");
     bind_one(api.decode_prefix, addresses, "plx_decode_prefix");
     bind_one(api.pages_workspace_bytes, addresses, "plx_pages_workspace_bytes");
+    bind_one(api.pages_free_workspace_bytes, addresses, "plx_pages_free_workspace_bytes");
     bind_one(api.pages_copy, addresses, "plx_pages_copy");
     bind_one(api.pages_fork, addresses, "plx_pages_fork");
     bind_one(api.pages_compact, addresses, "plx_pages_compact");
@@ -839,8 +841,9 @@ py::object pages_free(const py::object &table_, const py::object &lens_, const p
     at::AutoDispatchBelowADInplaceOrView below;
     const c10::cuda::CUDAGuard device(table.device());
     RECORD_FUNCTION("plx::pages_free", Values({table, lens, rows}));
-    const Tensor ws = pages_scratch(table, n_pages, table.size(0), 0);
-    if (!ws.defined()) return py::none();
+    size_t need = 0;
+    if (api.pages_free_workspace_bytes(static_cast<int32_t>(n_pages), &need) != PLX_OK) return py::none();
+    const Tensor ws = at::empty({static_cast<int64_t>(need)}, table.options().dtype(at::kByte));
     Tensor new_lens = at::empty(lens.sizes(), lens.options()), free_list = at::empty({n_pages}, lens.options()), n_free = at::empty({1}, lens.options());
     if (api.pages_free(ints(table), ints(lens), static_cast<int32_t>(table.size(0)), static_cast<int32_t>(table.size(1)), ints(rows),
                        static_cast<int32_t>(rows.numel()), static_cast<int32_t>(n_pages), static_cast<int32_t>(page_size), ints(new_lens), ints(free_list),

@@ -96,6 +96,7 @@ int launch_prefix_merge(const float *parts, int n_parts, int64_t n_rows, int hea
 // pages of a cache (see plx_pages.cu)
 int launch_pages_copy(const plx_page_pool *p, const int32_t *src, const int32_t *dst, int n, cudaStream_t stream);
 int pages_workspace_bytes(int n_pages, int batch, int n_forks, size_t *bytes);
+int pages_free_workspace_bytes(int n_pages, size_t *bytes);
 int launch_pages_fork(const plx_page_pool *p, const int32_t *table, const int32_t *lens, int batch, int pages_per_seq, const int32_t *parents,
                       const int32_t *children, int n, int32_t *new_table, int32_t *new_lens, int32_t *missing, void *ws, size_t ws_bytes,
                       cudaStream_t stream);

@@ -4,10 +4,11 @@
 // be captured; what a table holds beyond a row's active entries is not looked at, and page or row numbers out of range
 // are passed over.
 //
-// A call is two launches (copying: one).  The PLAN is one CTA: a bitmap of the live pages in shared memory (up to 524288
+// Forking and compacting are two launches each.  The PLAN is one CTA: a bitmap of the live pages in shared memory (up to 524288
 // pages; beyond that in global memory), filled from the active entries, counted once, from which ranks
 // of live and free pages follow by popcount.  The APPLICATION is spread over the chip: table entries, and pages cut into
-// pieces of 16 KB that CTAs take in turn, four 16-byte loads a thread in flight.
+// pieces of 16 KB that CTAs take in turn, four 16-byte loads a thread in flight.  Copying is an application alone, freeing a plan that
+// writes its lists.
 #include <mutex>
 
 #include "plx_common.cuh"
@@ -369,7 +370,8 @@ bool opt_in() {
 
 size_t aligned(size_t bytes) { return (bytes + 15u) & ~static_cast<size_t>(15u); }
 
-// The parts of a workspace; returns its size.  `moves`: the most there can be.
+// The parts of a workspace; returns its size.  n_forks: 0 for compacting, kFree for freeing, which needs the bitmap alone.
+constexpr int kFree = -1;
 size_t lay_out(unsigned char *ws, int n_pages, int batch, int n_forks, Plan *plan) {
     size_t at = 0;
     auto part = [&](size_t bytes) {
@@ -377,16 +379,16 @@ size_t lay_out(unsigned char *ws, int n_pages, int batch, int n_forks, Plan *pla
         at += aligned(bytes);
         return p;
     };
-    const int most = n_forks > 0 ? n_forks : n_pages, words = (n_pages + 31) / 32;
+    const size_t moves = n_forks > 0 ? n_forks : n_forks == kFree ? 0 : n_pages, words = (static_cast<size_t>(n_pages) + 31) / 32;
     const bool global = plan_smem(n_pages) == 0;
     Plan p{};
-    p.n_moves = reinterpret_cast<int32_t *>(part(4));
-    p.moves = reinterpret_cast<Move *>(part(sizeof(Move) * static_cast<size_t>(most)));
-    p.map = reinterpret_cast<int32_t *>(part(n_forks > 0 ? 0 : 4 * static_cast<size_t>(n_pages)));
+    p.n_moves = reinterpret_cast<int32_t *>(part(moves ? 4 : 0));
+    p.moves = reinterpret_cast<Move *>(part(sizeof(Move) * moves));
+    p.map = reinterpret_cast<int32_t *>(part(n_forks == 0 ? 4 * moves : 0));
     p.last = reinterpret_cast<int32_t *>(part(n_forks > 0 ? 4 * static_cast<size_t>(batch) : 0));
-    p.fresh = reinterpret_cast<int32_t *>(part(4 * static_cast<size_t>(n_forks)));
-    p.bits = global ? reinterpret_cast<uint32_t *>(part(4 * static_cast<size_t>(words))) : nullptr;
-    p.before = global ? reinterpret_cast<int32_t *>(part(4 * static_cast<size_t>(words))) : nullptr;
+    p.fresh = reinterpret_cast<int32_t *>(part(n_forks > 0 ? 4 * moves : 0));
+    p.bits = global ? reinterpret_cast<uint32_t *>(part(4 * words)) : nullptr;
+    p.before = global ? reinterpret_cast<int32_t *>(part(4 * words)) : nullptr;
     if (plan) *plan = p;
     return at;
 }
@@ -466,6 +468,12 @@ int pages_workspace_bytes(int n_pages, int batch, int n_forks, size_t *bytes) {
     *bytes = lay_out(nullptr, n_pages, batch, n_forks, nullptr);
     return PLX_OK;
 }
+int pages_free_workspace_bytes(int n_pages, size_t *bytes) {
+    if (n_pages <= 0 || !bytes) return PLX_ERR_BAD_ARG;
+    if (n_pages > kMost) return PLX_ERR_UNSUPPORTED;
+    *bytes = lay_out(nullptr, n_pages, 1, kFree, nullptr);
+    return PLX_OK;
+}
 
 int launch_pages_compact(const plx_page_pool *p, const int32_t *table, const int32_t *lens, int batch, int pages_per_seq, int32_t *new_table, int32_t *n_live,
                          void *ws, size_t ws_bytes, cudaStream_t stream) {
@@ -520,7 +528,8 @@ int launch_pages_free(const int32_t *table, const int32_t *lens, int batch, int 
     if (n_rows < 0 || (n_rows > 0 && !rows) || !new_lens || !free_list || !n_free) return PLX_ERR_BAD_ARG;
     if (n_rows > kMost) return PLX_ERR_UNSUPPORTED;
     Plan plan;
-    if (!ws || (reinterpret_cast<uintptr_t>(ws) & 15u) != 0 || lay_out(static_cast<unsigned char *>(ws), n_pages, batch, 0, &plan) > ws_bytes) return PLX_ERR_WORKSPACE;
+    const size_t need = lay_out(static_cast<unsigned char *>(ws), n_pages, batch, kFree, &plan);
+    if (need > 0 && (!ws || (reinterpret_cast<uintptr_t>(ws) & 15u) != 0 || need > ws_bytes)) return PLX_ERR_WORKSPACE;
     t.new_lens = new_lens;
     if ((st = check_device()) != PLX_OK) return st;
     if (!opt_in<free_kernel>()) return PLX_ERR_LAUNCH;

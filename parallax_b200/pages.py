@@ -84,7 +84,9 @@ def _(k_cache, v_cache, page_table, seqused_k):
 @torch.library.custom_op("plx::pages_free", mutates_args=(), device_types="cuda")
 def pages_free(page_table: Tensor, seqused_k: Tensor, rows: Tensor, n_pages: int, page_size: int) -> Tuple[Tensor, Tensor, Tensor]:
     lens, free, n_free = torch.empty_like(seqused_k), seqused_k.new_empty(n_pages), seqused_k.new_empty(1)
-    ws = _workspace(n_pages, page_table.shape[0], 0, page_table.device)
+    need = C.c_size_t(0)
+    _cabi.check(_cabi.lib().plx_pages_free_workspace_bytes(n_pages, C.byref(need)), "plx_pages_free_workspace_bytes")
+    ws = torch.empty(need.value, device=page_table.device, dtype=torch.uint8)
     with torch.cuda.device(page_table.device):
         st = _cabi.lib().plx_pages_free(_ptr(page_table), _ptr(seqused_k), page_table.shape[0], page_table.shape[1], _ptr(rows), rows.numel(),
                                         n_pages, page_size, _ptr(lens), _ptr(free), _ptr(n_free), _ptr(ws), C.c_size_t(ws.numel()),

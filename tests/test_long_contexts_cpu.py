@@ -135,3 +135,15 @@ def test_lists_of_pages_that_are_too_long_for_their_indices():
     assert lib.plx_pages_fork(big, one, one, 2, 4, one, one, 1, one, one, one, one, ws, None) == refused
     assert lib.plx_pages_compact(big, one, one, 2, 4, one, one, one, ws, None) == refused
     assert lib.plx_pages_workspace_bytes(most, 2, 0, C.byref(n)) == 0 and n.value > 16 * most
+
+
+def test_what_freeing_needs():
+    """A bitmap and ranks where they do not fit in shared memory, not the moves of a compaction."""
+    lib, one, n = _cabi.lib(), C.c_void_p(1 << 20), C.c_size_t(1)
+    for pages in (1, 8, 524288):
+        assert lib.plx_pages_free_workspace_bytes(pages, C.byref(n)) == 0 and n.value == 0
+    assert lib.plx_pages_free_workspace_bytes(1700000, C.byref(n)) == 0 and n.value == 2 * 4 * 53125 + 2 * 12       # (16-byte parts)
+    free = lambda ws, size: lib.plx_pages_free(one, one, 2, 4, one, 1, 1700000, 16, one, one, one, ws, size, None)     # noqa: E731
+    assert free(one, n.value - 1) == free(None, n.value) == free(C.c_void_p((1 << 20) + 4), n.value) == -4
+    assert lib.plx_pages_free_workspace_bytes(0, C.byref(n)) == lib.plx_pages_free_workspace_bytes(8, None) == -1
+    assert lib.plx_pages_free_workspace_bytes((1 << 30) + 1, C.byref(n)) == _cabi.PLX_ERR_UNSUPPORTED
