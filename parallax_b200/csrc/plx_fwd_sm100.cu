@@ -943,24 +943,24 @@ int launch_t(const TrainArgs &a, cudaStream_t stream) {
         count_launch();
         return st == cudaSuccess && cudaGetLastError() == cudaSuccess ? PLX_OK : PLX_ERR_LAUNCH;
     } else {
-    const int tiles = a.cu ? (a.len_q + kBM - 1) / kBM + a.n_seqs : (a.len_q + kBM - 1) / kBM;
-    const int n_items = tiles * a.batch * a.heads_q;
-    static std::mutex attr_mu;
-    static bool attr_done[2][tma::kMaxDevices] = {};
-    if (items_by_hardware(n_items, sms, a.cu || EXT)) {
-        auto kern = fwd_sm100_kernel<T, D, NS, MODE, true>;
-        if (!tma::opt_in_smem(kern, static_cast<int>(L::kBytes), attr_done[1], attr_mu)) return PLX_ERR_LAUNCH;
-        const int group = a.cu || EXT ? 1 : item_group(a.batch * a.heads_q, tiles, sms);
-        kern<<<n_items, 352, L::kBytes, stream>>>(a, tq, tr, tk, tv, sink, tiles, n_items, 0, group);
-    } else {
-        auto kern = fwd_sm100_kernel<T, D, NS, MODE, false>;
-        if (!tma::opt_in_smem(kern, static_cast<int>(L::kBytes), attr_done[0], attr_mu)) return PLX_ERR_LAUNCH;
-        // with plenty of items a CTA takes them in neighbouring pairs (a heavy and a light row tile)
-        const int chunk_shift = n_items >= 2 * sms ? 1 : 0, units = (n_items + (1 << chunk_shift) - 1) >> chunk_shift;
-        kern<<<units < sms ? units : sms, 352, L::kBytes, stream>>>(a, tq, tr, tk, tv, sink, tiles, n_items, chunk_shift, 0);
-    }
-    count_launch();
-    return cudaGetLastError() == cudaSuccess ? PLX_OK : PLX_ERR_LAUNCH;
+        const int tiles = a.cu ? (a.len_q + kBM - 1) / kBM + a.n_seqs : (a.len_q + kBM - 1) / kBM;
+        const int n_items = tiles * a.batch * a.heads_q;
+        static std::mutex attr_mu;
+        static bool attr_done[2][tma::kMaxDevices] = {};
+        if (items_by_hardware(n_items, sms, a.cu || EXT)) {
+            auto kern = fwd_sm100_kernel<T, D, NS, MODE, true>;
+            if (!tma::opt_in_smem(kern, static_cast<int>(L::kBytes), attr_done[1], attr_mu)) return PLX_ERR_LAUNCH;
+            const int group = a.cu || EXT ? 1 : item_group(a.batch * a.heads_q, tiles, sms);
+            kern<<<n_items, 352, L::kBytes, stream>>>(a, tq, tr, tk, tv, sink, tiles, n_items, 0, group);
+        } else {
+            auto kern = fwd_sm100_kernel<T, D, NS, MODE, false>;
+            if (!tma::opt_in_smem(kern, static_cast<int>(L::kBytes), attr_done[0], attr_mu)) return PLX_ERR_LAUNCH;
+            // with plenty of items a CTA takes them in neighbouring pairs (a heavy and a light row tile)
+            const int chunk_shift = n_items >= 2 * sms ? 1 : 0, units = (n_items + (1 << chunk_shift) - 1) >> chunk_shift;
+            kern<<<units < sms ? units : sms, 352, L::kBytes, stream>>>(a, tq, tr, tk, tv, sink, tiles, n_items, chunk_shift, 0);
+        }
+        count_launch();
+        return cudaGetLastError() == cudaSuccess ? PLX_OK : PLX_ERR_LAUNCH;
     }
 }
 

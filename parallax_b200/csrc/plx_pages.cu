@@ -27,9 +27,8 @@ constexpr int kMaxBitmapWords = 32 * 1024;                      // bitmap and ra
 struct PoolArgs {
     void *k, *v;
     int n_pages, page_size, chunks_per_key;                     // 16-byte chunks of all heads of a key
-    int chunks_per_row, heads;                                  // of one head of a key
+    int chunks_per_row;                                         // of one head of a key
     int64_t k_sp, k_st, k_sh, v_sp, v_st, v_sh;                 // strides in 16-byte chunks
-    int shift, mask;                                            // page size
 };
 
 struct TableArgs {
@@ -413,10 +412,9 @@ int make_pool(const plx_page_pool *p, PoolArgs &a, bool &flat) {
     a = PoolArgs{};
     a.k = p->k; a.v = p->v;
     a.n_pages = p->n_pages; a.page_size = p->page_size;
-    a.chunks_per_key = static_cast<int>(key / 8); a.chunks_per_row = static_cast<int>(row / 8); a.heads = p->heads_kv;
+    a.chunks_per_key = static_cast<int>(key / 8); a.chunks_per_row = static_cast<int>(row / 8);
     a.k_sp = p->k_stride_p / 8; a.k_st = p->k_stride_t / 8; a.k_sh = p->k_stride_h / 8;
     a.v_sp = p->v_stride_p / 8; a.v_st = p->v_stride_t / 8; a.v_sh = p->v_stride_h / 8;
-    a.shift = log2_of(p->page_size); a.mask = p->page_size - 1;
     auto dense = [&](int64_t st, int64_t sh) { return (p->page_size == 1 || st == key) && (p->heads_kv == 1 || sh == row); };
     flat = dense(p->k_stride_t, p->k_stride_h) && dense(p->v_stride_t, p->v_stride_h);
     return PLX_OK;
