@@ -3,9 +3,10 @@ import pytest
 import torch
 
 import parallax_b200 as plx
-from parallax_b200 import _cabi
+from parallax_b200 import _cabi, ops
 from tests.test_prefix_gpu import make, pages_of, reference
-from tests.test_sinks_gpu import close, decode_reference, hide, paged, randn
+from tests.test_sinks_gpu import check, close, decode_reference, hide, inputs, paged, randn, run
+from tests.test_sinks_gpu import reference as train_reference
 
 pytestmark = pytest.mark.gpu
 BF, FP = torch.bfloat16, torch.float16
@@ -59,3 +60,79 @@ def test_a_prefix_in_front_of_rows_with_room(hq, hkv, d, p, room, page):
     got = call()
     close(got, want, 2, "o")
     assert torch.equal(call(), got) and _cabi.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 64), (BF, 128), (FP, 128)])
+@pytest.mark.parametrize("window,sinks", [(1, 1), (0, 2), (2, 1), (1, 2)])
+def test_rows_of_two_keys(window, sinks, dtype, d):
+    """Every row but the first sees two keys (or three at most): where the gradients of q and r are differences of two terms, to the
+    tolerances of any other window."""
+    q, r, k, v = inputs(2, 4, 2, 500, 500, d, dtype)
+    go = randn(2, 4, 500, d, dtype=dtype, seed=9)
+    step = lambda: run(q, r, k, v, go, lambda *x: plx.parallax_func(*x, window_size_left=window, sink_tokens=sinks))                   # noqa: E731
+    got = step()
+    check(got, train_reference(q, r, k, v, go, window, sinks))
+    assert all(torch.equal(x, y) for x, y in zip(got, step())) and _cabi.device_error() == 0
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(8, 8, 128), (16, 4, 64)])
+def test_a_prefix_cut_out_of_wider_tensors(hq, hkv, d):
+    """Prefix and own keys whose tokens lie further apart than a token is long, by the call and by every way to split."""
+    p, lens = 700, [60, 0, 17, 1]
+    q, r, kp, vp, k, v = make(4, hq, hkv, d, BF, p, 60)
+    want = reference(q, r, [torch.cat((kp, k[i, :n])) for i, n in enumerate(lens)], [torch.cat((vp, v[i, :n])) for i, n in enumerate(lens)])
+    heads = lambda x: torch.cat((torch.full_like(x, torch.nan), x, torch.full_like(x, torch.nan)), -2)[..., hkv:2 * hkv, :]           # noqa: E731
+    channels = lambda x: torch.cat((x, torch.full_like(x, torch.nan)), -1)[..., :d]                                                  # noqa: E731
+    for wide in (heads, channels):
+        cut = [wide(x) for x in (kp, vp, k, v)]
+        assert all(x.stride() != y.stride() and torch.equal(x, y) for x, y in zip(cut, (kp, vp, k, v)))
+        assert cut[0].stride(0) > hkv * d
+        close(plx.parallax_decode_shared_prefix(q, r, *cut, seqused_k=ints(lens)), want, 2, "o")
+        for splits in (0, 1, 7):
+            for own in (1, 3):
+                out, ws = torch.empty_like(q), torch.zeros(ops.decode_prefix_workspace_bytes(q, cut[2], own, splits, None) // 4, device="cuda")
+                ops.decode_prefix(q, r, cut[0], cut[1], p, cut[2], cut[3], out, ws, d ** -0.5, own, splits, ints(lens), None)
+                close(out, want, 2, (splits, own))
+    assert _cabi.device_error() == 0
+
+
+def test_prefixes_on_two_streams_at_once():
+    """Calls of one shape that overlap on the device have workspaces of their own, and read what their own stream wrote before."""
+    p, t, b = 3000, 200, 24
+    sets = [make(b, 16, 4, 128, BF, p, t, seed=10 * i + 1) for i in range(2)]
+    lens = [[(i * 7 + j) % (t + 1) for i in range(b)] for j in range(2)]
+    want = [plx.parallax_decode_shared_prefix(*x, seqused_k=ints(n)) for x, n in zip(sets, lens)]
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    held = [ints(n) for n in lens]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                q = sets[i][0] * 1                                  # made on this stream, right before
+                got[i].append(plx.parallax_decode_shared_prefix(q, *sets[i][1:], seqused_k=held[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for xs, y in zip(got, want) for x in xs) and _cabi.device_error() == 0
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_compiled_calls(backend):
+    """Training with sinks and the page calls inside torch.compile: the same bits as outside."""
+    q, r, k, v = inputs(1, 4, 2, 700, 700, 64, BF)
+    go = randn(1, 4, 700, 64, seed=9)
+    step = lambda *x: plx.parallax_func(*x, window_size_left=64, sink_tokens=4)                     # noqa: E731
+    torch._dynamo.reset()
+    assert all(torch.equal(x, y) for x, y in zip(run(q, r, k, v, go, torch.compile(step, backend=backend)), run(q, r, k, v, go, step)))
+
+    def pages(k, v, table, lens, rows):
+        table, lens, missing = plx.parallax_fork_pages(k, v, table, lens, rows[:1], rows[1:])
+        lens, free, n_free = plx.parallax_free_pages(table, lens, rows[:1], 32, 16)
+        table, n_live = plx.parallax_compact_pages(k, v, table, lens)
+        plx.parallax_copy_pages(k, v, rows[:1], rows[1:] + 20)
+        return k, v, table, lens, missing, free, n_free, n_live
+
+    args = (torch.arange(31, 3, -1, dtype=torch.int32, device="cuda").view(2, 14), ints([100, 0]), ints([0, 1]))
+    pools = randn(32, 16, 2, 64, seed=1), randn(32, 16, 2, 64, seed=2)
+    torch._dynamo.reset()
+    got, want = torch.compile(pages, backend=backend)(*(x.clone() for x in pools), *args), pages(*(x.clone() for x in pools), *args)
+    assert all(torch.equal(x, y) for x, y in zip(got, want)) and _cabi.device_error() == 0
