@@ -282,6 +282,8 @@ def _prefix_core(q, r, k_prefix, v_prefix, prefix_len: int, k, v, scale, *, sequ
     if k_prefix is not None and (k_prefix.ndim != 3 or tuple(k_prefix.shape[1:]) != tuple(k.shape[2:]) or v_prefix.shape != k_prefix.shape or
                                  k_prefix.shape[0] == 0):
         raise ValueError(f"k_prefix/v_prefix must be (P, H_kv={k.shape[2]}, D={d}), got {tuple(k_prefix.shape)}/{tuple(v_prefix.shape)}")
+    if k.shape[1] == 0:
+        raise ValueError(f"{name}: k and v need room for a key a row at least, got {tuple(k.shape)}")
     tensors = [x for x in (r, k, v, k_prefix, v_prefix) if x is not None]
     if any(x.dtype != q.dtype for x in tensors):
         raise TypeError(f"{name}: q, r and the keys and values must have one type, got {[x.dtype for x in (q, *tensors)]}")
@@ -322,7 +324,7 @@ def parallax_decode_shared_prefix(q: torch.Tensor, r: torch.Tensor, k_prefix: to
     """Single-token decode of a batch whose rows share a prefix, which is read once for all of them.
 
     ``q``, ``r``: ``(B, 1, H_q, D)``; ``k_prefix``, ``v_prefix``: ``(P, H_kv, D)``, the keys that every row begins with; ``k``, ``v``:
-    ``(B, T, H_kv, D)``, each row's own keys behind them, of which ``seqused_k`` ``(B,)`` int32 (0 to T; without it T) are active.  The
+    ``(B, T, H_kv, D)`` with T >= 1, each row's own keys behind them, of which ``seqused_k`` ``(B,)`` int32 (0 to T; without it T) are active.  The
     result is that of :func:`parallax_decode` on the two put together.  For a paged cache:
     ``parallax_attn_with_kvcache(..., shared_prefix=P)``.  Can be captured in a CUDA graph (without ``seqused_k`` being checked).
     """

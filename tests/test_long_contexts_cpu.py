@@ -147,3 +147,8 @@ def test_what_freeing_needs():
     assert free(one, n.value - 1) == free(None, n.value) == free(C.c_void_p((1 << 20) + 4), n.value) == -4
     assert lib.plx_pages_free_workspace_bytes(0, C.byref(n)) == lib.plx_pages_free_workspace_bytes(8, None) == -1
     assert lib.plx_pages_free_workspace_bytes((1 << 30) + 1, C.byref(n)) == _cabi.PLX_ERR_UNSUPPORTED
+
+
+def test_a_prefix_in_front_of_no_room_is_refused():
+    with pytest.raises(ValueError, match="room for a key"):
+        plx.parallax_decode_shared_prefix(z(2, 1, 4, 64), z(2, 1, 4, 64), z(16, 2, 64), z(16, 2, 64), z(2, 0, 2, 64), z(2, 0, 2, 64))
