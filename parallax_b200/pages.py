@@ -5,7 +5,9 @@ with a power-of-two ``page_size``, a ``page_table`` ``(B, max_num_blocks)`` int3
 entries of a row are the first ``ceil(seqused_k / page_size)``; a page is live while some row's active entry names it, and free
 otherwise.  There is no other bookkeeping: what a table holds beyond its active entries is never looked at.
 
-Pools are written in place; tables and lengths come back as new tensors.  Everything is decided on the device -- nothing here
+Pools are written in place; tables and lengths come back as new tensors.  A model has a pair of pools per layer under ONE table: call
+once a layer, each time with the table and lengths from BEFORE; every call returns the same new ones, to be used from then on (a layer
+that is given the new table would fork or compact again).  Everything is decided on the device -- nothing here
 waits for it, so the calls can be captured in a CUDA graph -- and numbers out of range (a page outside the pool, a row outside
 the table) are passed over.  (The reference names paged caches but does not implement them:
 parallax/cute/parallax_decode.py:1578-1580.)

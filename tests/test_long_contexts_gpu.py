@@ -136,3 +136,25 @@ def test_compiled_calls(backend):
     torch._dynamo.reset()
     got, want = torch.compile(pages, backend=backend)(*(x.clone() for x in pools), *args), pages(*(x.clone() for x in pools), *args)
     assert all(torch.equal(x, y) for x, y in zip(got, want)) and _cabi.device_error() == 0
+
+
+def test_the_layers_of_a_model_under_one_table():
+    """Every layer's call takes the table as it was before: all return the same new one, and each layer's rows hold what they held."""
+    page, n_pages, lens = 16, 64, [100, 37, 0, 64]
+    layers = [(randn(n_pages, page, 2, 64, seed=2 * i), randn(n_pages, page, 2, 64, seed=2 * i + 1)) for i in range(3)]
+    order = torch.randperm(n_pages, generator=torch.Generator().manual_seed(3))[:28].view(4, 7)
+    table, used = order.to(torch.int32).cuda(), ints(lens)
+    rows = lambda pool, table, lens: [pool[table[b, :-(-n // page)].long()].flatten(0, 1)[:n].clone() for b, n in enumerate(lens.tolist())]   # noqa: E731
+    held = [[rows(x, table, used) for x in pair] for pair in layers]
+
+    new = [plx.parallax_fork_pages(*pair, table, used, ints([0, 1]), ints([2, 3])) for pair in layers]
+    assert all(torch.equal(x, y) for other in new[1:] for x, y in zip(new[0], other)) and new[0][2].item() == 0
+    table, used = new[0][:2]
+    want = [[[x[0], x[1], x[0], x[1]] for x in pair] for pair in held]
+    used, _, n_free = plx.parallax_free_pages(table, used, ints([0]), n_pages, page)
+    new = [plx.parallax_compact_pages(*pair, table, used) for pair in layers]
+    assert all(torch.equal(x, y) for other in new[1:] for x, y in zip(new[0], other)) and new[0][1].item() + n_free.item() == n_pages
+    for pair, expected in zip(layers, want):
+        for pool, x in zip(pair, expected):
+            got = rows(pool, new[0][0], used)
+            assert got[0].numel() == 0 and all(torch.equal(a, b) for a, b in zip(got[1:], x[1:]))
