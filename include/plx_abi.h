@@ -282,7 +282,8 @@ typedef struct plx_prefix {
     int32_t len;
     int32_t n_splits;
 } plx_prefix;
-/* n_splits of plx_prefix and of the problem, for own keys of up to own_len a row.  Pure host arithmetic. */
+/* n_splits of plx_prefix and of the problem, for rows with room for own_len keys of their own (what they hold is on the device).
+ * Pure host arithmetic. */
 int plx_decode_prefix_plan(int32_t batch, int32_t heads_q, int32_t heads_kv, int32_t len, int32_t own_len, int32_t head_dim,
                            int32_t sm_count, int32_t *prefix_splits, int32_t *own_splits);
 /* The same for the call that `p` and `x` describe (their n_splits are not looked at): 0 and the splits of all keys where no shared

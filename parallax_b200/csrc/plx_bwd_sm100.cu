@@ -13,6 +13,11 @@
 //   gl = p (A - t + cs delta), gu = -p delta, W = p (1 + cs); dQ and the gl part of dK carry qk_scale.
 // Evaluated as W = p (1 + bart - S2), gl = W delta + p (b - t) with 1/d1 folded into the exponent.
 //
+// Rounded to 16 bits: gl, gu and W (operands of tensor-core products with k, q, r, dO, which have 16), o and bar v, which the
+// forward left in 16 and from which t and b are formed, and the gradients; all else, sums of chunks among it, has 32.  That makes
+// 1.4 to 1.6 times the error of a rounded result, the same in a simulation in 64 bits with these roundings alone; with o and bar v in
+// 32 it would be 1.41 to 1.45, for two more tensors to store and read.
+//
 // The kernel is persistent: at most one CTA per SM, each walking its share of the work items.
 // Pipeline per CTA (12 warps):
 //   warp 0      TMA producer (resident tiles once per item, streamed tiles through an NS-deep ring)

@@ -1020,6 +1020,9 @@ struct GqaSmem {
 //
 // FRONT: a tile holds keys of one kind, and rows of it that are not visible are zeroed and masked.
 //
+// The weights of V are rounded to its 16 bits, as operands of its products; scores, maxima, sums (of the rounded weights) and
+// records have 32.
+//
 // WARPS per CTA: eight, or one beside the CTAs of another kernel (a.under).
 template <typename T, int D, bool PAGED, bool FEW, int FRONT = kNone, int WARPS = kGqaWarps>
 __global__ void __launch_bounds__(WARPS * 32, 1) decode_gqa_kernel(const DecodeArgs a, int n_hgroups) {
